@@ -240,6 +240,71 @@ int xsg_activate_bwd(int64_t n, const float* scales, const float* opacities, con
                      const float* v_opacities, float* v_log_scales, float* v_opacity_logits,
                      xsg_stream_t stream);
 
+/* ---------------------------------------------------------- training step
+ * Extensions, no reference counterpart: what a training step does behind the frame's backward. Every
+ * call takes a list of tensors (an array on the host, read before the call returns); the lists travel in
+ * the kernels' arguments, so a captured graph holds them by value. Tensors are densely packed in memory.
+ * `mask`, where given, is a packed mask (bit i % 32 of word i / 32, as xsg_packed_visibility_from_radii
+ * and xsg_packed_mask_from_instances write it) over `rows` rows of numel / rows consecutive elements:
+ * elements of rows whose bit is 0 are neither read nor written. No two written arrays may overlap, nor a
+ * written and a read one. Results are the same bits on every call. */
+#define XSG_DTYPE_F32 0
+#define XSG_DTYPE_BF16 1
+#define XSG_DTYPE_F16 2
+
+#define XSG_NORM_INF 0   /* largest magnitude; NaN if any value is */
+#define XSG_NORM_L1 1
+#define XSG_NORM_L2 2
+
+typedef struct {
+    void* data;
+    int64_t numel;
+    const uint32_t* mask;   /* NULL: every row */
+    int64_t rows;           /* rows under the mask (ignored without one) */
+    int dtype;              /* XSG_DTYPE_* */
+} xsg_grad_tensor;
+
+/* total[1]: the norm over all tensors' kept elements (0 of none); each[n], unless NULL: each tensor's
+ * own. Sums are held in 64 bits and rounded once, so a norm overflows only where float32 cannot hold it. */
+size_t xsg_grad_norm_workspace_bytes(const xsg_grad_tensor* tensors, int n);
+int xsg_grad_norm(const xsg_grad_tensor* tensors, int n, int norm, float* total, float* each, void* workspace,
+                  xsg_stream_t stream);
+
+/* Scales the kept elements in place by min(1, max_norm / (norm + eps)), rounded once; a factor of 1 writes
+ * nothing. total[1]: the norm before. A NaN norm makes every kept element NaN, an infinite one zeros them
+ * (and NaN where they are infinite). Workspace as xsg_grad_norm's. */
+int xsg_clip_grads(const xsg_grad_tensor* tensors, int n, int norm, double max_norm, double eps, float* total,
+                   void* workspace, xsg_stream_t stream);
+
+typedef struct {
+    void* param;
+    const void* grad;
+    float* exp_avg;         /* moments are held in 32 bits whatever the parameter's type */
+    float* exp_avg_sq;
+    int64_t numel;
+    const uint32_t* mask;   /* NULL: every row */
+    int64_t rows;
+    double lr, weight_decay;
+    int param_dtype, grad_dtype;
+} xsg_adam_tensor;
+
+typedef struct {
+    double beta1, beta2, eps;
+    int clip;               /* 1: gradients count as scaled by min(1, max_norm / (norm + 1e-6)) */
+    int skip_nonfinite;     /* 1: a norm that is not finite leaves everything, the counter too, as it is */
+    int norm;               /* XSG_NORM_*, with either of the above */
+    double max_norm;
+} xsg_adam_options;
+
+/* One Adam update of the kept elements, with t = step[0] + 1 (the counter, on the device, then holds t):
+ *   g = c grad;  m += (1 - beta1) (g - m);  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * c is the clip factor over all tensors (1 without clip); the gradients are not written. total[1], unless
+ * NULL: the norm before clipping, with clip or skip_nonfinite (else not written, and no workspace needed). */
+size_t xsg_adam_step_workspace_bytes(const xsg_adam_tensor* tensors, int n, const xsg_adam_options* options);
+int xsg_adam_step(const xsg_adam_tensor* tensors, int n, const xsg_adam_options* options, int64_t* step,
+                  float* total, void* workspace, xsg_stream_t stream);
+
 /* ------------------------------------------------------------------ binning */
 int xsg_mask_radii(int64_t n, const uint8_t* mask, float* radii, xsg_stream_t stream);
 int xsg_mask_radii_packed(int64_t n, const uint32_t* packed_mask, float* radii, xsg_stream_t stream);

@@ -2,7 +2,8 @@
 
 ``xsimgs_amd._C`` re-exports the reference's native op names (``xsimgs._C``) over hand-written
 HIP kernels; ``xsimgs_amd.rendering`` and ``xsimgs_amd.cameras`` mirror the reference's Python
-layer (``xsimgs.rendering``, ``xsimgs.cameras.ext``). Importing fails loudly when the native
+layer (``xsimgs.rendering``, ``xsimgs.cameras.ext``); ``xsimgs_amd.optim`` holds the training step
+behind the backward (gradient norm, clipping, Adam under the visibility mask). Importing fails loudly when the native
 libraries have not been built: there is no CPU fallback.
 """
 import os as _os
@@ -16,7 +17,7 @@ except ImportError as _e:  # pragma: no cover - exercised only without a build
         "xsimgs_amd native extension is not built; run `python -c \"import __graft_entry__ as g; g.build()\"` "
         f"from the repository root ({_e})") from _e
 
-from . import rendering, cameras  # noqa: E402,F401
+from . import rendering, cameras, optim  # noqa: E402,F401
 from .rendering import ut_gs_render, ut_gs_tiling, ut_gs_rasterize  # noqa: E402,F401
 from .rendering.sh import *  # noqa: E402,F401,F403
 

@@ -2,9 +2,12 @@
 // xsimgs_amd C-ABI. This file validates and allocates exactly as the reference ops do, then calls
 // the HIP kernels through include/xsimgs_amd.h on the current stream of the input's device.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <algorithm>
+#include <cmath>
 #include <optional>
 #include <string>
 #include <vector>
@@ -593,6 +596,228 @@ std::tuple<Tensor, Tensor> radix_sort_pairs(const Tensor& keys, const Tensor& va
                                           v1.data_ptr<int32_t>(), n, (int)begin_bit, (int)end_bit, ws.data_ptr(),
                                           &sel, stream_of(keys)));
     return sel ? std::make_tuple(k1, v1) : std::make_tuple(k0, v0);
+}
+
+// ------------------------------------------------------------------ training step
+// Extensions: the global gradient norm, clipping by it and the Adam update (optim.hip). Lists of tensors of
+// float32, bfloat16 or float16 on one GPU; masks: empty, or one optional packed mask per tensor over the rows
+// of its first dimension.
+int norm_kind(double norm_type) {
+    if (norm_type == 2.0) return XSG_NORM_L2;
+    if (norm_type == 1.0) return XSG_NORM_L1;
+    TORCH_CHECK(std::isinf(norm_type) && norm_type > 0, "norm_type must be 1, 2 or inf (got ", norm_type, ")");
+    return XSG_NORM_INF;
+}
+
+int dtype_of(const Tensor& t, const char* what, size_t i) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return XSG_DTYPE_F32;
+        case at::kBFloat16: return XSG_DTYPE_BF16;
+        case at::kHalf: return XSG_DTYPE_F16;
+        default:
+            TORCH_CHECK(false, what, " ", i, " must be float32, bfloat16 or float16 (got ", t.scalar_type(), ")");
+    }
+}
+
+void check_listed(const Tensor& t, const at::Device& device, const char* what, size_t i) {
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided, what, " ", i, " must be a strided tensor");
+    TORCH_CHECK(t.is_cuda(), "xsimgs_amd ops take GPU tensors (got ", what, " ", i, " on ", t.device(), ")");
+    TORCH_CHECK(t.device() == device, "All tensors must be on the same device");
+}
+
+// the mask of tensor i, or null
+const uint32_t* mask_of(const std::vector<OptT>& masks, size_t i, const Tensor& t, int64_t* rows) {
+    *rows = 0;
+    if (masks.empty() || !masks[i].has_value()) return nullptr;
+    const Tensor& m = *masks[i];
+    TORCH_CHECK(m.scalar_type() == at::kUInt32 || m.scalar_type() == at::kInt, "Packed mask must be UInt32 tensor");
+    TORCH_CHECK(m.device() == t.device(), "All tensors must be on the same device");
+    TORCH_CHECK(m.is_contiguous(), "All tensors must be contiguous");
+    TORCH_CHECK(t.dim() >= 1, "a masked tensor needs a first dimension of rows (tensor ", i, " has none)");
+    TORCH_CHECK(m.numel() * 32 >= t.size(0), "Packed mask size mismatch with tensor ", i, " of ", t.size(0), " rows");
+    *rows = t.size(0);
+    return (const uint32_t*)m.data_ptr();
+}
+
+// t itself where its elements lie densely (in row order, under a mask), else a dense copy
+Tensor dense_of(const Tensor& t, bool masked) {
+    return (masked ? t.is_contiguous() : t.is_non_overlapping_and_dense()) ? t : t.contiguous();
+}
+
+struct GradArgs {
+    std::vector<Tensor> held;   // what the pointers point into
+    std::vector<xsg_grad_tensor> list;
+};
+
+GradArgs grad_args(const std::vector<Tensor>& tensors, const std::vector<OptT>& masks) {
+    TORCH_CHECK(!tensors.empty(), "an empty list of tensors has no device");
+    TORCH_CHECK(masks.empty() || masks.size() == tensors.size(), "masks must hold one entry per tensor");
+    GradArgs a;
+    a.held.reserve(tensors.size());
+    a.list.resize(tensors.size());
+    for (size_t i = 0; i < tensors.size(); ++i) {
+        const Tensor& t = tensors[i];
+        check_listed(t, tensors[0].device(), "tensor", i);
+        xsg_grad_tensor& x = a.list[i];
+        x.dtype = dtype_of(t, "tensor", i);
+        x.mask = mask_of(masks, i, t, &x.rows);
+        a.held.push_back(dense_of(t, x.mask != nullptr));
+        x.data = a.held[i].data_ptr();
+        x.numel = t.numel();
+    }
+    return a;
+}
+
+// No two written arrays of a call may overlap, nor a written and a read one: the kernels would race.
+struct Span {
+    uintptr_t lo, hi;
+    bool written;
+};
+
+void add_span(std::vector<Span>& spans, const Tensor& t, bool written) {
+    const auto lo = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (t.numel() > 0) spans.push_back({lo, lo + t.numel() * t.element_size(), written});
+}
+
+void check_no_overlap(std::vector<Span>& spans) {
+    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+    uintptr_t any = 0, written = 0;   // ends of what came before
+    for (const Span& s : spans) {
+        TORCH_CHECK(s.lo >= (s.written ? any : written),
+                    "the tensors overlap in memory: each one that is written must be given once");
+        any = std::max(any, s.hi);
+        if (s.written) written = std::max(written, s.hi);
+    }
+}
+
+void mark_written(const Tensor& t) {   // autograd notices what it saved before
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<Tensor, OptT> grad_norm(const std::vector<Tensor>& tensors, double norm_type,
+                                   const std::vector<OptT>& masks, bool per_tensor) {
+    const int kind = norm_kind(norm_type);
+    at::NoGradGuard no_grad;
+    GradArgs a = grad_args(tensors, masks);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(tensors[0].device());
+    const auto opts = tensors[0].options().dtype(at::kFloat);
+    const int n = (int)a.list.size();
+    Tensor total = at::empty({}, opts), each;
+    if (per_tensor) each = at::empty({n}, opts);
+    Tensor ws = workspace(tensors[0], xsg_grad_norm_workspace_bytes(a.list.data(), n));
+    check_rc(xsg_grad_norm(a.list.data(), n, kind, total.data_ptr<float>(),
+                           per_tensor ? each.data_ptr<float>() : nullptr, ws.data_ptr(), stream_of(tensors[0])));
+    return {total, per_tensor ? OptT(each) : OptT()};
+}
+
+Tensor clip_grads_(const std::vector<Tensor>& tensors, double max_norm, double norm_type, double eps,
+                   const std::vector<OptT>& masks) {
+    const int kind = norm_kind(norm_type);
+    at::NoGradGuard no_grad;
+    GradArgs a = grad_args(tensors, masks);
+    std::vector<Span> spans;
+    for (size_t i = 0; i < tensors.size(); ++i) {
+        TORCH_CHECK(at::has_internal_overlap(tensors[i]) != at::MemOverlap::Yes, "tensor ", i,
+                    " has elements that share memory and cannot be scaled in place");
+        if (a.held[i].is_same(tensors[i])) add_span(spans, tensors[i], true);
+    }
+    check_no_overlap(spans);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(tensors[0].device());
+    Tensor total = at::empty({}, tensors[0].options().dtype(at::kFloat));
+    const int n = (int)a.list.size();
+    Tensor ws = workspace(tensors[0], xsg_grad_norm_workspace_bytes(a.list.data(), n));
+    check_rc(xsg_clip_grads(a.list.data(), n, kind, max_norm, eps, total.data_ptr<float>(), ws.data_ptr(),
+                            stream_of(tensors[0])));
+    for (size_t i = 0; i < tensors.size(); ++i) {
+        if (a.held[i].is_same(tensors[i])) mark_written(tensors[i]);
+        else tensors[i].copy_(a.held[i]);
+    }
+    return total;
+}
+
+bool same_layout(const Tensor& a, const Tensor& b) {
+    return a.sizes() == b.sizes() && (a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()));
+}
+
+OptT adam_step_(const std::vector<Tensor>& params, const std::vector<Tensor>& grads,
+                const std::vector<Tensor>& exp_avgs, const std::vector<Tensor>& exp_avg_sqs, const Tensor& step,
+                const std::vector<double>& lr, const std::vector<double>& weight_decay, double beta1, double beta2,
+                double eps, const std::optional<double>& max_norm, double norm_type, bool skip_nonfinite,
+                const std::vector<OptT>& masks) {
+    const size_t n = params.size();
+    TORCH_CHECK(n > 0, "an empty list of tensors has no device");
+    TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && lr.size() == n &&
+                    weight_decay.size() == n && (masks.empty() || masks.size() == n),
+                "params, grads, exp_avgs, exp_avg_sqs, lr, weight_decay and masks must hold one entry per tensor");
+    xsg_adam_options o{};
+    o.beta1 = beta1;
+    o.beta2 = beta2;
+    o.eps = eps;
+    o.clip = max_norm.has_value();
+    o.max_norm = max_norm.value_or(0.0);
+    o.skip_nonfinite = skip_nonfinite;
+    o.norm = norm_kind(norm_type);
+    const at::Device device = params[0].device();
+    TORCH_CHECK(step.scalar_type() == at::kLong && step.numel() == 1 && step.device() == device,
+                "step must be one int64 value on the parameters' device");
+    at::NoGradGuard no_grad;
+    std::vector<xsg_adam_tensor> list(n);
+    std::vector<Tensor> held;
+    std::vector<Span> spans;
+    spans.reserve(4 * n + 1);
+    add_span(spans, step, true);
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor &p = params[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
+        Tensor g = grads[i];
+        check_listed(p, device, "parameter", i);
+        check_listed(g, device, "gradient", i);
+        check_listed(m, device, "exp_avg", i);
+        check_listed(v, device, "exp_avg_sq", i);
+        xsg_adam_tensor& x = list[i];
+        x.param_dtype = dtype_of(p, "parameter", i);
+        x.grad_dtype = dtype_of(g, "gradient", i);
+        x.mask = mask_of(masks, i, p, &x.rows);
+        TORCH_CHECK(x.mask ? p.is_contiguous() : p.is_non_overlapping_and_dense(), "parameter ", i, " must be ",
+                    x.mask ? "contiguous under a mask" : "dense in memory");
+        TORCH_CHECK(m.scalar_type() == at::kFloat && v.scalar_type() == at::kFloat, "moments ", i,
+                    " must be float32 tensors");
+        TORCH_CHECK(same_layout(m, p) && same_layout(v, p), "moments ", i,
+                    " must have their parameter's sizes and strides");
+        TORCH_CHECK(g.sizes() == p.sizes(), "gradient ", i, " must have its parameter's sizes");
+        if (!same_layout(g, p)) {
+            g = at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g);
+            held.push_back(g);
+        }
+        x.param = p.data_ptr();
+        x.grad = g.data_ptr();
+        x.exp_avg = m.data_ptr<float>();
+        x.exp_avg_sq = v.data_ptr<float>();
+        x.numel = p.numel();
+        x.lr = lr[i];
+        x.weight_decay = weight_decay[i];
+        add_span(spans, p, true);
+        add_span(spans, m, true);
+        add_span(spans, v, true);
+        add_span(spans, g, false);
+    }
+    check_no_overlap(spans);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
+    const bool normed = o.clip || o.skip_nonfinite;
+    Tensor total, ws;
+    if (normed) {
+        total = at::empty({}, params[0].options().dtype(at::kFloat));
+        ws = workspace(params[0], xsg_adam_step_workspace_bytes(list.data(), (int)n, &o));
+    }
+    check_rc(xsg_adam_step(list.data(), (int)n, &o, step.data_ptr<int64_t>(),
+                           normed ? total.data_ptr<float>() : nullptr, normed ? ws.data_ptr() : nullptr,
+                           stream_of(params[0])));
+    for (size_t i = 0; i < n; ++i) {
+        mark_written(params[i]);
+        mark_written(exp_avgs[i]);
+        mark_written(exp_avg_sqs[i]);
+    }
+    mark_written(step);
+    return normed ? OptT(total) : OptT();
 }
 
 // ------------------------------------------------------------------ scene-assembly producers
@@ -1264,6 +1489,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     // extension: the visibility mask of the regular tilings' Gaussians (an SH mask)
     m.def("packed_visibility_mask", &packed_visibility_mask, py::arg("radii"));
     // extension: the caller's parameter activations and their gradients
+    m.def("grad_norm", &grad_norm, py::arg("tensors"), py::arg("norm_type"), py::arg("masks"), py::arg("per_tensor"));
+    m.def("clip_grads_", &clip_grads_, py::arg("tensors"), py::arg("max_norm"), py::arg("norm_type"), py::arg("eps"),
+          py::arg("masks"));
+    m.def("adam_step_", &adam_step_, py::arg("params"), py::arg("grads"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"),
+          py::arg("step"), py::arg("lr"), py::arg("weight_decay"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
+          py::arg("max_norm"), py::arg("norm_type"), py::arg("skip_nonfinite"), py::arg("masks"));
     m.def("activate_fwd", &activate_fwd, py::arg("log_scales"), py::arg("opacity_logits"));
     m.def("activate_bwd", &activate_bwd, py::arg("scales"), py::arg("opacities"), py::arg("v_scales"),
           py::arg("v_opacities"));

@@ -18,6 +18,7 @@ import torch
 
 from . import cameras as C
 from ._C import isect_regular_tiles_batched, packed_visibility_mask
+from .optim import Adam
 from .rendering.activate import activate_gaussians
 from .rendering.rasterize import ut_gs_rasterize, ut_gs_rasterize_batched
 from .rendering.render import ut_gs_tiling
@@ -186,6 +187,37 @@ def _colors(st: FrameState, origin, radii=None):
         return st.colors
     mask = packed_visibility_mask(radii.detach().contiguous()) if radii is not None else None
     return spherical_harmonics_fused(st.sh, st.means, origin, st.scene.sh_degree, mask=mask)
+
+
+# learning rates of a scene's parameters (the SH rate serves fixed colours too)
+RATES = dict(means=1.6e-4, quats=1e-3, log_scales=5e-3, opacity_logits=5e-2, sh=2.5e-3, colors=2.5e-3)
+
+
+def make_optimizer(st: FrameState, rates=None, **kw) -> Adam:
+    """An Adam over the scene's parameters, one group for each with its own rate; ``kw``: max_norm,
+    skip_nonfinite and the other arguments of ``optim.Adam``."""
+    rates = dict(RATES, **(rates or {}))
+    return Adam([dict(params=[getattr(st, k)], lr=r, name=k) for k, r in rates.items() if getattr(st, k) is not None],
+                **kw)
+
+
+def train_frame(st: FrameState, optimizer: Adam, grads, cam_index: int = 0, rig: bool = False) -> dict:
+    """One training step: the frame (of one camera, or of the whole rig) forward and backward, then the
+    optimizer's update with whatever clipping it carries. In a regular tiling only the Gaussians that some
+    tile can hold are updated (their packed mask from the projection's radii; the others' gradients are
+    zeros, their momentum rests). Returns the frame's outputs and ``grad_norm`` before clipping."""
+    zero_grads(st)
+    if rig:
+        out = render_rig(st, backward=True, grads=grads)
+    else:
+        out = render_frame(st, backward=True, grads=grads, cam_index=cam_index)
+    masks = None
+    if rig or st.scene.cameras[cam_index].kind in REGULAR_TILING:
+        mask = packed_visibility_mask(out["radii"].detach().contiguous())
+        masks = {p: mask for group in optimizer.param_groups for p in group["params"] if p.shape[0] == st.scene.n}
+    optimizer.step(masks=masks)
+    out["grad_norm"] = optimizer.grad_norm
+    return out
 
 
 def zero_grads(st: FrameState) -> None:

@@ -1,0 +1,105 @@
+"""Adam over many tensors in a few launches: decoupled weight decay, clipping by the global norm fused in (the
+factor stays on the GPU and the gradients are not rewritten), and the renderer's packed visibility mask, under
+which Gaussians out of view keep their parameters and moments. Moments are float32 whatever the parameter's
+type; the step counter lives on the GPU, so a step can be captured in a graph and replayed."""
+import torch
+
+from .. import _C
+from .clip import listed_masks
+
+
+def _per_tensor(value, n: int, name: str) -> list:
+    if isinstance(value, (int, float)):
+        return [float(value)] * n
+    value = [float(v) for v in value]
+    if len(value) != n:
+        raise ValueError(f"{name} must be a number or hold one per tensor: {len(value)} for {n}")
+    return value
+
+
+def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay=0.0, max_norm: float | None = None, norm_type: float = 2.0,
+               skip_nonfinite: bool = False, masks=None):
+    """One update in place; with t = step + 1 and c = min(1, max_norm / (norm of all grads + 1e-6)) (1 without
+    ``max_norm``):
+
+        m += (1 - beta1) (c g - m);  v = beta2 v + (1 - beta2) (c g)^2
+        p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+
+    ``step``: one int64 value on the GPU, which then holds t. ``lr`` and ``weight_decay``: a number, or one per
+    tensor. ``masks`` as in ``grad_norm`` (rows out of the mask do not change, and do not count in the norm).
+    ``skip_nonfinite``: a norm that is not finite leaves everything as it is, ``step`` too. Returns the norm
+    before clipping (with ``max_norm`` or ``skip_nonfinite``, else None). Parameters and gradients are float32,
+    bfloat16 or float16; moments are float32 tensors of their parameter's sizes and strides."""
+    params = list(params)
+    n = len(params)
+    return _C.adam_step_(params, list(grads), list(exp_avgs), list(exp_avg_sqs), step, _per_tensor(lr, n, "lr"),
+                         _per_tensor(weight_decay, n, "weight_decay"), float(betas[0]), float(betas[1]), float(eps),
+                         None if max_norm is None else float(max_norm), float(norm_type), bool(skip_nonfinite),
+                         listed_masks(masks, n))
+
+
+class Adam(torch.optim.Optimizer):
+    """Adam over ``adam_step_``. Groups carry their own ``lr`` and ``weight_decay``; betas, eps, ``max_norm``,
+    ``norm_type`` and ``skip_nonfinite`` hold for the whole optimizer, whose tensors are one list with one norm
+    and one step counter (a parameter without a gradient sits a step out; bias correction goes by the
+    optimizer's count). ``grad_norm`` is the last step's norm before clipping, or None."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-15, weight_decay: float = 0.0, *,
+                 max_norm: float | None = None, norm_type: float = 2.0, skip_nonfinite: bool = False):
+        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError("lr, eps and weight_decay must not be negative, betas must lie in [0, 1)")
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay))
+        self.betas, self.eps = tuple(betas), eps
+        self.max_norm, self.norm_type, self.skip_nonfinite = max_norm, norm_type, skip_nonfinite
+        self.step_count = None   # int64 [1] on the parameters' GPU, from the first step on
+        self.grad_norm = None
+
+    def add_param_group(self, param_group):
+        if shared := {"betas", "eps", "max_norm", "norm_type", "skip_nonfinite"} & set(param_group):
+            raise ValueError(f"{sorted(shared)} hold for the whole optimizer; a group may set lr and weight_decay")
+        super().add_param_group(param_group)
+
+    @torch.no_grad()
+    def step(self, closure=None, *, masks=None):
+        """``masks``: a dict from parameters to their packed masks, for those that have one."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params, lr, decay = [], [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is not None:
+                    params.append(p)
+                    lr.append(float(group["lr"]))
+                    decay.append(float(group["weight_decay"]))
+        self.grad_norm = None
+        if not params:
+            return loss
+        for p in params:
+            if not self.state[p]:
+                self.state[p]["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+                self.state[p]["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        if self.step_count is None:
+            self.step_count = torch.zeros(1, dtype=torch.int64, device=params[0].device)
+        self.grad_norm = adam_step_(params, [p.grad for p in params], [self.state[p]["exp_avg"] for p in params],
+                                    [self.state[p]["exp_avg_sq"] for p in params], self.step_count, lr=lr,
+                                    betas=self.betas, eps=self.eps, weight_decay=decay, max_norm=self.max_norm,
+                                    norm_type=self.norm_type, skip_nonfinite=self.skip_nonfinite,
+                                    masks=None if masks is None else [masks.get(p) for p in params])
+        return loss
+
+    def state_dict(self):
+        return dict(super().state_dict(), step=None if self.step_count is None else self.step_count.clone())
+
+    def load_state_dict(self, state_dict):
+        """The moments come back in float32 (the base class would give them their parameter's type)."""
+        super().load_state_dict({k: v for k, v in state_dict.items() if k != "step"})
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            for k, v in state_dict["state"].get(i, {}).items():
+                self.state[p][k] = torch.empty_like(p, dtype=torch.float32).copy_(v)
+        step = state_dict.get("step")
+        self.step_count = None if step is None else step.detach().clone().to(params[0].device)
