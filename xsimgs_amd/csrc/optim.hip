@@ -20,18 +20,25 @@ constexpr int64_t kTargetChunks = 2048;   // chunks of a call, when its tensors 
 constexpr int64_t kMaxChunk = 1 << 30;    // offsets inside a chunk are 32-bit
 constexpr int64_t kMaxRow = 1 << 30;      // and so are rows under a mask
 constexpr int64_t kMaxElements = (int64_t)1 << 48;
-constexpr int kListMax = 112;             // gradient tensors to a launch
-constexpr int kAdamMax = 52;              // tensors with their states to a launch
+constexpr int kListMax = 96;             // gradient tensors to a launch
+constexpr int kAdamMax = 48;              // tensors with their states to a launch
+
+// Division of n < 2^31 by the row length: (mulhi(n, magic) + n) >> shift
+struct RowDiv {
+    uint32_t row, magic;
+    uint32_t shift;
+};
 
 struct GradList {
     void* data[kListMax];
     int64_t numel[kListMax];
     const uint32_t* mask[kListMax];
-    int32_t row[kListMax];        // elements to a mask bit
-    int32_t first[kListMax + 1];  // first chunk of each tensor in this launch
+    uint32_t row[kListMax], magic[kListMax];  // elements to a mask bit, and its division
+    int32_t first[kListMax + 1];              // first chunk of each tensor in this launch
+    uint8_t shift[kListMax];
     uint8_t dtype[kListMax];
     int32_t n;
-    int64_t chunk;
+    int32_t chunk;
 };
 static_assert(sizeof(GradList) <= 3900, "the list and the other arguments share 4 KB");
 
@@ -42,40 +49,100 @@ struct AdamList {
     float* sq[kAdamMax];
     int64_t numel[kAdamMax];
     const uint32_t* mask[kAdamMax];
-    int32_t row[kAdamMax];
+    uint32_t row[kAdamMax], magic[kAdamMax];
     int32_t first[kAdamMax + 1];
     float lr[kAdamMax];
     float keep[kAdamMax];         // 1 - lr * weight decay
-    uint8_t pdtype[kAdamMax], gdtype[kAdamMax];
+    uint8_t shift[kAdamMax], pdtype[kAdamMax], gdtype[kAdamMax];
     int32_t n;
-    int64_t chunk;
+    int32_t chunk;
 };
 static_assert(sizeof(AdamList) <= 3900, "the list and the other arguments share 4 KB");
 
-XSG_DEV float load_as_float(const void* p, int64_t i, int dtype) {
-    if (dtype == XSG_DTYPE_F32) return ((const float*)p)[i];
-    if (dtype == XSG_DTYPE_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
+// round to nearest even; a NaN stays one
+XSG_DEV uint32_t bf16_bits(float x) {
+    const uint32_t u = __float_as_uint(x);
+    if (x != x) return (u >> 16) | 0x40u;
+    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+}
+
+// Elements of one type, one at a time or four at a time from a place aligned for that (16 bytes of float32, 8
+// of the others).
+template <int DT> XSG_DEV float load1(const void* p, uint32_t i) {
+    if (DT == XSG_DTYPE_F32) return ((const float*)p)[i];
+    if (DT == XSG_DTYPE_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
     return (float)((const _Float16*)p)[i];
 }
-
-// round to nearest even; a NaN stays one
-XSG_DEV uint16_t bf16_bits(float x) {
-    const uint32_t u = __float_as_uint(x);
-    if (x != x) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
-
-XSG_DEV void store_from_float(void* p, int64_t i, int dtype, float x) {
-    if (dtype == XSG_DTYPE_F32) ((float*)p)[i] = x;
-    else if (dtype == XSG_DTYPE_BF16) ((uint16_t*)p)[i] = bf16_bits(x);
+template <int DT> XSG_DEV void store1(void* p, uint32_t i, float x) {
+    if (DT == XSG_DTYPE_F32) ((float*)p)[i] = x;
+    else if (DT == XSG_DTYPE_BF16) ((uint16_t*)p)[i] = (uint16_t)bf16_bits(x);
     else ((_Float16*)p)[i] = (_Float16)x;
 }
-
-XSG_DEV bool in_mask(const uint32_t* mask, int64_t i, int32_t row) {
-    if (!mask) return true;
-    const int64_t r = i / row;
-    return (mask[r >> 5] >> (r & 31)) & 1u;
+template <int DT> XSG_DEV float4 load4(const void* p, uint32_t i) {
+    if (DT == XSG_DTYPE_F32) return *reinterpret_cast<const float4*>((const float*)p + i);
+    const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*)p + i);
+    if (DT == XSG_DTYPE_BF16)
+        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
+                           __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+    union { uint2 u; _Float16 h[4]; } c{u};
+    return make_float4((float)c.h[0], (float)c.h[1], (float)c.h[2], (float)c.h[3]);
 }
+template <int DT> XSG_DEV void store4(void* p, uint32_t i, float4 x) {
+    if (DT == XSG_DTYPE_F32) {
+        *reinterpret_cast<float4*>((float*)p + i) = x;
+    } else if (DT == XSG_DTYPE_BF16) {
+        *reinterpret_cast<uint2*>((uint16_t*)p + i) =
+            make_uint2(bf16_bits(x.x) | bf16_bits(x.y) << 16, bf16_bits(x.z) | bf16_bits(x.w) << 16);
+    } else {
+        union { uint2 u; _Float16 h[4]; } c;
+        c.h[0] = (_Float16)x.x; c.h[1] = (_Float16)x.y; c.h[2] = (_Float16)x.z; c.h[3] = (_Float16)x.w;
+        *reinterpret_cast<uint2*>((uint16_t*)p + i) = c.u;
+    }
+}
+XSG_HD uint32_t type_size(int dtype) { return dtype == XSG_DTYPE_F32 ? 4 : 2; }
+XSG_DEV const void* at(const void* p, int64_t i, int dtype) { return (const char*)p + i * type_size(dtype); }
+XSG_DEV void* at(void* p, int64_t i, int dtype) { return (char*)p + i * type_size(dtype); }
+
+// Elements before p is aligned for four of its type at once (0 to 3).
+XSG_DEV uint32_t phase_of(const void* p, int dtype) {
+    const uint32_t e = (uint32_t)((uintptr_t)p / type_size(dtype)) & 3u;
+    return (4u - e) & 3u;
+}
+
+// The packed mask seen from one chunk: element i of the chunk lies in row (rem + i) / row after word `words`
+// and bit `bit`.
+struct ChunkMask {
+    const uint32_t* words;
+    uint32_t bit, rem, row, magic, shift;
+
+    XSG_DEV void open(const uint32_t* mask, int64_t base, uint32_t row_, uint32_t magic_, uint32_t shift_) {
+        const int64_t r = base / row_;
+        words = mask + (r >> 5);
+        bit = (uint32_t)(r & 31);
+        rem = (uint32_t)(base - r * row_);
+        row = row_;
+        magic = magic_;
+        shift = shift_;
+    }
+    XSG_DEV uint32_t quotient(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
+    XSG_DEV bool one(uint32_t i) const {
+        const uint32_t r = bit + quotient(rem + i);
+        return (words[r >> 5] >> (r & 31)) & 1u;
+    }
+    // bit k: element i + k; all four lie in the chunk. Their rows span at most two words.
+    XSG_DEV uint32_t four(uint32_t i) const {
+        const uint32_t n = rem + i, q = quotient(n), r0 = bit + q;
+        const uint32_t r3 = bit + quotient(n + 3);
+        const uint64_t w = (uint64_t)words[r0 >> 5] | (uint64_t)words[r3 >> 5] << 32;
+        uint32_t at = n - q * row, r = r0 & 31, keep = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            keep |= (uint32_t)((w >> r) & 1u) << k;
+            if (++at == row) { at = 0; ++r; }
+        }
+        return keep;
+    }
+};
 
 // the tensor whose chunks hold chunk b: the last one with first[t] <= b (empty tensors have no chunk)
 XSG_DEV int find_tensor(const int32_t* first, int n, int b) {
@@ -87,51 +154,130 @@ XSG_DEV int find_tensor(const int32_t* first, int n, int b) {
     return lo;
 }
 
-// Accumulation of one kind of norm in 64 bits: squares of any float32 stay finite and above zero there. A
-// maximum keeps a NaN once it has seen one.
-template <int NORM> XSG_DEV double norm_add(double acc, double x) {
-    if (NORM == XSG_NORM_L2) return acc + x * x;
-    if (NORM == XSG_NORM_L1) return acc + fabs(x);
-    x = fabs(x);
-    return (x > acc || x != x) ? x : acc;
-}
-template <int NORM> XSG_DEV double norm_join(double a, double b) {
-    if (NORM == XSG_NORM_INF) return (b > a || b != b) ? b : a;
-    return a + b;
-}
-template <int NORM> XSG_DEV double norm_finish(double a) { return NORM == XSG_NORM_L2 ? sqrt(a) : a; }
+// Accumulation of one kind of norm. Sums are in 64 bits, where squares of any float32 stay finite and above
+// zero. The largest magnitude is the largest of the values' bits without their sign, where a NaN is above
+// infinity and so stays.
+template <int NORM> struct Accum {
+    double sum = 0.0;
+    XSG_DEV void add(float x) {
+        const double d = x;
+        if (NORM == XSG_NORM_L2) sum = fma(d, d, sum);
+        else sum += fabs(d);
+    }
+    XSG_DEV void join(const Accum& o) { sum += o.sum; }
+    XSG_DEV double value() const { return sum; }
+    XSG_DEV void join_value(double v) { sum += v; }
+    XSG_DEV Accum shuffled(int d) const { Accum a; a.sum = __shfl_xor(sum, d); return a; }
+    XSG_DEV double finish() const { return NORM == XSG_NORM_L2 ? sqrt(sum) : sum; }
+};
+template <> struct Accum<XSG_NORM_INF> {
+    uint32_t bits = 0;
+    XSG_DEV void add(float x) { bits = max(bits, __float_as_uint(x) & 0x7fffffffu); }
+    XSG_DEV void join(const Accum& o) { bits = max(bits, o.bits); }
+    XSG_DEV double value() const { return __uint_as_float(bits); }
+    XSG_DEV void join_value(double v) { add((float)v); }
+    XSG_DEV Accum shuffled(int d) const { Accum a; a.bits = __shfl_xor(bits, d); return a; }
+    XSG_DEV double finish() const { return value(); }
+};
 
 // The workgroup's joined value, in every thread; the order is fixed.
-template <int NORM> XSG_DEV double block_join(double v) {
+template <int NORM> XSG_DEV Accum<NORM> block_join(Accum<NORM> v) {
     __shared__ double part[kBlock / 64];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v = norm_join<NORM>(v, __shfl_xor(v, d));
+    for (int d = 32; d > 0; d >>= 1) v.join(v.shuffled(d));
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v.value();
     __syncthreads();
-    v = part[0];
+    Accum<NORM> all;
 #pragma unroll
-    for (int w = 1; w < kBlock / 64; ++w) v = norm_join<NORM>(v, part[w]);
-    return v;
+    for (int w = 0; w < kBlock / 64; ++w) all.join_value(part[w]);
+    return all;
+}
+
+// A chunk's elements: `head` single ones up to the first aligned group of four, `groups` groups, `tail`
+// single ones. Bodies take (first element, group in mask bits or 15).
+struct ChunkSpan {
+    uint32_t head, groups, tail;
+    XSG_DEV ChunkSpan(uint32_t count, uint32_t phase) {
+        head = min(phase, count);
+        groups = (count - head) >> 2;
+        tail = (count - head) & 3u;
+    }
+    XSG_DEV uint32_t tail_at() const { return head + 4 * groups; }
+};
+
+constexpr int kUnroll = 4;   // groups in flight per thread
+
+// one(i): a single element; many(i[], keep[]): kUnroll groups, of which those with keep 0 are left out
+template <bool MASK, typename One, typename Many>
+XSG_DEV void for_chunk(const ChunkSpan& span, const ChunkMask& mask, One&& one, Many&& many) {
+    for (uint32_t g = threadIdx.x; g < span.groups; g += kBlock * kUnroll) {
+        uint32_t i[kUnroll], keep[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            i[u] = span.head + 4 * (g + u * kBlock);
+            keep[u] = g + u * kBlock < span.groups ? (MASK ? mask.four(i[u]) : 15u) : 0u;
+        }
+        many(i, keep);
+    }
+    if (threadIdx.x < span.head && (!MASK || mask.one(threadIdx.x))) one(threadIdx.x);
+    const uint32_t i = span.tail_at() + threadIdx.x;
+    if (threadIdx.x < span.tail && (!MASK || mask.one(i))) one(i);
+}
+
+template <int NORM, int DT, bool MASK>
+XSG_DEV Accum<NORM> chunk_norm(const void* p, const ChunkSpan& span, const ChunkMask& mask) {
+    Accum<NORM> acc[kUnroll];
+    for_chunk<MASK>(span, mask, [&](uint32_t i) { acc[0].add(load1<DT>(p, i)); },
+                    [&](const uint32_t* i, const uint32_t* keep) {
+        float4 x[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) x[u] = keep[u] ? load4<DT>(p, i[u]) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            acc[u].add(!MASK || (keep[u] & 1) ? x[u].x : 0.f);
+            acc[u].add(!MASK || (keep[u] & 2) ? x[u].y : 0.f);
+            acc[u].add(!MASK || (keep[u] & 4) ? x[u].z : 0.f);
+            acc[u].add(!MASK || (keep[u] & 8) ? x[u].w : 0.f);
+        }
+    });
+#pragma unroll
+    for (int u = 1; u < kUnroll; ++u) acc[0].join(acc[u]);
+    return acc[0];
+}
+
+// calls f with the type, and with whether there is a mask, as constants
+template <typename F> XSG_DEV void with_type(int dtype, F&& f) {
+    if (dtype == XSG_DTYPE_F32) f(std::integral_constant<int, XSG_DTYPE_F32>{});
+    else if (dtype == XSG_DTYPE_BF16) f(std::integral_constant<int, XSG_DTYPE_BF16>{});
+    else f(std::integral_constant<int, XSG_DTYPE_F16>{});
+}
+template <typename F> XSG_DEV void with_mask(bool masked, F&& f) {
+    if (masked) f(std::true_type{});
+    else f(std::false_type{});
 }
 
 template <int NORM>
 __global__ __launch_bounds__(kBlock) void norm_partial_kernel(GradList list, double* __restrict__ partial) {
-    const int b = blockIdx.x, t = find_tensor(list.first, list.n, b);
+    const int b = blockIdx.x, t = find_tensor(list.first, list.n, b), dtype = list.dtype[t];
     const int64_t base = (int64_t)(b - list.first[t]) * list.chunk;
-    const int64_t end = min(base + list.chunk, list.numel[t]);
-    double acc = 0.0;
-    for (int64_t i = base + threadIdx.x; i < end; i += kBlock)
-        if (in_mask(list.mask[t], i, list.row[t]))
-            acc = norm_add<NORM>(acc, load_as_float(list.data[t], i, list.dtype[t]));
+    const uint32_t count = (uint32_t)min((int64_t)list.chunk, list.numel[t] - base);
+    const void* p = at((const void*)list.data[t], base, dtype);
+    const ChunkSpan span(count, phase_of(p, dtype));
+    ChunkMask mask;
+    if (list.mask[t]) mask.open(list.mask[t], base, list.row[t], list.magic[t], list.shift[t]);
+    Accum<NORM> acc;
+    with_type(dtype, [&](auto dt) {
+        with_mask(list.mask[t] != nullptr, [&](auto m) { acc = chunk_norm<NORM, dt.value, m.value>(p, span, mask); });
+    });
     acc = block_join<NORM>(acc);
-    if (threadIdx.x == 0) partial[b] = acc;
+    if (threadIdx.x == 0) partial[b] = acc.value();
 }
 
 template <int NORM> XSG_DEV double join_partials(const double* __restrict__ partial, int n) {
-    double acc = 0.0;
-    for (int i = threadIdx.x; i < n; i += kBlock) acc = norm_join<NORM>(acc, partial[i]);
-    return block_join<NORM>(acc);
+    Accum<NORM> acc;
+    for (int i = threadIdx.x; i < n; i += kBlock) acc.join_value(partial[i]);
+    return block_join<NORM>(acc).finish();
 }
 
 // Block 0: the norm over every chunk of the call, to `total` (float32) and `sum` (64 bits).
@@ -142,7 +288,7 @@ __global__ __launch_bounds__(kBlock) void norm_finish_kernel(GradList list, cons
                                                              float* __restrict__ total, double* __restrict__ sum,
                                                              float* __restrict__ each) {
     if (blockIdx.x == 0) {
-        const double v = norm_finish<NORM>(join_partials<NORM>(all, n_all));
+        const double v = join_partials<NORM>(all, n_all);
         if (threadIdx.x == 0) {
             if (total) *total = (float)v;
             *sum = v;
@@ -150,7 +296,7 @@ __global__ __launch_bounds__(kBlock) void norm_finish_kernel(GradList list, cons
     } else {
         const int t = blockIdx.x - 1;
         const int lo = list.first[t], hi = list.first[t + 1];
-        const double v = norm_finish<NORM>(join_partials<NORM>(partial + lo, hi - lo));
+        const double v = join_partials<NORM>(partial + lo, hi - lo);
         if (threadIdx.x == 0) each[t] = (float)v;
     }
 }
@@ -161,21 +307,48 @@ XSG_DEV float clip_factor(double norm, double max_norm, double eps) {
     return c > 1.0 ? 1.0f : (float)c;
 }
 
+template <int DT, bool MASK>
+XSG_DEV void chunk_scale(void* p, float c, const ChunkSpan& span, const ChunkMask& mask) {
+    for_chunk<MASK>(span, mask, [&](uint32_t i) { store1<DT>(p, i, load1<DT>(p, i) * c); },
+                    [&](const uint32_t* i, const uint32_t* keep) {
+        float4 x[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (keep[u]) x[u] = load4<DT>(p, i[u]);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const float4 y = make_float4(x[u].x * c, x[u].y * c, x[u].z * c, x[u].w * c);
+            if (keep[u] == 15u) {
+                store4<DT>(p, i[u], y);
+            } else if (keep[u]) {
+                if (keep[u] & 1) store1<DT>(p, i[u], y.x);
+                if (keep[u] & 2) store1<DT>(p, i[u] + 1, y.y);
+                if (keep[u] & 4) store1<DT>(p, i[u] + 2, y.z);
+                if (keep[u] & 8) store1<DT>(p, i[u] + 3, y.w);
+            }
+        }
+    });
+}
+
 __global__ __launch_bounds__(kBlock) void clip_scale_kernel(GradList list, const double* __restrict__ norm,
                                                             double max_norm, double eps) {
     const float c = clip_factor(*norm, max_norm, eps);
     if (c == 1.0f) return;   // the values stay as they are
-    const int b = blockIdx.x, t = find_tensor(list.first, list.n, b);
+    const int b = blockIdx.x, t = find_tensor(list.first, list.n, b), dtype = list.dtype[t];
     const int64_t base = (int64_t)(b - list.first[t]) * list.chunk;
-    const int64_t end = min(base + list.chunk, list.numel[t]);
-    for (int64_t i = base + threadIdx.x; i < end; i += kBlock)
-        if (in_mask(list.mask[t], i, list.row[t]))
-            store_from_float(list.data[t], i, list.dtype[t], load_as_float(list.data[t], i, list.dtype[t]) * c);
+    const uint32_t count = (uint32_t)min((int64_t)list.chunk, list.numel[t] - base);
+    void* p = at(list.data[t], base, dtype);
+    const ChunkSpan span(count, phase_of(p, dtype));
+    ChunkMask mask;
+    if (list.mask[t]) mask.open(list.mask[t], base, list.row[t], list.magic[t], list.shift[t]);
+    with_type(dtype, [&](auto dt) {
+        with_mask(list.mask[t] != nullptr, [&](auto m) { chunk_scale<dt.value, m.value>(p, c, span, mask); });
+    });
 }
 
 struct AdamScalars {
     double log_beta1, log_beta2;   // natural logarithms
-    float beta1, beta2, one_minus_beta1, one_minus_beta2, eps;
+    float beta2, one_minus_beta1, one_minus_beta2, eps;
     int clip, skip_nonfinite;
     double max_norm;
 };
@@ -184,9 +357,85 @@ constexpr double kAdamClipEps = 1e-6;
 // The step counter counts this step; adam_kernel takes it back where the step is not taken.
 __global__ void adam_count_kernel(int64_t* step) { *step += 1; }
 
+// One value of the update; rate: lr / (1 - beta1^t), root: 1 / sqrt(1 - beta2^t)
+struct AdamTerms {
+    float beta2, one_minus_beta1, one_minus_beta2, eps, c, rate, root, keep;
+    XSG_DEV void update(float& p, float g, float& m, float& v) const {
+        g *= c;
+        m += one_minus_beta1 * (g - m);
+        v = beta2 * v + one_minus_beta2 * g * g;
+        p = p * keep - rate * m / (sqrtf(v) * root + eps);
+    }
+};
+
+struct AdamArrays {
+    void* p;
+    const void* g;
+    float *m, *v;
+};
+
+template <int PT, int GT> XSG_DEV void adam_one(const AdamArrays& a, const AdamTerms& s, uint32_t i) {
+    float p = load1<PT>(a.p, i), m = a.m[i], v = a.v[i];
+    s.update(p, load1<GT>(a.g, i), m, v);
+    store1<PT>(a.p, i, p);
+    a.m[i] = m;
+    a.v[i] = v;
+}
+
+constexpr int kAdamUnroll = 2;
+
+template <int PT, int GT, bool MASK>
+XSG_DEV void chunk_adam(const AdamArrays& a, const AdamTerms& s, const ChunkSpan& span, const ChunkMask& mask) {
+    for (uint32_t g0 = threadIdx.x; g0 < span.groups; g0 += kBlock * kAdamUnroll) {
+        uint32_t i[kAdamUnroll], keep[kAdamUnroll];
+        float4 p[kAdamUnroll], g[kAdamUnroll], m[kAdamUnroll], v[kAdamUnroll];
+#pragma unroll
+        for (int u = 0; u < kAdamUnroll; ++u) {
+            i[u] = span.head + 4 * (g0 + u * kBlock);
+            keep[u] = g0 + u * kBlock < span.groups ? (MASK ? mask.four(i[u]) : 15u) : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < kAdamUnroll; ++u) {
+            if (keep[u]) {
+                p[u] = load4<PT>(a.p, i[u]);
+                g[u] = load4<GT>(a.g, i[u]);
+                m[u] = load4<XSG_DTYPE_F32>(a.m, i[u]);
+                v[u] = load4<XSG_DTYPE_F32>(a.v, i[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAdamUnroll; ++u) {
+            if (!keep[u]) continue;
+            s.update(p[u].x, g[u].x, m[u].x, v[u].x);
+            s.update(p[u].y, g[u].y, m[u].y, v[u].y);
+            s.update(p[u].z, g[u].z, m[u].z, v[u].z);
+            s.update(p[u].w, g[u].w, m[u].w, v[u].w);
+            if (keep[u] == 15u) {
+                store4<PT>(a.p, i[u], p[u]);
+                store4<XSG_DTYPE_F32>(a.m, i[u], m[u]);
+                store4<XSG_DTYPE_F32>(a.v, i[u], v[u]);
+            } else {
+                const float pe[4] = {p[u].x, p[u].y, p[u].z, p[u].w}, me[4] = {m[u].x, m[u].y, m[u].z, m[u].w},
+                            ve[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (!((keep[u] >> k) & 1)) continue;
+                    store1<PT>(a.p, i[u] + k, pe[k]);
+                    a.m[i[u] + k] = me[k];
+                    a.v[i[u] + k] = ve[k];
+                }
+            }
+        }
+    }
+    if (threadIdx.x < span.head && (!MASK || mask.one(threadIdx.x))) adam_one<PT, GT>(a, s, threadIdx.x);
+    for (uint32_t i = span.tail_at() + threadIdx.x, end = span.tail_at() + span.tail; i < end; i += kBlock)
+        if (!MASK || mask.one(i)) adam_one<PT, GT>(a, s, i);
+}
+
 __global__ __launch_bounds__(kBlock) void adam_kernel(AdamList list, AdamScalars s, const double* __restrict__ norm,
                                                       int64_t* __restrict__ step, int last_launch) {
-    float c = 1.0f;
+    AdamTerms e;
+    e.c = 1.0f;
     if (norm) {
         const double v = *norm;
         if (s.skip_nonfinite && !(v < (double)INFINITY)) {
@@ -194,29 +443,37 @@ __global__ __launch_bounds__(kBlock) void adam_kernel(AdamList list, AdamScalars
             if (last_launch && blockIdx.x == 0 && threadIdx.x == 0) *step -= 1;
             return;
         }
-        if (s.clip) c = clip_factor(v, s.max_norm, kAdamClipEps);
+        if (s.clip) e.c = clip_factor(v, s.max_norm, kAdamClipEps);
     }
     const int b = blockIdx.x;
     if (b >= list.first[list.n]) return;   // a launch without elements still takes a step back
-    const int t = find_tensor(list.first, list.n, b);
+    const int t = find_tensor(list.first, list.n, b), pt = list.pdtype[t], gt = list.gdtype[t];
     const double k = (double)*step;
     // 1 - beta^k without the cancellation
-    const float fix1 = (float)-expm1(k * s.log_beta1), fix2 = (float)sqrt(-expm1(k * s.log_beta2));
+    e.rate = (float)(list.lr[t] / -expm1(k * s.log_beta1));
+    e.root = (float)(1.0 / sqrt(-expm1(k * s.log_beta2)));
+    e.beta2 = s.beta2;
+    e.one_minus_beta1 = s.one_minus_beta1;
+    e.one_minus_beta2 = s.one_minus_beta2;
+    e.eps = s.eps;
+    e.keep = list.keep[t];
     const int64_t base = (int64_t)(b - list.first[t]) * list.chunk;
-    const int64_t end = min(base + list.chunk, list.numel[t]);
-    const float rate = list.lr[t] / fix1;
-    for (int64_t i = base + threadIdx.x; i < end; i += kBlock) {
-        if (!in_mask(list.mask[t], i, list.row[t])) continue;
-        const float g = load_as_float(list.grad[t], i, list.gdtype[t]) * c;
-        const float m0 = list.avg[t][i], v0 = list.sq[t][i];
-        const float m = m0 + s.one_minus_beta1 * (g - m0);
-        const float v = s.beta2 * v0 + s.one_minus_beta2 * g * g;
-        const float p = load_as_float(list.param[t], i, list.pdtype[t]) * list.keep[t]
-                        - rate * m / (sqrtf(v) / fix2 + s.eps);
-        list.avg[t][i] = m;
-        list.sq[t][i] = v;
-        store_from_float(list.param[t], i, list.pdtype[t], p);
+    const uint32_t count = (uint32_t)min((int64_t)list.chunk, list.numel[t] - base);
+    const AdamArrays a{at(list.param[t], base, pt), at(list.grad[t], base, gt), list.avg[t] + base, list.sq[t] + base};
+    const uint32_t phase = phase_of(a.p, pt);
+    ChunkSpan span(count, phase);
+    if (phase != phase_of(a.g, gt) || phase != phase_of(a.m, XSG_DTYPE_F32) || phase != phase_of(a.v, XSG_DTYPE_F32)) {
+        span.head = span.groups = 0;   // the arrays are not aligned alike: one element at a time
+        span.tail = count;
     }
+    ChunkMask mask;
+    if (list.mask[t]) mask.open(list.mask[t], base, list.row[t], list.magic[t], list.shift[t]);
+    with_type(pt, [&](auto p) {
+        with_type(gt, [&](auto g) {
+            with_mask(list.mask[t] != nullptr,
+                      [&](auto m) { chunk_adam<p.value, g.value, m.value>(a, e, span, mask); });
+        });
+    });
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -245,6 +502,14 @@ int check_rows(int64_t numel, const void* mask, int64_t rows, const char* who, i
     return XSG_OK;
 }
 
+// rows of a mask: d = 2^shift needs no magic; else magic = floor(2^32 (2^shift - d) / d) + 1, 2^(shift-1) < d < 2^shift
+RowDiv row_div(int64_t numel, const void* mask, int64_t rows) {
+    const uint32_t d = mask && numel ? (uint32_t)(numel / rows) : 1u;
+    uint32_t shift = 0;
+    while (((uint64_t)1 << shift) < d) ++shift;
+    return RowDiv{d, (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift};
+}
+
 xsg_grad_tensor grad_of(const xsg_grad_tensor& x) { return x; }
 xsg_grad_tensor grad_of(const xsg_adam_tensor& x) {
     return xsg_grad_tensor{const_cast<void*>(x.grad), x.numel, x.mask, x.rows, x.grad_dtype};
@@ -271,7 +536,7 @@ size_t partial_bytes(int64_t chunks) { return 256 + (size_t)chunks * sizeof(doub
 
 // fills list from ts[i0...] and returns how many tensors it took
 template <typename T> int fill_list(const T* ts, int n, int i0, int64_t chunk, GradList* list) {
-    list->chunk = chunk;
+    list->chunk = (int32_t)chunk;
     int k = 0;
     int32_t at = 0;
     for (; k < kListMax && i0 + k < n; ++k) {
@@ -279,7 +544,10 @@ template <typename T> int fill_list(const T* ts, int n, int i0, int64_t chunk, G
         list->data[k] = x.data;
         list->numel[k] = x.numel;
         list->mask[k] = x.mask;
-        list->row[k] = x.mask && x.numel ? (int32_t)(x.numel / x.rows) : 1;
+        const RowDiv div = row_div(x.numel, x.mask, x.rows);
+        list->row[k] = div.row;
+        list->magic[k] = div.magic;
+        list->shift[k] = (uint8_t)div.shift;
         list->dtype[k] = (uint8_t)x.dtype;
         list->first[k] = at;
         at += (int32_t)chunks_of(x.numel, chunk);
@@ -430,7 +698,6 @@ extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_op
     AdamScalars a;
     a.log_beta1 = log(o->beta1);   // beta 0: -inf, and 1 - beta^k is 1
     a.log_beta2 = log(o->beta2);
-    a.beta1 = (float)o->beta1;
     a.beta2 = (float)o->beta2;
     a.one_minus_beta1 = (float)(1.0 - o->beta1);
     a.one_minus_beta2 = (float)(1.0 - o->beta2);
@@ -440,7 +707,7 @@ extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_op
     a.max_norm = o->max_norm;
     AdamList list;
     for (int i = 0; i < n;) {
-        list.chunk = p.chunk;
+        list.chunk = (int32_t)p.chunk;
         int k = 0;
         int32_t at = 0;
         for (; k < kAdamMax && i + k < n; ++k) {
@@ -451,7 +718,10 @@ extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_op
             list.sq[k] = x.exp_avg_sq;
             list.numel[k] = x.numel;
             list.mask[k] = x.mask;
-            list.row[k] = x.mask && x.numel ? (int32_t)(x.numel / x.rows) : 1;
+            const RowDiv div = row_div(x.numel, x.mask, x.rows);
+            list.row[k] = div.row;
+            list.magic[k] = div.magic;
+            list.shift[k] = (uint8_t)div.shift;
             list.pdtype[k] = (uint8_t)x.param_dtype;
             list.gdtype[k] = (uint8_t)x.grad_dtype;
             list.lr[k] = (float)x.lr;
