@@ -109,11 +109,14 @@ XSG_DEV uint32_t phase_of(const void* p, int dtype) {
     return (4u - e) & 3u;
 }
 
+constexpr uint32_t kRowBatch = 2048;   // rows a wavefront lists at once
+
 // The packed mask seen from one chunk: element i of the chunk lies in row (rem + i) / row after word `words`
 // and bit `bit`.
 struct ChunkMask {
     const uint32_t* words;
     uint32_t bit, rem, row, magic, shift;
+    uint16_t* list;   // in LDS, kRowBatch entries for each wavefront
 
     XSG_DEV void open(const uint32_t* mask, int64_t base, uint32_t row_, uint32_t magic_, uint32_t shift_) {
         const int64_t r = base / row_;
@@ -225,6 +228,115 @@ XSG_DEV void for_chunk(const ChunkSpan& span, const ChunkMask& mask, One&& one, 
     if (threadIdx.x < span.tail && (!MASK || mask.one(i))) one(i);
 }
 
+// Under a mask of short rows each wavefront lists the kept rows of its share of the chunk (a mask word a lane, so
+// up to 2048 rows for one load's latency) and then walks their elements alone, VEC at a time, so that lanes are
+// busy and loads in flight however few rows are kept.
+// many(i[], on[]): UNROLL units of VEC elements from element i, of which those not on are left out.
+constexpr uint32_t kShortRow = 128;
+
+template <int VEC, int UNROLL, typename Many>
+XSG_DEV void for_kept_rows(const ChunkMask& mask, uint32_t count, Many&& many) {
+    uint16_t* const list = mask.list + (threadIdx.x >> 6) * kRowBatch;
+    const uint32_t lane = threadIdx.x & 63, rows = mask.quotient(mask.rem + count - 1) + 1;
+    const uint32_t share = (rows + kBlock / 64 - 1) / (kBlock / 64);
+    // the wavefront's rows as bits from mask.words[0] on
+    const uint32_t lo = mask.bit + min((threadIdx.x >> 6) * share, rows);
+    const uint32_t hi = min(lo + share, mask.bit + rows);
+    const uint32_t units = mask.row / VEC, magic = 0xffffffffu / units + 1;   // exact: units^2 kRowBatch < 2^32
+    const auto word_of = [&](uint32_t first) {   // bits of rows outside lo..hi are cleared
+        const uint32_t at = first + 32 * lane;
+        if (at >= hi) return 0u;
+        uint32_t w = mask.words[at >> 5];
+        if (at < lo) w &= 0xffffffffu << (lo - at);   // lo lies in the first word
+        return hi - at < 32 ? w & ~(0xffffffffu << (hi - at)) : w;
+    };
+    uint32_t next = word_of(lo & ~31u);
+    for (uint32_t batch = lo & ~31u; batch < hi; batch += kRowBatch) {
+        uint32_t word = next, upto = (uint32_t)__popc(word);
+        next = word_of(batch + kRowBatch);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t below = __shfl_up(upto, d);
+            if (lane >= d) upto += below;
+        }
+        const uint32_t n = __shfl(upto, 63);
+        for (uint32_t k = upto - (uint32_t)__popc(word); word; word &= word - 1)
+            list[k++] = (uint16_t)(32 * lane + __ffs(word) - 1);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint32_t total = n * units;
+        for (uint32_t w0 = lane; w0 < total; w0 += 64 * UNROLL) {
+            uint32_t i[UNROLL];
+            bool on[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const uint32_t w = w0 + 64 * u;
+                on[u] = w < total;
+                const uint32_t q = units == 1 ? w : __umulhi(w, magic);
+                const uint32_t r = batch + (on[u] ? list[q] : 0u) - mask.bit;
+                // the chunk's first and last row may lie in it in part; before it the difference wraps
+                i[u] = r * mask.row + (w - q * units) * VEC - mask.rem;
+                on[u] = on[u] && i[u] < count;
+            }
+            many(i, on);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+template <int NORM, int DT>
+XSG_DEV Accum<NORM> rows_norm(const void* p, uint32_t count, bool whole, const ChunkMask& mask) {
+    Accum<NORM> acc[4];
+    if (whole) {
+        for_kept_rows<4, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
+            float4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = on[u] ? load4<DT>(p, i[u]) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                acc[u].add(x[u].x);
+                acc[u].add(x[u].y);
+                acc[u].add(x[u].z);
+                acc[u].add(x[u].w);
+            }
+        });
+    } else {
+        for_kept_rows<1, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
+            float x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = on[u] ? load1<DT>(p, i[u]) : 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[u].add(x[u]);
+        });
+    }
+#pragma unroll
+    for (int u = 1; u < 4; ++u) acc[0].join(acc[u]);
+    return acc[0];
+}
+
+template <int DT> XSG_DEV void rows_scale(void* p, float c, uint32_t count, bool whole, const ChunkMask& mask) {
+    if (whole) {
+        for_kept_rows<4, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
+            float4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (on[u]) x[u] = load4<DT>(p, i[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (on[u]) store4<DT>(p, i[u], make_float4(x[u].x * c, x[u].y * c, x[u].z * c, x[u].w * c));
+        });
+    } else {
+        for_kept_rows<1, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
+            float x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (on[u]) x[u] = load1<DT>(p, i[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (on[u]) store1<DT>(p, i[u], x[u] * c);
+        });
+    }
+}
+
 template <int NORM, int DT, bool MASK>
 XSG_DEV Accum<NORM> chunk_norm(const void* p, const ChunkSpan& span, const ChunkMask& mask) {
     Accum<NORM> acc[kUnroll];
@@ -246,15 +358,11 @@ XSG_DEV Accum<NORM> chunk_norm(const void* p, const ChunkSpan& span, const Chunk
     return acc[0];
 }
 
-// calls f with the type, and with whether there is a mask, as constants
+// calls f with the type as a constant
 template <typename F> XSG_DEV void with_type(int dtype, F&& f) {
     if (dtype == XSG_DTYPE_F32) f(std::integral_constant<int, XSG_DTYPE_F32>{});
     else if (dtype == XSG_DTYPE_BF16) f(std::integral_constant<int, XSG_DTYPE_BF16>{});
     else f(std::integral_constant<int, XSG_DTYPE_F16>{});
-}
-template <typename F> XSG_DEV void with_mask(bool masked, F&& f) {
-    if (masked) f(std::true_type{});
-    else f(std::false_type{});
 }
 
 template <int NORM>
@@ -265,10 +373,14 @@ __global__ __launch_bounds__(kBlock) void norm_partial_kernel(GradList list, dou
     const void* p = at((const void*)list.data[t], base, dtype);
     const ChunkSpan span(count, phase_of(p, dtype));
     ChunkMask mask;
+    __shared__ uint16_t listed[kBlock / 64 * kRowBatch];
+    mask.list = listed;
     if (list.mask[t]) mask.open(list.mask[t], base, list.row[t], list.magic[t], list.shift[t]);
     Accum<NORM> acc;
     with_type(dtype, [&](auto dt) {
-        with_mask(list.mask[t] != nullptr, [&](auto m) { acc = chunk_norm<NORM, dt.value, m.value>(p, span, mask); });
+        if (!list.mask[t]) acc = chunk_norm<NORM, dt.value, false>(p, span, mask);
+        else if (mask.row > kShortRow) acc = chunk_norm<NORM, dt.value, true>(p, span, mask);
+        else acc = rows_norm<NORM, dt.value>(p, count, span.head == 0 && mask.row % 4 == 0, mask);
     });
     acc = block_join<NORM>(acc);
     if (threadIdx.x == 0) partial[b] = acc.value();
@@ -340,9 +452,13 @@ __global__ __launch_bounds__(kBlock) void clip_scale_kernel(GradList list, const
     void* p = at(list.data[t], base, dtype);
     const ChunkSpan span(count, phase_of(p, dtype));
     ChunkMask mask;
+    __shared__ uint16_t listed[kBlock / 64 * kRowBatch];
+    mask.list = listed;
     if (list.mask[t]) mask.open(list.mask[t], base, list.row[t], list.magic[t], list.shift[t]);
     with_type(dtype, [&](auto dt) {
-        with_mask(list.mask[t] != nullptr, [&](auto m) { chunk_scale<dt.value, m.value>(p, c, span, mask); });
+        if (!list.mask[t]) chunk_scale<dt.value, false>(p, c, span, mask);
+        else if (mask.row > kShortRow) chunk_scale<dt.value, true>(p, c, span, mask);
+        else rows_scale<dt.value>(p, c, count, span.head == 0 && mask.row % 4 == 0, mask);
     });
 }
 
@@ -432,6 +548,54 @@ XSG_DEV void chunk_adam(const AdamArrays& a, const AdamTerms& s, const ChunkSpan
         if (!MASK || mask.one(i)) adam_one<PT, GT>(a, s, i);
 }
 
+template <int PT, int GT>
+XSG_DEV void rows_adam(const AdamArrays& a, const AdamTerms& s, uint32_t count, bool whole, const ChunkMask& mask) {
+    if (whole) {
+        for_kept_rows<4, kAdamUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
+            float4 p[kAdamUnroll], g[kAdamUnroll], m[kAdamUnroll], v[kAdamUnroll];
+#pragma unroll
+            for (int u = 0; u < kAdamUnroll; ++u) {
+                if (!on[u]) continue;
+                p[u] = load4<PT>(a.p, i[u]);
+                g[u] = load4<GT>(a.g, i[u]);
+                m[u] = load4<XSG_DTYPE_F32>(a.m, i[u]);
+                v[u] = load4<XSG_DTYPE_F32>(a.v, i[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kAdamUnroll; ++u) {
+                if (!on[u]) continue;
+                s.update(p[u].x, g[u].x, m[u].x, v[u].x);
+                s.update(p[u].y, g[u].y, m[u].y, v[u].y);
+                s.update(p[u].z, g[u].z, m[u].z, v[u].z);
+                s.update(p[u].w, g[u].w, m[u].w, v[u].w);
+                store4<PT>(a.p, i[u], p[u]);
+                store4<XSG_DTYPE_F32>(a.m, i[u], m[u]);
+                store4<XSG_DTYPE_F32>(a.v, i[u], v[u]);
+            }
+        });
+    } else {
+        for_kept_rows<1, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
+            float p[4], g[4], m[4], v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (!on[u]) continue;
+                p[u] = load1<PT>(a.p, i[u]);
+                g[u] = load1<GT>(a.g, i[u]);
+                m[u] = a.m[i[u]];
+                v[u] = a.v[i[u]];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (!on[u]) continue;
+                s.update(p[u], g[u], m[u], v[u]);
+                store1<PT>(a.p, i[u], p[u]);
+                a.m[i[u]] = m[u];
+                a.v[i[u]] = v[u];
+            }
+        });
+    }
+}
+
 __global__ __launch_bounds__(kBlock) void adam_kernel(AdamList list, AdamScalars s, const double* __restrict__ norm,
                                                       int64_t* __restrict__ step, int last_launch) {
     AdamTerms e;
@@ -466,12 +630,16 @@ __global__ __launch_bounds__(kBlock) void adam_kernel(AdamList list, AdamScalars
         span.head = span.groups = 0;   // the arrays are not aligned alike: one element at a time
         span.tail = count;
     }
+    const bool whole = span.groups > 0 && span.head == 0 && list.row[t] % 4 == 0;   // rows of whole groups
     ChunkMask mask;
+    __shared__ uint16_t listed[kBlock / 64 * kRowBatch];
+    mask.list = listed;
     if (list.mask[t]) mask.open(list.mask[t], base, list.row[t], list.magic[t], list.shift[t]);
     with_type(pt, [&](auto p) {
         with_type(gt, [&](auto g) {
-            with_mask(list.mask[t] != nullptr,
-                      [&](auto m) { chunk_adam<p.value, g.value, m.value>(a, e, span, mask); });
+            if (!list.mask[t]) chunk_adam<p.value, g.value, false>(a, e, span, mask);
+            else if (mask.row > kShortRow) chunk_adam<p.value, g.value, true>(a, e, span, mask);
+            else rows_adam<p.value, g.value>(a, e, count, whole, mask);
         });
     });
 }
