@@ -3,12 +3,14 @@
 // counterpart (the reference's trainer is outside its rendering library).
 //
 // All three run over a list of tensors cut into chunks of one length; a workgroup takes one chunk. The list
-// travels in the kernel's arguments (no copy, no allocation, and a captured graph holds it by value), as many
-// tensors to a launch as 4 KB of arguments hold. Sums are held in 64 bits and added in a fixed order, so a
-// call's results are the same bits each time.
+// travels in the kernels' arguments (no copy from the host, and a captured graph holds it by value): a short one
+// in the arguments of each kernel, a long one piece by piece into the workspace, so that each pass stays one
+// launch over all tensors. Sums are held in 64 bits and added in a fixed order, so a call's results are the
+// same bits each time.
 #include <math.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "xsg_common.h"
 
@@ -20,8 +22,8 @@ constexpr int64_t kTargetChunks = 2048;   // chunks of a call, when its tensors 
 constexpr int64_t kMaxChunk = 1 << 30;    // offsets inside a chunk are 32-bit
 constexpr int64_t kMaxRow = 1 << 30;      // and so are rows under a mask
 constexpr int64_t kMaxElements = (int64_t)1 << 48;
-constexpr int kListMax = 96;             // gradient tensors to a launch
-constexpr int kAdamMax = 48;              // tensors with their states to a launch
+constexpr int kArgumentBytes = 3900;      // of a list, beside the other arguments in 4 KB
+constexpr int kJoinMax = 4096;            // partial sums that every workgroup joins by itself
 
 // Division of n < 2^31 by the row length: (mulhi(n, magic) + n) >> shift
 struct RowDiv {
@@ -29,35 +31,60 @@ struct RowDiv {
     uint32_t shift;
 };
 
-struct GradList {
-    void* data[kListMax];
-    int64_t numel[kListMax];
-    const uint32_t* mask[kListMax];
-    uint32_t row[kListMax], magic[kListMax];  // elements to a mask bit, and its division
-    int32_t first[kListMax + 1];              // first chunk of each tensor in this launch
-    uint8_t shift[kListMax];
-    uint8_t dtype[kListMax];
-    int32_t n;
-    int32_t chunk;
+struct GradEntry {
+    void* data;
+    int64_t numel;
+    const uint32_t* mask;
+    uint32_t row, magic;      // elements to a mask bit, and its division
+    uint8_t shift, dtype;
+    XSG_HD const void* grad() const { return data; }
+    XSG_HD int grad_dtype() const { return dtype; }
 };
-static_assert(sizeof(GradList) <= 3900, "the list and the other arguments share 4 KB");
 
-struct AdamList {
-    void* param[kAdamMax];
-    const void* grad[kAdamMax];
-    float* avg[kAdamMax];
-    float* sq[kAdamMax];
-    int64_t numel[kAdamMax];
-    const uint32_t* mask[kAdamMax];
-    uint32_t row[kAdamMax], magic[kAdamMax];
-    int32_t first[kAdamMax + 1];
-    float lr[kAdamMax];
-    float keep[kAdamMax];         // 1 - lr * weight decay
-    uint8_t shift[kAdamMax], pdtype[kAdamMax], gdtype[kAdamMax];
-    int32_t n;
-    int32_t chunk;
+struct AdamEntry {
+    void* param;
+    const void* gradient;
+    float *avg, *sq;
+    int64_t numel;
+    const uint32_t* mask;
+    uint32_t row, magic;
+    float lr, keep;           // keep: 1 - lr * weight decay
+    uint8_t shift, pdtype, gdtype;
+    XSG_HD const void* grad() const { return gradient; }
+    XSG_HD int grad_dtype() const { return gdtype; }
 };
-static_assert(sizeof(AdamList) <= 3900, "the list and the other arguments share 4 KB");
+
+template <typename E> constexpr int kInline = kArgumentBytes / (sizeof(E) + 4);
+
+// first[t]: the first chunk of tensor t; first[n] = chunks
+template <typename E> struct InlineList {
+    E entry[kInline<E>];
+    int32_t first[kInline<E> + 1];
+    int32_t n, chunk, chunks;
+};
+template <typename E> struct TableList {
+    const E* __restrict__ entry;
+    const int32_t* __restrict__ first;
+    int32_t n, chunk, chunks;
+};
+// a piece of a table on its way to the workspace
+template <typename E> struct TablePiece {
+    E entry[kInline<E>];
+    int32_t first[kInline<E>];
+    int32_t n;
+};
+static_assert(sizeof(InlineList<GradEntry>) <= 3920 && sizeof(InlineList<AdamEntry>) <= 3920 &&
+                  sizeof(GradEntry) % 8 == 0 && sizeof(AdamEntry) % 8 == 0,
+              "lists share 4 KB with the other arguments and are copied by words");
+
+template <typename E>
+__global__ __launch_bounds__(kBlock) void table_kernel(TablePiece<E> piece, E* __restrict__ entry,
+                                                       int32_t* __restrict__ first, int last) {
+    const uint64_t* const from = reinterpret_cast<const uint64_t*>(piece.entry);
+    uint64_t* const to = reinterpret_cast<uint64_t*>(entry);
+    for (int i = threadIdx.x; i < piece.n * (int)(sizeof(E) / 8); i += kBlock) to[i] = from[i];
+    if (threadIdx.x < piece.n + last) first[threadIdx.x] = piece.first[threadIdx.x];
+}
 
 // round to nearest even; a NaN stays one
 XSG_DEV uint32_t bf16_bits(float x) {
@@ -147,14 +174,18 @@ struct ChunkMask {
     }
 };
 
-// the tensor whose chunks hold chunk b: the last one with first[t] <= b (empty tensors have no chunk)
-XSG_DEV int find_tensor(const int32_t* first, int n, int b) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= b) lo = mid; else hi = mid;
+// The tensor whose chunks hold chunk b: the last one with first[t] <= b (empty tensors have no chunk). The
+// wavefront looks at 64 places of what is left at once.
+template <typename L> XSG_DEV int find_tensor(const L& list, int b) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = list.n;
+    for (;;) {
+        const int step = (n + 63) >> 6, i = lane * step;
+        const int below = __popcll(__ballot(i < n && list.first[lo + min(i, n - 1)] <= b)) - 1;
+        lo += below * step;
+        n = min(step, n - below * step);
+        if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
     }
-    return lo;
 }
 
 // Accumulation of one kind of norm. Sums are in 64 bits, where squares of any float32 stay finite and above
@@ -365,52 +396,79 @@ template <typename F> XSG_DEV void with_type(int dtype, F&& f) {
     else f(std::integral_constant<int, XSG_DTYPE_F16>{});
 }
 
-template <int NORM>
-__global__ __launch_bounds__(kBlock) void norm_partial_kernel(GradList list, double* __restrict__ partial) {
-    const int b = blockIdx.x, t = find_tensor(list.first, list.n, b), dtype = list.dtype[t];
-    const int64_t base = (int64_t)(b - list.first[t]) * list.chunk;
-    const uint32_t count = (uint32_t)min((int64_t)list.chunk, list.numel[t] - base);
-    const void* p = at((const void*)list.data[t], base, dtype);
-    const ChunkSpan span(count, phase_of(p, dtype));
+// What a workgroup does first: its chunk of its tensor.
+struct Chunk {
+    int64_t base;
+    uint32_t count;
+    template <typename L, typename E> XSG_DEV Chunk(const L& list, const E& e, int b, int t) {
+        base = (int64_t)(b - list.first[t]) * list.chunk;
+        count = (uint32_t)min((int64_t)list.chunk, e.numel - base);
+    }
+};
+
+// `step`, unless null, counts one step more; the launches behind this one read it.
+template <int NORM, typename L>
+__global__ __launch_bounds__(kBlock) void norm_partial_kernel(L list, double* __restrict__ partial, int64_t* step) {
+    const int b = blockIdx.x;
+    if (step && b == 0 && threadIdx.x == 0) *step += 1;
+    if (b >= list.chunks) return;   // no elements at all
+    const int t = find_tensor(list, b);
+    const auto& e = list.entry[t];
+    const Chunk chunk(list, e, b, t);
+    const int dtype = e.grad_dtype();
+    const void* p = at(e.grad(), chunk.base, dtype);
+    const ChunkSpan span(chunk.count, phase_of(p, dtype));
     ChunkMask mask;
     __shared__ uint16_t listed[kBlock / 64 * kRowBatch];
     mask.list = listed;
-    if (list.mask[t]) mask.open(list.mask[t], base, list.row[t], list.magic[t], list.shift[t]);
+    if (e.mask) mask.open(e.mask, chunk.base, e.row, e.magic, e.shift);
     Accum<NORM> acc;
     with_type(dtype, [&](auto dt) {
-        if (!list.mask[t]) acc = chunk_norm<NORM, dt.value, false>(p, span, mask);
+        if (!e.mask) acc = chunk_norm<NORM, dt.value, false>(p, span, mask);
         else if (mask.row > kShortRow) acc = chunk_norm<NORM, dt.value, true>(p, span, mask);
-        else acc = rows_norm<NORM, dt.value>(p, count, span.head == 0 && mask.row % 4 == 0, mask);
+        else acc = rows_norm<NORM, dt.value>(p, chunk.count, span.head == 0 && mask.row % 4 == 0, mask);
     });
     acc = block_join<NORM>(acc);
     if (threadIdx.x == 0) partial[b] = acc.value();
 }
 
-template <int NORM> XSG_DEV double join_partials(const double* __restrict__ partial, int n) {
+template <int NORM> XSG_DEV Accum<NORM> join_partials(const double* __restrict__ partial, int n) {
     Accum<NORM> acc;
     for (int i = threadIdx.x; i < n; i += kBlock) acc.join_value(partial[i]);
-    return block_join<NORM>(acc).finish();
+    return block_join<NORM>(acc);
 }
 
-// Block 0: the norm over every chunk of the call, to `total` (float32) and `sum` (64 bits).
-// Blocks 1..n: the norm of each tensor of this list, whose chunks start at partial[0].
-template <int NORM>
-__global__ __launch_bounds__(kBlock) void norm_finish_kernel(GradList list, const double* __restrict__ all,
-                                                             int n_all, const double* __restrict__ partial,
-                                                             float* __restrict__ total, double* __restrict__ sum,
-                                                             float* __restrict__ each) {
-    if (blockIdx.x == 0) {
-        const double v = join_partials<NORM>(all, n_all);
-        if (threadIdx.x == 0) {
-            if (total) *total = (float)v;
-            *sum = v;
-        }
-    } else {
-        const int t = blockIdx.x - 1;
-        const int lo = list.first[t], hi = list.first[t + 1];
-        const double v = join_partials<NORM>(partial + lo, hi - lo);
-        if (threadIdx.x == 0) each[t] = (float)v;
-    }
+// The norm from the partial sums of its chunks, in every thread of the workgroup.
+XSG_DEV double norm_of(const double* __restrict__ partial, int n, int norm) {
+    if (norm == XSG_NORM_L2) return join_partials<XSG_NORM_L2>(partial, n).finish();
+    if (norm == XSG_NORM_L1) return join_partials<XSG_NORM_L1>(partial, n).finish();
+    return join_partials<XSG_NORM_INF>(partial, n).finish();
+}
+
+// Many partial sums become one, where each workgroup of the next launch would join them all again.
+__global__ __launch_bounds__(kBlock) void norm_reduce_kernel(const double* __restrict__ partial, int n, int norm,
+                                                             double* __restrict__ one) {
+    double v;
+    if (norm == XSG_NORM_L2) v = join_partials<XSG_NORM_L2>(partial, n).value();
+    else if (norm == XSG_NORM_L1) v = join_partials<XSG_NORM_L1>(partial, n).value();
+    else v = join_partials<XSG_NORM_INF>(partial, n).value();
+    if (threadIdx.x == 0) *one = v;
+}
+
+__global__ __launch_bounds__(kBlock) void norm_total_kernel(const double* __restrict__ partial, int n, int norm,
+                                                            float* __restrict__ total) {
+    const double v = norm_of(partial, n, norm);
+    if (threadIdx.x == 0) *total = (float)v;
+}
+
+// Block t < n: the norm of tensor t. Block n: the norm over all of them.
+template <typename L>
+__global__ __launch_bounds__(kBlock) void norm_each_kernel(L list, const double* __restrict__ partial, int norm,
+                                                           float* __restrict__ total, float* __restrict__ each) {
+    const int t = blockIdx.x;
+    const int lo = t < list.n ? list.first[t] : 0, hi = t < list.n ? list.first[t + 1] : list.chunks;
+    const double v = norm_of(partial + lo, hi - lo, norm);
+    if (threadIdx.x == 0) *(t < list.n ? each + t : total) = (float)v;
 }
 
 // min(1, max_norm / (norm + eps)); a NaN norm gives NaN, an infinite one 0
@@ -442,23 +500,34 @@ XSG_DEV void chunk_scale(void* p, float c, const ChunkSpan& span, const ChunkMas
     });
 }
 
-__global__ __launch_bounds__(kBlock) void clip_scale_kernel(GradList list, const double* __restrict__ norm,
-                                                            double max_norm, double eps) {
-    const float c = clip_factor(*norm, max_norm, eps);
-    if (c == 1.0f) return;   // the values stay as they are
-    const int b = blockIdx.x, t = find_tensor(list.first, list.n, b), dtype = list.dtype[t];
-    const int64_t base = (int64_t)(b - list.first[t]) * list.chunk;
-    const uint32_t count = (uint32_t)min((int64_t)list.chunk, list.numel[t] - base);
-    void* p = at(list.data[t], base, dtype);
-    const ChunkSpan span(count, phase_of(p, dtype));
+// The norm that a launch clips by: partial sums, how many, and what kind.
+struct NormParts {
+    const double* __restrict__ partial;
+    int n, norm;
+};
+
+template <typename L>
+__global__ __launch_bounds__(kBlock) void clip_scale_kernel(L list, NormParts parts, double max_norm, double eps,
+                                                            float* __restrict__ total) {
+    const double norm = norm_of(parts.partial, parts.n, parts.norm);
+    const int b = blockIdx.x;
+    if (b == 0 && threadIdx.x == 0) *total = (float)norm;
+    const float c = clip_factor(norm, max_norm, eps);
+    if (c == 1.0f || b >= list.chunks) return;   // the values stay as they are
+    const int t = find_tensor(list, b);
+    const auto& e = list.entry[t];
+    const Chunk chunk(list, e, b, t);
+    const int dtype = e.dtype;
+    void* p = at(e.data, chunk.base, dtype);
+    const ChunkSpan span(chunk.count, phase_of(p, dtype));
     ChunkMask mask;
     __shared__ uint16_t listed[kBlock / 64 * kRowBatch];
     mask.list = listed;
-    if (list.mask[t]) mask.open(list.mask[t], base, list.row[t], list.magic[t], list.shift[t]);
+    if (e.mask) mask.open(e.mask, chunk.base, e.row, e.magic, e.shift);
     with_type(dtype, [&](auto dt) {
-        if (!list.mask[t]) chunk_scale<dt.value, false>(p, c, span, mask);
+        if (!e.mask) chunk_scale<dt.value, false>(p, c, span, mask);
         else if (mask.row > kShortRow) chunk_scale<dt.value, true>(p, c, span, mask);
-        else rows_scale<dt.value>(p, c, count, span.head == 0 && mask.row % 4 == 0, mask);
+        else rows_scale<dt.value>(p, c, chunk.count, span.head == 0 && mask.row % 4 == 0, mask);
     });
 }
 
@@ -470,7 +539,7 @@ struct AdamScalars {
 };
 constexpr double kAdamClipEps = 1e-6;
 
-// The step counter counts this step; adam_kernel takes it back where the step is not taken.
+// Without a norm to compute, the step is counted by a launch of its own.
 __global__ void adam_count_kernel(int64_t* step) { *step += 1; }
 
 // One value of the update; rate: lr / (1 - beta1^t), root: 1 / sqrt(1 - beta2^t)
@@ -596,50 +665,54 @@ XSG_DEV void rows_adam(const AdamArrays& a, const AdamTerms& s, uint32_t count, 
     }
 }
 
-__global__ __launch_bounds__(kBlock) void adam_kernel(AdamList list, AdamScalars s, const double* __restrict__ norm,
-                                                      int64_t* __restrict__ step, int last_launch) {
-    AdamTerms e;
-    e.c = 1.0f;
-    if (norm) {
-        const double v = *norm;
-        if (s.skip_nonfinite && !(v < (double)INFINITY)) {
-            // no workgroup of any of the call's launches reads the counter in this case
-            if (last_launch && blockIdx.x == 0 && threadIdx.x == 0) *step -= 1;
+// parts.n < 0: no norm. The counter already counts this step; it is taken back where the step is not taken.
+template <typename L>
+__global__ __launch_bounds__(kBlock) void adam_kernel(L list, AdamScalars s, NormParts parts, int64_t* step,
+                                                      float* __restrict__ total) {
+    const int b = blockIdx.x;
+    AdamTerms terms;
+    terms.c = 1.0f;
+    if (parts.n >= 0) {
+        const double norm = norm_of(parts.partial, parts.n, parts.norm);
+        if (total && b == 0 && threadIdx.x == 0) *total = (float)norm;
+        if (s.skip_nonfinite && !(norm < (double)INFINITY)) {
+            if (b == 0 && threadIdx.x == 0) *step -= 1;   // no other workgroup reads the counter in this case
             return;
         }
-        if (s.clip) e.c = clip_factor(v, s.max_norm, kAdamClipEps);
+        if (s.clip) terms.c = clip_factor(norm, s.max_norm, kAdamClipEps);
     }
-    const int b = blockIdx.x;
-    if (b >= list.first[list.n]) return;   // a launch without elements still takes a step back
-    const int t = find_tensor(list.first, list.n, b), pt = list.pdtype[t], gt = list.gdtype[t];
+    if (b >= list.chunks) return;
+    const int t = find_tensor(list, b);
+    const auto& e = list.entry[t];
+    const Chunk chunk(list, e, b, t);
     const double k = (double)*step;
     // 1 - beta^k without the cancellation
-    e.rate = (float)(list.lr[t] / -expm1(k * s.log_beta1));
-    e.root = (float)(1.0 / sqrt(-expm1(k * s.log_beta2)));
-    e.beta2 = s.beta2;
-    e.one_minus_beta1 = s.one_minus_beta1;
-    e.one_minus_beta2 = s.one_minus_beta2;
-    e.eps = s.eps;
-    e.keep = list.keep[t];
-    const int64_t base = (int64_t)(b - list.first[t]) * list.chunk;
-    const uint32_t count = (uint32_t)min((int64_t)list.chunk, list.numel[t] - base);
-    const AdamArrays a{at(list.param[t], base, pt), at(list.grad[t], base, gt), list.avg[t] + base, list.sq[t] + base};
+    terms.rate = (float)(e.lr / -expm1(k * s.log_beta1));
+    terms.root = (float)(1.0 / sqrt(-expm1(k * s.log_beta2)));
+    terms.beta2 = s.beta2;
+    terms.one_minus_beta1 = s.one_minus_beta1;
+    terms.one_minus_beta2 = s.one_minus_beta2;
+    terms.eps = s.eps;
+    terms.keep = e.keep;
+    const int pt = e.pdtype, gt = e.gdtype;
+    const AdamArrays a{at(e.param, chunk.base, pt), at(e.gradient, chunk.base, gt), e.avg + chunk.base,
+                       e.sq + chunk.base};
     const uint32_t phase = phase_of(a.p, pt);
-    ChunkSpan span(count, phase);
+    ChunkSpan span(chunk.count, phase);
     if (phase != phase_of(a.g, gt) || phase != phase_of(a.m, XSG_DTYPE_F32) || phase != phase_of(a.v, XSG_DTYPE_F32)) {
         span.head = span.groups = 0;   // the arrays are not aligned alike: one element at a time
-        span.tail = count;
+        span.tail = chunk.count;
     }
-    const bool whole = span.groups > 0 && span.head == 0 && list.row[t] % 4 == 0;   // rows of whole groups
+    const bool whole = span.groups > 0 && span.head == 0 && e.row % 4 == 0;   // rows of whole groups
     ChunkMask mask;
     __shared__ uint16_t listed[kBlock / 64 * kRowBatch];
     mask.list = listed;
-    if (list.mask[t]) mask.open(list.mask[t], base, list.row[t], list.magic[t], list.shift[t]);
+    if (e.mask) mask.open(e.mask, chunk.base, e.row, e.magic, e.shift);
     with_type(pt, [&](auto p) {
         with_type(gt, [&](auto g) {
-            if (!list.mask[t]) chunk_adam<p.value, g.value, false>(a, e, span, mask);
-            else if (mask.row > kShortRow) chunk_adam<p.value, g.value, true>(a, e, span, mask);
-            else rows_adam<p.value, g.value>(a, e, count, whole, mask);
+            if (!e.mask) chunk_adam<p.value, g.value, false>(a, terms, span, mask);
+            else if (mask.row > kShortRow) chunk_adam<p.value, g.value, true>(a, terms, span, mask);
+            else rows_adam<p.value, g.value>(a, terms, chunk.count, whole, mask);
         });
     });
 }
@@ -683,11 +756,29 @@ xsg_grad_tensor grad_of(const xsg_adam_tensor& x) {
     return xsg_grad_tensor{const_cast<void*>(x.grad), x.numel, x.mask, x.rows, x.grad_dtype};
 }
 
+GradEntry entry_of(const xsg_grad_tensor& x) {
+    const RowDiv div = row_div(x.numel, x.mask, x.rows);
+    return GradEntry{x.data, x.numel, x.numel ? x.mask : nullptr, div.row, div.magic, (uint8_t)div.shift, (uint8_t)x.dtype};
+}
+AdamEntry entry_of(const xsg_adam_tensor& x) {
+    const RowDiv div = row_div(x.numel, x.mask, x.rows);
+    return AdamEntry{x.param, x.grad, x.exp_avg, x.exp_avg_sq, x.numel, x.numel ? x.mask : nullptr, div.row, div.magic,
+                     (float)x.lr, (float)(1.0 - x.lr * x.weight_decay), (uint8_t)div.shift, (uint8_t)x.param_dtype,
+                     (uint8_t)x.grad_dtype};
+}
+template <typename T> using EntryOf = decltype(entry_of(std::declval<const T&>()));
+
+// How a call is cut, and where things lie in its workspace: one double for a reduced norm, then (256 bytes on)
+// a partial sum per chunk, then a long list's table.
 struct Plan {
     int64_t elements = 0, chunk = 0, chunks = 0;
+    bool table = false;
+    size_t first_at = 0, entry_at = 0, bytes = 0;
 };
 
-template <typename T> int make_plan(const T* ts, int n, const char* who, Plan* p) {
+size_t aligned(size_t x) { return (x + 255) / 256 * 256; }
+
+template <typename T> int make_plan(const T* ts, int n, const char* who, bool norm, Plan* p) {
     if (n < 0 || (n > 0 && !ts)) return xsg_fail(XSG_ERR_INVALID, "%s: null or negative list of tensors", who);
     for (int i = 0; i < n; ++i) {
         if (ts[i].numel < 0) return xsg_fail(XSG_ERR_INVALID, "%s: tensor %d has a negative size", who, i);
@@ -697,32 +788,64 @@ template <typename T> int make_plan(const T* ts, int n, const char* who, Plan* p
     p->chunk = chunk_for(p->elements);
     for (int i = 0; i < n; ++i) p->chunks += chunks_of(ts[i].numel, p->chunk);
     if (p->chunks > kMaxChunk) return xsg_fail(XSG_ERR_INVALID, "%s: too many tensors", who);
+    p->table = n > kInline<EntryOf<T>>;
+    p->bytes = norm ? 256 + aligned((size_t)p->chunks * sizeof(double)) : 0;
+    if (p->table) {
+        p->first_at = p->bytes;
+        p->entry_at = p->first_at + aligned(((size_t)n + 1) * sizeof(int32_t));
+        p->bytes = p->entry_at + aligned((size_t)n * sizeof(EntryOf<T>));
+    }
     return XSG_OK;
 }
 
-size_t partial_bytes(int64_t chunks) { return 256 + (size_t)chunks * sizeof(double); }
-
-// fills list from ts[i0...] and returns how many tensors it took
-template <typename T> int fill_list(const T* ts, int n, int i0, int64_t chunk, GradList* list) {
-    list->chunk = (int32_t)chunk;
-    int k = 0;
+template <typename T> void fill_inline(const T* ts, int n, const Plan& p, InlineList<EntryOf<T>>* list) {
     int32_t at = 0;
-    for (; k < kListMax && i0 + k < n; ++k) {
-        const xsg_grad_tensor x = grad_of(ts[i0 + k]);
-        list->data[k] = x.data;
-        list->numel[k] = x.numel;
-        list->mask[k] = x.mask;
-        const RowDiv div = row_div(x.numel, x.mask, x.rows);
-        list->row[k] = div.row;
-        list->magic[k] = div.magic;
-        list->shift[k] = (uint8_t)div.shift;
-        list->dtype[k] = (uint8_t)x.dtype;
-        list->first[k] = at;
-        at += (int32_t)chunks_of(x.numel, chunk);
+    for (int i = 0; i < n; ++i) {
+        list->entry[i] = entry_of(ts[i]);
+        list->first[i] = at;
+        at += (int32_t)chunks_of(ts[i].numel, p.chunk);
     }
-    list->first[k] = at;
-    list->n = k;
-    return k;
+    list->first[n] = at;
+    list->n = n;
+    list->chunk = (int32_t)p.chunk;
+    list->chunks = at;
+}
+
+template <typename T>
+int send_table(const T* ts, int n, const Plan& p, void* ws, hipStream_t s, TableList<EntryOf<T>>* list) {
+    using E = EntryOf<T>;
+    int32_t* const first = (int32_t*)((char*)ws + p.first_at);
+    E* const entry = (E*)((char*)ws + p.entry_at);
+    TablePiece<E> piece;
+    int32_t at = 0;
+    // first[n], the end, goes as one more tensor's first chunk
+    for (int i = 0; i <= n;) {
+        const int i0 = i;
+        for (piece.n = 0; piece.n < kInline<E> && i < n; ++i, ++piece.n) {
+            piece.entry[piece.n] = entry_of(ts[i]);
+            piece.first[piece.n] = at;
+            at += (int32_t)chunks_of(ts[i].numel, p.chunk);
+        }
+        const bool last = i == n && piece.n < kInline<E>;
+        if (last) piece.first[piece.n] = at;
+        table_kernel<E><<<1, kBlock, 0, s>>>(piece, entry + i0, first + i0, last);
+        XSG_TRY_LAUNCH("table");
+        if (last) break;
+    }
+    *list = TableList<E>{entry, first, n, (int32_t)p.chunk, at};
+    return XSG_OK;
+}
+
+// calls f with the list as the kernels take it
+template <typename T, typename F> int with_list(const T* ts, int n, const Plan& p, void* ws, hipStream_t s, F&& f) {
+    if (p.table) {
+        TableList<EntryOf<T>> list;
+        const int rc = send_table(ts, n, p, ws, s, &list);
+        return rc == XSG_OK ? f(list) : rc;
+    }
+    InlineList<EntryOf<T>> list;
+    fill_inline(ts, n, p, &list);
+    return f(list);
 }
 
 template <typename T> int check_list(const T* ts, int n, int norm, const char* who) {
@@ -744,64 +867,56 @@ template <typename F> void with_norm(int norm, F&& f) {
     else f(std::integral_constant<int, XSG_NORM_INF>{});
 }
 
-// workspace: the norm in 64 bits, then (256 bytes on) one partial per chunk
-template <typename T>
-int launch_norm(const T* ts, int n, int norm, const Plan& p, float* total, float* each, void* ws, hipStream_t s) {
-    double* sum = (double*)ws;
-    double* partial = (double*)((char*)ws + 256);
-    GradList list;
-    int64_t at = 0;
-    for (int i = 0; i < n;) {
-        const int k = fill_list(ts, n, i, p.chunk, &list);
-        const int chunks = list.first[k];
-        if (chunks > 0) {
-            with_norm(norm, [&](auto kind) {
-                norm_partial_kernel<kind.value><<<chunks, kBlock, 0, s>>>(list, partial + at);
-            });
-            XSG_TRY_LAUNCH("grad_norm");
-        }
-        at += chunks;
-        i += k;
-    }
-    at = 0;
-    int i = 0;
-    do {
-        const int k = fill_list(ts, n, i, p.chunk, &list);
-        with_norm(norm, [&](auto kind) {
-            norm_finish_kernel<kind.value><<<each ? 1 + k : 1, kBlock, 0, s>>>(list, partial, (int)p.chunks,
-                                                                              partial + at, total, sum,
-                                                                              each ? each + i : nullptr);
-        });
-        XSG_TRY_LAUNCH("grad_norm");
-        at += list.first[k];
-        i += k;
-    } while (each && i < n);
-    return XSG_OK;
+double* partials(void* ws) { return (double*)((char*)ws + 256); }
+
+template <typename L>
+int launch_partials(const L& list, int norm, void* ws, int64_t* step, hipStream_t s) {
+    with_norm(norm, [&](auto kind) {
+        norm_partial_kernel<kind.value><<<std::max(list.chunks, 1), kBlock, 0, s>>>(list, partials(ws), step);
+    });
+    return xsg_launch_status("grad_norm");
+}
+
+// the partial sums as the next launch's workgroups join them
+int join_parts(int chunks, int norm, void* ws, hipStream_t s, NormParts* parts) {
+    *parts = NormParts{partials(ws), chunks, norm};
+    if (chunks <= kJoinMax) return XSG_OK;
+    norm_reduce_kernel<<<1, kBlock, 0, s>>>(partials(ws), chunks, norm, (double*)ws);
+    *parts = NormParts{(const double*)ws, 1, norm};
+    return xsg_launch_status("grad_norm");
 }
 
 }  // namespace
 
 extern "C" size_t xsg_grad_norm_workspace_bytes(const xsg_grad_tensor* ts, int n) {
     Plan p;
-    return make_plan(ts, n, "grad_norm", &p) == XSG_OK ? partial_bytes(p.chunks) : 0;
+    return make_plan(ts, n, "grad_norm", true, &p) == XSG_OK ? p.bytes : 0;
 }
 
 extern "C" int xsg_grad_norm(const xsg_grad_tensor* ts, int n, int norm, float* total, float* each, void* workspace,
                              xsg_stream_t stream) {
     Plan p;
-    int rc = make_plan(ts, n, "grad_norm", &p);
+    int rc = make_plan(ts, n, "grad_norm", true, &p);
     if (rc == XSG_OK) rc = check_list(ts, n, norm, "grad_norm");
     if (rc != XSG_OK) return rc;
     if (!total || !workspace) return xsg_fail(XSG_ERR_INVALID, "grad_norm: null output or workspace");
     rc = xsg_check_workspace(workspace, "grad_norm");
     if (rc != XSG_OK) return rc;
-    return launch_norm(ts, n, norm, p, total, each, workspace, (hipStream_t)stream);
+    const hipStream_t s = (hipStream_t)stream;
+    return with_list(ts, n, p, workspace, s, [&](const auto& list) {
+        const int status = launch_partials(list, norm, workspace, nullptr, s);
+        if (status != XSG_OK) return status;
+        const double* const partial = partials(workspace);
+        if (each) norm_each_kernel<<<n + 1, kBlock, 0, s>>>(list, partial, norm, total, each);
+        else norm_total_kernel<<<1, kBlock, 0, s>>>(partial, (int)p.chunks, norm, total);
+        return xsg_launch_status("grad_norm");
+    });
 }
 
 extern "C" int xsg_clip_grads(const xsg_grad_tensor* ts, int n, int norm, double max_norm, double eps, float* total,
                               void* workspace, xsg_stream_t stream) {
     Plan p;
-    int rc = make_plan(ts, n, "clip_grads", &p);
+    int rc = make_plan(ts, n, "clip_grads", true, &p);
     if (rc == XSG_OK) rc = check_list(ts, n, norm, "clip_grads");
     if (rc != XSG_OK) return rc;
     if (!(max_norm >= 0.0) || !(eps >= 0.0))
@@ -809,32 +924,29 @@ extern "C" int xsg_clip_grads(const xsg_grad_tensor* ts, int n, int norm, double
     if (!total || !workspace) return xsg_fail(XSG_ERR_INVALID, "clip_grads: null output or workspace");
     rc = xsg_check_workspace(workspace, "clip_grads");
     if (rc != XSG_OK) return rc;
-    hipStream_t s = (hipStream_t)stream;
-    rc = launch_norm(ts, n, norm, p, total, nullptr, workspace, s);
-    if (rc != XSG_OK) return rc;
-    GradList list;
-    for (int i = 0; i < n;) {
-        const int k = fill_list(ts, n, i, p.chunk, &list);
-        if (list.first[k] > 0) {
-            clip_scale_kernel<<<list.first[k], kBlock, 0, s>>>(list, (const double*)workspace, max_norm, eps);
-            XSG_TRY_LAUNCH("clip_grads");
-        }
-        i += k;
-    }
-    return XSG_OK;
+    const hipStream_t s = (hipStream_t)stream;
+    return with_list(ts, n, p, workspace, s, [&](const auto& list) {
+        int status = launch_partials(list, norm, workspace, nullptr, s);
+        if (status != XSG_OK) return status;
+        NormParts parts;
+        status = join_parts(list.chunks, norm, workspace, s, &parts);
+        if (status != XSG_OK) return status;
+        clip_scale_kernel<<<std::max(list.chunks, 1), kBlock, 0, s>>>(list, parts, max_norm, eps, total);
+        return xsg_launch_status("clip_grads");
+    });
 }
 
 extern "C" size_t xsg_adam_step_workspace_bytes(const xsg_adam_tensor* ts, int n, const xsg_adam_options* o) {
     Plan p;
-    if (!o || make_plan(ts, n, "adam_step", &p) != XSG_OK) return 0;
-    return o->clip || o->skip_nonfinite ? partial_bytes(p.chunks) : 0;
+    return o && make_plan(ts, n, "adam_step", o->clip || o->skip_nonfinite, &p) == XSG_OK ? p.bytes : 0;
 }
 
 extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_options* o, int64_t* step, float* total,
                              void* workspace, xsg_stream_t stream) {
     if (!o || !step) return xsg_fail(XSG_ERR_INVALID, "adam_step: null options or step counter");
+    const bool needs_norm = o->clip || o->skip_nonfinite;
     Plan p;
-    int rc = make_plan(ts, n, "adam_step", &p);
+    int rc = make_plan(ts, n, "adam_step", needs_norm, &p);
     if (rc != XSG_OK) return rc;
     if (!(o->beta1 >= 0.0 && o->beta1 < 1.0 && o->beta2 >= 0.0 && o->beta2 < 1.0))
         return xsg_fail(XSG_ERR_INVALID, "adam_step: betas %g and %g must lie in [0, 1)", o->beta1, o->beta2);
@@ -848,21 +960,13 @@ extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_op
         rc = check_dtype(x.param_dtype, "adam_step", i);
         if (rc != XSG_OK) return rc;
     }
-    const bool needs_norm = o->clip || o->skip_nonfinite;
     rc = check_list(ts, n, needs_norm ? o->norm : XSG_NORM_L2, "adam_step");
     if (rc != XSG_OK) return rc;
-    hipStream_t s = (hipStream_t)stream;
-    const double* norm = nullptr;
-    if (needs_norm) {
+    if (p.bytes > 0) {
         if (!workspace) return xsg_fail(XSG_ERR_INVALID, "adam_step: null workspace");
         rc = xsg_check_workspace(workspace, "adam_step");
         if (rc != XSG_OK) return rc;
-        rc = launch_norm(ts, n, o->norm, p, total, nullptr, workspace, s);
-        if (rc != XSG_OK) return rc;
-        norm = (const double*)workspace;
     }
-    adam_count_kernel<<<1, 1, 0, s>>>(step);
-    XSG_TRY_LAUNCH("adam_step");
     AdamScalars a;
     a.log_beta1 = log(o->beta1);   // beta 0: -inf, and 1 - beta^k is 1
     a.log_beta2 = log(o->beta2);
@@ -873,38 +977,19 @@ extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_op
     a.clip = o->clip;
     a.skip_nonfinite = o->skip_nonfinite;
     a.max_norm = o->max_norm;
-    AdamList list;
-    for (int i = 0; i < n;) {
-        list.chunk = (int32_t)p.chunk;
-        int k = 0;
-        int32_t at = 0;
-        for (; k < kAdamMax && i + k < n; ++k) {
-            const xsg_adam_tensor& x = ts[i + k];
-            list.param[k] = x.param;
-            list.grad[k] = x.grad;
-            list.avg[k] = x.exp_avg;
-            list.sq[k] = x.exp_avg_sq;
-            list.numel[k] = x.numel;
-            list.mask[k] = x.mask;
-            const RowDiv div = row_div(x.numel, x.mask, x.rows);
-            list.row[k] = div.row;
-            list.magic[k] = div.magic;
-            list.shift[k] = (uint8_t)div.shift;
-            list.pdtype[k] = (uint8_t)x.param_dtype;
-            list.gdtype[k] = (uint8_t)x.grad_dtype;
-            list.lr[k] = (float)x.lr;
-            list.keep[k] = (float)(1.0 - x.lr * x.weight_decay);
-            list.first[k] = at;
-            at += (int32_t)chunks_of(x.numel, p.chunk);
+    const hipStream_t s = (hipStream_t)stream;
+    return with_list(ts, n, p, workspace, s, [&](const auto& list) {
+        NormParts parts{nullptr, -1, o->norm};
+        int status;
+        if (needs_norm) {
+            status = launch_partials(list, o->norm, workspace, step, s);
+            if (status == XSG_OK) status = join_parts(list.chunks, o->norm, workspace, s, &parts);
+        } else {
+            adam_count_kernel<<<1, 1, 0, s>>>(step);
+            status = xsg_launch_status("adam_step");
         }
-        list.first[k] = at;
-        list.n = k;
-        i += k;
-        const int last = i >= n;
-        if (at > 0 || last) {
-            adam_kernel<<<std::max(at, 1), kBlock, 0, s>>>(list, a, norm, step, last);
-            XSG_TRY_LAUNCH("adam_step");
-        }
-    }
-    return XSG_OK;
+        if (status != XSG_OK) return status;
+        adam_kernel<<<std::max(list.chunks, 1), kBlock, 0, s>>>(list, a, parts, step, total);
+        return xsg_launch_status("adam_step");
+    });
 }
