@@ -272,7 +272,8 @@ int xsg_grad_norm(const xsg_grad_tensor* tensors, int n, int norm, float* total,
 
 /* Scales the kept elements in place by min(1, max_norm / (norm + eps)), rounded once; a factor of 1 writes
  * nothing. total[1]: the norm before. A NaN norm makes every kept element NaN, an infinite one zeros them
- * (and NaN where they are infinite). Workspace as xsg_grad_norm's. */
+ * (and NaN where they are infinite). */
+size_t xsg_clip_grads_workspace_bytes(const xsg_grad_tensor* tensors, int n);
 int xsg_clip_grads(const xsg_grad_tensor* tensors, int n, int norm, double max_norm, double eps, float* total,
                    void* workspace, xsg_stream_t stream);
 
@@ -300,7 +301,8 @@ typedef struct {
  *   g = c grad;  m += (1 - beta1) (g - m);  v = beta2 v + (1 - beta2) g^2
  *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * c is the clip factor over all tensors (1 without clip); the gradients are not written. total[1], unless
- * NULL: the norm before clipping, with clip or skip_nonfinite (else not written, and no workspace needed). */
+ * NULL: the norm before clipping, with clip or skip_nonfinite (else not written). A workspace query of 0 takes a
+ * NULL workspace. */
 size_t xsg_adam_step_workspace_bytes(const xsg_adam_tensor* tensors, int n, const xsg_adam_options* options);
 int xsg_adam_step(const xsg_adam_tensor* tensors, int n, const xsg_adam_options* options, int64_t* step,
                   float* total, void* workspace, xsg_stream_t stream);

@@ -18,12 +18,18 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int64_t kChunkUnit = 1024;      // chunks are multiples of this many elements
-constexpr int64_t kTargetChunks = 2048;   // chunks of a call, when its tensors are long enough
-constexpr int64_t kMaxChunk = 1 << 30;    // offsets inside a chunk are 32-bit
+constexpr int64_t kTargetChunks = 2048;   // of a call whose tensors are long enough: every CU's eight workgroups
+// Longest chunk of a call that writes more than the caches hold: many short workgroups follow each other through
+// memory, where few long ones write in as many places at once (an update of 236 M elements: 2048 chunks 1310 us,
+// 57618 chunks 1230, around the caches 1145).
+constexpr int64_t kWriteChunk = 4096;
+constexpr int64_t kMaskedChunks = 4;      // such chunks to one of a masked tensor
+constexpr int64_t kMaxChunk = 1 << 26;    // offsets inside a chunk are 32-bit, in bytes
+constexpr int64_t kCacheBytes = (int64_t)256 << 20;   // of the last-level cache
 constexpr int64_t kMaxRow = 1 << 30;      // and so are rows under a mask
-constexpr int64_t kMaxElements = (int64_t)1 << 48;
+constexpr int64_t kMaxElements = (int64_t)1 << 41;
+constexpr int64_t kMaxChunks = 1 << 30;
 constexpr int kArgumentBytes = 3900;      // of a list, beside the other arguments in 4 KB
-constexpr int kJoinMax = 4096;            // partial sums that every workgroup joins by itself
 
 // Division of n < 2^31 by the row length: (mulhi(n, magic) + n) >> shift
 struct RowDiv {
@@ -31,6 +37,65 @@ struct RowDiv {
     uint32_t shift;
 };
 
+// round to nearest even; a NaN stays one
+XSG_DEV uint32_t bf16_bits(float x) {
+    const uint32_t u = __float_as_uint(x);
+    if (x != x) return (u >> 16) | 0x40u;
+    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+}
+
+// Elements of one type, one at a time or four at a time from a place aligned for that (16 bytes of float32, 8
+// of the others). A chunk's bytes fit 32 bits, so an access is a base held by the wavefront and a lane's offset.
+// STREAM: around the caches, for arrays that would only push each other out of them.
+#define XSG_GLOBAL __attribute__((address_space(1)))
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+template <typename V, bool STREAM = false> XSG_DEV V get(const void* p, uint32_t byte) {
+    const XSG_GLOBAL V* const q = (const XSG_GLOBAL V*)((const XSG_GLOBAL char*)p + byte);
+    return STREAM ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool STREAM = false, typename V> XSG_DEV void put(void* p, uint32_t byte, V x) {
+    XSG_GLOBAL V* const q = (XSG_GLOBAL V*)((XSG_GLOBAL char*)p + byte);
+    if (STREAM) __builtin_nontemporal_store(x, q);
+    else *q = x;
+}
+
+template <int DT> XSG_DEV float load1(const void* p, uint32_t i) {
+    if (DT == XSG_DTYPE_F32) return get<float>(p, 4 * i);
+    if (DT == XSG_DTYPE_BF16) return __uint_as_float((uint32_t)get<uint16_t>(p, 2 * i) << 16);
+    return (float)get<_Float16>(p, 2 * i);
+}
+template <int DT> XSG_DEV void store1(void* p, uint32_t i, float x) {
+    if (DT == XSG_DTYPE_F32) put(p, 4 * i, x);
+    else if (DT == XSG_DTYPE_BF16) put(p, 2 * i, (uint16_t)bf16_bits(x));
+    else put(p, 2 * i, (_Float16)x);
+}
+template <int DT, bool STREAM = false> XSG_DEV f32x4 load4(const void* p, uint32_t i) {
+    if (DT == XSG_DTYPE_F32) return get<f32x4, STREAM>(p, 4 * i);
+    if (DT == XSG_DTYPE_BF16) {
+        const u32x2 u = get<u32x2, STREAM>(p, 2 * i);
+        return f32x4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                     __uint_as_float(u.y & 0xffff0000u)};
+    }
+    return __builtin_convertvector(get<f16x4, STREAM>(p, 2 * i), f32x4);
+}
+template <int DT, bool STREAM = false> XSG_DEV void store4(void* p, uint32_t i, f32x4 x) {
+    if (DT == XSG_DTYPE_F32)
+        put<STREAM>(p, 4 * i, x);
+    else if (DT == XSG_DTYPE_BF16)
+        put<STREAM>(p, 2 * i, u32x2{bf16_bits(x.x) | bf16_bits(x.y) << 16, bf16_bits(x.z) | bf16_bits(x.w) << 16});
+    else
+        put<STREAM>(p, 2 * i, __builtin_convertvector(x, f16x4));
+}
+// those of x whose bit in keep is set
+template <int DT, bool STREAM> XSG_DEV void store4(void* p, uint32_t i, f32x4 x, uint32_t keep) {
+    if (keep == 15u) return store4<DT, STREAM>(p, i, x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if ((keep >> k) & 1) store1<DT>(p, i + k, x[k]);
+}
 struct GradEntry {
     void* data;
     int64_t numel;
@@ -57,15 +122,30 @@ struct AdamEntry {
 template <typename E> constexpr int kInline = kArgumentBytes / (sizeof(E) + 4);
 
 // first[t]: the first chunk of tensor t; first[n] = chunks
+// masked_chunk: the chunk of a masked tensor
 template <typename E> struct InlineList {
+    typedef E Entry;
     E entry[kInline<E>];
     int32_t first[kInline<E> + 1];
-    int32_t n, chunk, chunks;
+    int32_t n, chunk, masked_chunk, chunks;
+    XSG_DEV const E& at(int t) const { return entry[t]; }
+    XSG_DEV int32_t first_of(int t) const { return first[t]; }
 };
 template <typename E> struct TableList {
-    const E* __restrict__ entry;
-    const int32_t* __restrict__ first;
-    int32_t n, chunk, chunks;
+    typedef E Entry;
+    const E* entry;
+    const int32_t* first;
+    int32_t n, chunk, masked_chunk, chunks;
+    // t is the wavefront's: the entry comes by scalar loads, as an inline one does
+    XSG_DEV E at(int t) const {
+        typedef const uint64_t __attribute__((address_space(4)))* Words;
+        const Words w = (Words)(entry + t);
+        union { uint64_t words[sizeof(E) / 8]; E e; } u;
+#pragma unroll
+        for (int k = 0; k < (int)(sizeof(E) / 8); ++k) u.words[k] = w[k];
+        return u.e;
+    }
+    XSG_DEV int32_t first_of(int t) const { return get<int32_t>(first, 4 * t); }
 };
 // a piece of a table on its way to the workspace
 template <typename E> struct TablePiece {
@@ -86,46 +166,6 @@ __global__ __launch_bounds__(kBlock) void table_kernel(TablePiece<E> piece, E* _
     if (threadIdx.x < piece.n + last) first[threadIdx.x] = piece.first[threadIdx.x];
 }
 
-// round to nearest even; a NaN stays one
-XSG_DEV uint32_t bf16_bits(float x) {
-    const uint32_t u = __float_as_uint(x);
-    if (x != x) return (u >> 16) | 0x40u;
-    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-}
-
-// Elements of one type, one at a time or four at a time from a place aligned for that (16 bytes of float32, 8
-// of the others).
-template <int DT> XSG_DEV float load1(const void* p, uint32_t i) {
-    if (DT == XSG_DTYPE_F32) return ((const float*)p)[i];
-    if (DT == XSG_DTYPE_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
-    return (float)((const _Float16*)p)[i];
-}
-template <int DT> XSG_DEV void store1(void* p, uint32_t i, float x) {
-    if (DT == XSG_DTYPE_F32) ((float*)p)[i] = x;
-    else if (DT == XSG_DTYPE_BF16) ((uint16_t*)p)[i] = (uint16_t)bf16_bits(x);
-    else ((_Float16*)p)[i] = (_Float16)x;
-}
-template <int DT> XSG_DEV float4 load4(const void* p, uint32_t i) {
-    if (DT == XSG_DTYPE_F32) return *reinterpret_cast<const float4*>((const float*)p + i);
-    const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*)p + i);
-    if (DT == XSG_DTYPE_BF16)
-        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
-                           __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
-    union { uint2 u; _Float16 h[4]; } c{u};
-    return make_float4((float)c.h[0], (float)c.h[1], (float)c.h[2], (float)c.h[3]);
-}
-template <int DT> XSG_DEV void store4(void* p, uint32_t i, float4 x) {
-    if (DT == XSG_DTYPE_F32) {
-        *reinterpret_cast<float4*>((float*)p + i) = x;
-    } else if (DT == XSG_DTYPE_BF16) {
-        *reinterpret_cast<uint2*>((uint16_t*)p + i) =
-            make_uint2(bf16_bits(x.x) | bf16_bits(x.y) << 16, bf16_bits(x.z) | bf16_bits(x.w) << 16);
-    } else {
-        union { uint2 u; _Float16 h[4]; } c;
-        c.h[0] = (_Float16)x.x; c.h[1] = (_Float16)x.y; c.h[2] = (_Float16)x.z; c.h[3] = (_Float16)x.w;
-        *reinterpret_cast<uint2*>((uint16_t*)p + i) = c.u;
-    }
-}
 XSG_HD uint32_t type_size(int dtype) { return dtype == XSG_DTYPE_F32 ? 4 : 2; }
 XSG_DEV const void* at(const void* p, int64_t i, int dtype) { return (const char*)p + i * type_size(dtype); }
 XSG_DEV void* at(void* p, int64_t i, int dtype) { return (char*)p + i * type_size(dtype); }
@@ -157,13 +197,14 @@ struct ChunkMask {
     XSG_DEV uint32_t quotient(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
     XSG_DEV bool one(uint32_t i) const {
         const uint32_t r = bit + quotient(rem + i);
-        return (words[r >> 5] >> (r & 31)) & 1u;
+        return (word(r >> 5) >> (r & 31)) & 1u;
     }
+    XSG_DEV uint32_t word(uint32_t k) const { return get<uint32_t>(words, 4 * k); }
     // bit k: element i + k; all four lie in the chunk. Their rows span at most two words.
     XSG_DEV uint32_t four(uint32_t i) const {
         const uint32_t n = rem + i, q = quotient(n), r0 = bit + q;
         const uint32_t r3 = bit + quotient(n + 3);
-        const uint64_t w = (uint64_t)words[r0 >> 5] | (uint64_t)words[r3 >> 5] << 32;
+        const uint64_t w = (uint64_t)word(r0 >> 5) | (uint64_t)word(r3 >> 5) << 32;
         uint32_t at = n - q * row, r = r0 & 31, keep = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -181,7 +222,7 @@ template <typename L> XSG_DEV int find_tensor(const L& list, int b) {
     int lo = 0, n = list.n;
     for (;;) {
         const int step = (n + 63) >> 6, i = lane * step;
-        const int below = __popcll(__ballot(i < n && list.first[lo + min(i, n - 1)] <= b)) - 1;
+        const int below = __popcll(__ballot(i < n && list.first_of(lo + min(i, n - 1)) <= b)) - 1;
         lo += below * step;
         n = min(step, n - below * step);
         if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
@@ -240,24 +281,38 @@ struct ChunkSpan {
     XSG_DEV uint32_t tail_at() const { return head + 4 * groups; }
 };
 
-constexpr int kUnroll = 4;   // groups in flight per thread
-
-// one(i): a single element; many(i[], keep[]): kUnroll groups, of which those with keep 0 are left out
-template <bool MASK, typename One, typename Many>
+// many(i[], keep[], all): UNROLL groups, of which those with keep 0 are left out; `all` is a constant that says
+// that every group is there and kept. one(i): a single element.
+template <bool MASK, int UNROLL, typename One, typename Many>
 XSG_DEV void for_chunk(const ChunkSpan& span, const ChunkMask& mask, One&& one, Many&& many) {
-    for (uint32_t g = threadIdx.x; g < span.groups; g += kBlock * kUnroll) {
-        uint32_t i[kUnroll], keep[kUnroll];
+    constexpr uint32_t tile = kBlock * UNROLL;
+    const uint32_t whole = span.groups / tile * tile;
+    uint32_t g = threadIdx.x, i[UNROLL], keep[UNROLL];
+#pragma unroll 1
+    for (; g < whole; g += tile) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < UNROLL; ++u) {
+            i[u] = span.head + 4 * (g + u * kBlock);
+            keep[u] = MASK ? mask.four(i[u]) : 15u;
+        }
+        many(i, keep, std::integral_constant<bool, !MASK>{});
+    }
+    if (whole < span.groups) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
             i[u] = span.head + 4 * (g + u * kBlock);
             keep[u] = g + u * kBlock < span.groups ? (MASK ? mask.four(i[u]) : 15u) : 0u;
         }
-        many(i, keep);
+        many(i, keep, std::false_type{});
     }
     if (threadIdx.x < span.head && (!MASK || mask.one(threadIdx.x))) one(threadIdx.x);
-    const uint32_t i = span.tail_at() + threadIdx.x;
-    if (threadIdx.x < span.tail && (!MASK || mask.one(i))) one(i);
+#pragma unroll 1
+    for (uint32_t k = span.tail_at() + threadIdx.x; k < span.tail_at() + span.tail; k += kBlock)
+        if (!MASK || mask.one(k)) one(k);
 }
+
+constexpr int kUnroll = 4;       // groups in flight per thread: of one array
+constexpr int kAdamUnroll = 2;   // and of four
 
 // Under a mask of short rows each wavefront lists the kept rows of its share of the chunk (a mask word a lane, so
 // up to 2048 rows for one load's latency) and then walks their elements alone, VEC at a time, so that lanes are
@@ -277,11 +332,12 @@ XSG_DEV void for_kept_rows(const ChunkMask& mask, uint32_t count, Many&& many) {
     const auto word_of = [&](uint32_t first) {   // bits of rows outside lo..hi are cleared
         const uint32_t at = first + 32 * lane;
         if (at >= hi) return 0u;
-        uint32_t w = mask.words[at >> 5];
+        uint32_t w = mask.word(at >> 5);
         if (at < lo) w &= 0xffffffffu << (lo - at);   // lo lies in the first word
         return hi - at < 32 ? w & ~(0xffffffffu << (hi - at)) : w;
     };
     uint32_t next = word_of(lo & ~31u);
+#pragma unroll 1
     for (uint32_t batch = lo & ~31u; batch < hi; batch += kRowBatch) {
         uint32_t word = next, upto = (uint32_t)__popc(word);
         next = word_of(batch + kRowBatch);
@@ -295,6 +351,7 @@ XSG_DEV void for_kept_rows(const ChunkMask& mask, uint32_t count, Many&& many) {
             list[k++] = (uint16_t)(32 * lane + __ffs(word) - 1);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         const uint32_t total = n * units;
+#pragma unroll 1
         for (uint32_t w0 = lane; w0 < total; w0 += 64 * UNROLL) {
             uint32_t i[UNROLL];
             bool on[UNROLL];
@@ -314,79 +371,69 @@ XSG_DEV void for_kept_rows(const ChunkMask& mask, uint32_t count, Many&& many) {
     }
 }
 
-template <int NORM, int DT>
-XSG_DEV Accum<NORM> rows_norm(const void* p, uint32_t count, bool whole, const ChunkMask& mask) {
-    Accum<NORM> acc[4];
-    if (whole) {
-        for_kept_rows<4, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
-            float4 x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = on[u] ? load4<DT>(p, i[u]) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                acc[u].add(x[u].x);
-                acc[u].add(x[u].y);
-                acc[u].add(x[u].z);
-                acc[u].add(x[u].w);
-            }
-        });
-    } else {
-        for_kept_rows<1, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
-            float x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = on[u] ? load1<DT>(p, i[u]) : 0.f;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) acc[u].add(x[u]);
-        });
-    }
-#pragma unroll
-    for (int u = 1; u < 4; ++u) acc[0].join(acc[u]);
-    return acc[0];
-}
-
-template <int DT> XSG_DEV void rows_scale(void* p, float c, uint32_t count, bool whole, const ChunkMask& mask) {
-    if (whole) {
-        for_kept_rows<4, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
-            float4 x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (on[u]) x[u] = load4<DT>(p, i[u]);
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (on[u]) store4<DT>(p, i[u], make_float4(x[u].x * c, x[u].y * c, x[u].z * c, x[u].w * c));
-        });
-    } else {
-        for_kept_rows<1, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
-            float x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (on[u]) x[u] = load1<DT>(p, i[u]);
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (on[u]) store1<DT>(p, i[u], x[u] * c);
-        });
-    }
-}
-
-template <int NORM, int DT, bool MASK>
-XSG_DEV Accum<NORM> chunk_norm(const void* p, const ChunkSpan& span, const ChunkMask& mask) {
+template <int NORM> struct AccumSet {   // one for each group in flight
     Accum<NORM> acc[kUnroll];
-    for_chunk<MASK>(span, mask, [&](uint32_t i) { acc[0].add(load1<DT>(p, i)); },
-                    [&](const uint32_t* i, const uint32_t* keep) {
-        float4 x[kUnroll];
+    XSG_DEV void add(int u, f32x4 x) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) x[u] = keep[u] ? load4<DT>(p, i[u]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < 4; ++k) acc[u].add(x[k]);
+    }
+    XSG_DEV Accum<NORM> joined() {
+#pragma unroll
+        for (int u = 1; u < kUnroll; ++u) acc[0].join(acc[u]);
+        return acc[0];
+    }
+};
+
+template <int NORM, int DT, bool MASK, bool STREAM>
+XSG_DEV Accum<NORM> chunk_norm(const void* p, const ChunkSpan& span, const ChunkMask& mask) {
+    AccumSet<NORM> acc;
+    for_chunk<MASK, kUnroll>(span, mask, [&](uint32_t i) { acc.acc[0].add(load1<DT>(p, i)); },
+                             [&](const uint32_t* i, const uint32_t* keep, auto all) {
+        f32x4 x[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            acc[u].add(!MASK || (keep[u] & 1) ? x[u].x : 0.f);
-            acc[u].add(!MASK || (keep[u] & 2) ? x[u].y : 0.f);
-            acc[u].add(!MASK || (keep[u] & 4) ? x[u].z : 0.f);
-            acc[u].add(!MASK || (keep[u] & 8) ? x[u].w : 0.f);
+            x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (all.value || keep[u]) x[u] = load4<DT, STREAM>(p, i[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            if (MASK) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[u][k] = (keep[u] >> k) & 1 ? x[u][k] : 0.f;
+            }
+            acc.add(u, x[u]);
         }
     });
+    return acc.joined();
+}
+
+template <int NORM, int DT>
+XSG_DEV Accum<NORM> rows_norm(const void* p, uint32_t count, bool whole, const ChunkMask& mask) {
+    AccumSet<NORM> acc;
+    if (whole) {
+        for_kept_rows<4, kUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
+            f32x4 x[kUnroll];
 #pragma unroll
-    for (int u = 1; u < kUnroll; ++u) acc[0].join(acc[u]);
-    return acc[0];
+            for (int u = 0; u < kUnroll; ++u) {
+                x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (on[u]) x[u] = load4<DT>(p, i[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) acc.add(u, x[u]);
+        });
+    } else {
+        for_kept_rows<1, kUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
+            float x[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                x[u] = 0.f;
+                if (on[u]) x[u] = load1<DT>(p, i[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) acc.acc[u].add(x[u]);
+        });
+    }
+    return acc.joined();
 }
 
 // calls f with the type as a constant
@@ -401,35 +448,40 @@ struct Chunk {
     int64_t base;
     uint32_t count;
     template <typename L, typename E> XSG_DEV Chunk(const L& list, const E& e, int b, int t) {
-        base = (int64_t)(b - list.first[t]) * list.chunk;
-        count = (uint32_t)min((int64_t)list.chunk, e.numel - base);
+        const int64_t size = e.mask ? list.masked_chunk : list.chunk;
+        base = (b - list.first_of(t)) * size;
+        count = (uint32_t)min(size, e.numel - base);
     }
 };
 
-// `step`, unless null, counts one step more; the launches behind this one read it.
-template <int NORM, typename L>
-__global__ __launch_bounds__(kBlock) void norm_partial_kernel(L list, double* __restrict__ partial, int64_t* step) {
-    const int b = blockIdx.x;
-    if (step && b == 0 && threadIdx.x == 0) *step += 1;
-    if (b >= list.chunks) return;   // no elements at all
-    const int t = find_tensor(list, b);
-    const auto& e = list.entry[t];
-    const Chunk chunk(list, e, b, t);
-    const int dtype = e.grad_dtype();
-    const void* p = at(e.grad(), chunk.base, dtype);
-    const ChunkSpan span(chunk.count, phase_of(p, dtype));
-    ChunkMask mask;
+// A workgroup sums `each` chunks in a row. `step`, unless null, counts one step more; the launches behind this
+// one read it.
+template <int NORM, bool STREAM, typename L>
+__global__ __launch_bounds__(kBlock) void norm_partial_kernel(L list, int each, double* __restrict__ partial,
+                                                              int64_t* step) {
     __shared__ uint16_t listed[kBlock / 64 * kRowBatch];
-    mask.list = listed;
-    if (e.mask) mask.open(e.mask, chunk.base, e.row, e.magic, e.shift);
+    if (step && blockIdx.x == 0 && threadIdx.x == 0) *step += 1;
     Accum<NORM> acc;
-    with_type(dtype, [&](auto dt) {
-        if (!e.mask) acc = chunk_norm<NORM, dt.value, false>(p, span, mask);
-        else if (mask.row > kShortRow) acc = chunk_norm<NORM, dt.value, true>(p, span, mask);
-        else acc = rows_norm<NORM, dt.value>(p, chunk.count, span.head == 0 && mask.row % 4 == 0, mask);
-    });
+    const int end = min(((int)blockIdx.x + 1) * each, list.chunks);
+#pragma unroll 1
+    for (int b = blockIdx.x * each; b < end; ++b) {
+        const int t = find_tensor(list, b);
+        const auto& e = list.at(t);
+        const Chunk chunk(list, e, b, t);
+        const int dtype = e.grad_dtype();
+        const void* p = at(e.grad(), chunk.base, dtype);
+        const ChunkSpan span(chunk.count, phase_of(p, dtype));
+        ChunkMask mask;
+        mask.list = listed;
+        if (e.mask) mask.open(e.mask, chunk.base, e.row, e.magic, e.shift);
+        with_type(dtype, [&](auto dt) {
+            if (!e.mask) acc.join(chunk_norm<NORM, dt.value, false, STREAM>(p, span, mask));
+            else if (mask.row > kShortRow) acc.join(chunk_norm<NORM, dt.value, true, STREAM>(p, span, mask));
+            else acc.join(rows_norm<NORM, dt.value>(p, chunk.count, span.head == 0 && mask.row % 4 == 0, mask));
+        });
+    }
     acc = block_join<NORM>(acc);
-    if (threadIdx.x == 0) partial[b] = acc.value();
+    if (threadIdx.x == 0) partial[blockIdx.x] = acc.value();
 }
 
 template <int NORM> XSG_DEV Accum<NORM> join_partials(const double* __restrict__ partial, int n) {
@@ -445,16 +497,6 @@ XSG_DEV double norm_of(const double* __restrict__ partial, int n, int norm) {
     return join_partials<XSG_NORM_INF>(partial, n).finish();
 }
 
-// Many partial sums become one, where each workgroup of the next launch would join them all again.
-__global__ __launch_bounds__(kBlock) void norm_reduce_kernel(const double* __restrict__ partial, int n, int norm,
-                                                             double* __restrict__ one) {
-    double v;
-    if (norm == XSG_NORM_L2) v = join_partials<XSG_NORM_L2>(partial, n).value();
-    else if (norm == XSG_NORM_L1) v = join_partials<XSG_NORM_L1>(partial, n).value();
-    else v = join_partials<XSG_NORM_INF>(partial, n).value();
-    if (threadIdx.x == 0) *one = v;
-}
-
 __global__ __launch_bounds__(kBlock) void norm_total_kernel(const double* __restrict__ partial, int n, int norm,
                                                             float* __restrict__ total) {
     const double v = norm_of(partial, n, norm);
@@ -466,7 +508,7 @@ template <typename L>
 __global__ __launch_bounds__(kBlock) void norm_each_kernel(L list, const double* __restrict__ partial, int norm,
                                                            float* __restrict__ total, float* __restrict__ each) {
     const int t = blockIdx.x;
-    const int lo = t < list.n ? list.first[t] : 0, hi = t < list.n ? list.first[t + 1] : list.chunks;
+    const int lo = t < list.n ? list.first_of(t) : 0, hi = t < list.n ? list.first_of(t + 1) : list.chunks;
     const double v = norm_of(partial + lo, hi - lo, norm);
     if (threadIdx.x == 0) *(t < list.n ? each + t : total) = (float)v;
 }
@@ -477,45 +519,116 @@ XSG_DEV float clip_factor(double norm, double max_norm, double eps) {
     return c > 1.0 ? 1.0f : (float)c;
 }
 
-template <int DT, bool MASK>
+// What a call that writes takes from the norm and the step counter.
+struct StepTerms {
+    float c;        // the clip factor
+    float over1;    // 1 / (1 - beta1^t)
+    float root;     // 1 / sqrt(1 - beta2^t)
+    int taken;      // 0: the step is left out
+};
+
+struct StepRule {
+    double max_norm, clip_eps;
+    double log_beta1, log_beta2;   // natural logarithms
+    int norm;                      // the kind; -1: none is computed
+    int clip, skip_nonfinite;
+};
+
+// In every thread of the workgroup; the first workgroup also gives the norm out and takes the counter back where
+// the step is not taken (no other one reads it then). The counter already counts this step.
+XSG_DEV StepTerms step_terms(const StepRule& rule, const double* __restrict__ partial, int n, int64_t* step,
+                             float* __restrict__ total) {
+    StepTerms terms{1.0f, 1.0f, 1.0f, 1};
+    const bool first = blockIdx.x == 0 && threadIdx.x == 0;
+    if (rule.norm >= 0) {
+        const double norm = norm_of(partial, n, rule.norm);
+        if (first && total) *total = (float)norm;
+        if (rule.clip) terms.c = clip_factor(norm, rule.max_norm, rule.clip_eps);
+        if (rule.skip_nonfinite && !(norm < (double)INFINITY)) {
+            if (first) *step -= 1;
+            terms.taken = 0;
+            return terms;
+        }
+    }
+    if (step) {   // 1 - beta^t without the cancellation, by one wavefront: in 64 bits it is not cheap
+        __shared__ float corrections[2];
+        if (threadIdx.x < 64) {
+            const double t = (double)*step;
+            corrections[0] = (float)(-1.0 / expm1(t * rule.log_beta1));
+            corrections[1] = (float)(1.0 / sqrt(-expm1(t * rule.log_beta2)));
+        }
+        __syncthreads();
+        terms.over1 = corrections[0];
+        terms.root = corrections[1];
+    }
+    return terms;
+}
+
+// Of many partial sums the terms are made once, in a launch of their own.
+__global__ __launch_bounds__(kBlock) void step_terms_kernel(StepRule rule, const double* __restrict__ partial, int n,
+                                                            int64_t* step, float* __restrict__ total,
+                                                            StepTerms* __restrict__ ready) {
+    const StepTerms terms = step_terms(rule, partial, n, step, total);
+    if (threadIdx.x == 0) *ready = terms;
+}
+
+// Where a launch that writes has its terms from: made before, or its own to make from the partial sums.
+struct StepSource {
+    StepRule rule;
+    const double* __restrict__ partial;
+    int n;
+    int64_t* step;
+    float* __restrict__ total;
+    const StepTerms* __restrict__ ready;
+    XSG_DEV StepTerms terms() const { return ready ? *ready : step_terms(rule, partial, n, step, total); }
+};
+
+template <int DT, bool MASK, bool STREAM>
 XSG_DEV void chunk_scale(void* p, float c, const ChunkSpan& span, const ChunkMask& mask) {
-    for_chunk<MASK>(span, mask, [&](uint32_t i) { store1<DT>(p, i, load1<DT>(p, i) * c); },
-                    [&](const uint32_t* i, const uint32_t* keep) {
-        float4 x[kUnroll];
+    for_chunk<MASK, kUnroll>(span, mask, [&](uint32_t i) { store1<DT>(p, i, load1<DT>(p, i) * c); },
+                             [&](const uint32_t* i, const uint32_t* keep, auto all) {
+        f32x4 x[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-            if (keep[u]) x[u] = load4<DT>(p, i[u]);
+            if (all.value || keep[u]) x[u] = load4<DT, STREAM>(p, i[u]);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const float4 y = make_float4(x[u].x * c, x[u].y * c, x[u].z * c, x[u].w * c);
-            if (keep[u] == 15u) {
-                store4<DT>(p, i[u], y);
-            } else if (keep[u]) {
-                if (keep[u] & 1) store1<DT>(p, i[u], y.x);
-                if (keep[u] & 2) store1<DT>(p, i[u] + 1, y.y);
-                if (keep[u] & 4) store1<DT>(p, i[u] + 2, y.z);
-                if (keep[u] & 8) store1<DT>(p, i[u] + 3, y.w);
-            }
-        }
+        for (int u = 0; u < kUnroll; ++u)
+            if (all.value || keep[u]) store4<DT, STREAM>(p, i[u], x[u] * c, all.value ? 15u : keep[u]);
     });
 }
 
-// The norm that a launch clips by: partial sums, how many, and what kind.
-struct NormParts {
-    const double* __restrict__ partial;
-    int n, norm;
-};
+template <int DT, bool STREAM>
+XSG_DEV void rows_scale(void* p, float c, uint32_t count, bool whole, const ChunkMask& mask) {
+    if (whole) {
+        for_kept_rows<4, kUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
+            f32x4 x[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                if (on[u]) x[u] = load4<DT>(p, i[u]);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                if (on[u]) store4<DT, STREAM>(p, i[u], x[u] * c);
+        });
+    } else {
+        for_kept_rows<1, kUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
+            float x[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                if (on[u]) x[u] = load1<DT>(p, i[u]);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                if (on[u]) store1<DT>(p, i[u], x[u] * c);
+        });
+    }
+}
 
-template <typename L>
-__global__ __launch_bounds__(kBlock) void clip_scale_kernel(L list, NormParts parts, double max_norm, double eps,
-                                                            float* __restrict__ total) {
-    const double norm = norm_of(parts.partial, parts.n, parts.norm);
-    const int b = blockIdx.x;
-    if (b == 0 && threadIdx.x == 0) *total = (float)norm;
-    const float c = clip_factor(norm, max_norm, eps);
-    if (c == 1.0f || b >= list.chunks) return;   // the values stay as they are
+template <bool STREAM, typename L>
+__global__ __launch_bounds__(kBlock) void clip_scale_kernel(L list, StepSource source) {
+    const float c = source.terms().c;
+    const int b = list.chunks - 1 - (int)blockIdx.x;
+    if (c == 1.0f || b < 0) return;   // the values stay as they are
     const int t = find_tensor(list, b);
-    const auto& e = list.entry[t];
+    const auto& e = list.at(t);
     const Chunk chunk(list, e, b, t);
     const int dtype = e.dtype;
     void* p = at(e.data, chunk.base, dtype);
@@ -525,17 +638,14 @@ __global__ __launch_bounds__(kBlock) void clip_scale_kernel(L list, NormParts pa
     mask.list = listed;
     if (e.mask) mask.open(e.mask, chunk.base, e.row, e.magic, e.shift);
     with_type(dtype, [&](auto dt) {
-        if (!e.mask) chunk_scale<dt.value, false>(p, c, span, mask);
-        else if (mask.row > kShortRow) chunk_scale<dt.value, true>(p, c, span, mask);
-        else rows_scale<dt.value>(p, c, chunk.count, span.head == 0 && mask.row % 4 == 0, mask);
+        if (!e.mask) chunk_scale<dt.value, false, STREAM>(p, c, span, mask);
+        else if (mask.row > kShortRow) chunk_scale<dt.value, true, STREAM>(p, c, span, mask);
+        else rows_scale<dt.value, STREAM>(p, c, chunk.count, span.head == 0 && mask.row % 4 == 0, mask);
     });
 }
 
 struct AdamScalars {
-    double log_beta1, log_beta2;   // natural logarithms
     float beta2, one_minus_beta1, one_minus_beta2, eps;
-    int clip, skip_nonfinite;
-    double max_norm;
 };
 constexpr double kAdamClipEps = 1e-6;
 
@@ -559,142 +669,118 @@ struct AdamArrays {
     float *m, *v;
 };
 
-template <int PT, int GT> XSG_DEV void adam_one(const AdamArrays& a, const AdamTerms& s, uint32_t i) {
-    float p = load1<PT>(a.p, i), m = a.m[i], v = a.v[i];
-    s.update(p, load1<GT>(a.g, i), m, v);
-    store1<PT>(a.p, i, p);
-    a.m[i] = m;
-    a.v[i] = v;
-}
-
-constexpr int kAdamUnroll = 2;
-
-template <int PT, int GT, bool MASK>
-XSG_DEV void chunk_adam(const AdamArrays& a, const AdamTerms& s, const ChunkSpan& span, const ChunkMask& mask) {
-    for (uint32_t g0 = threadIdx.x; g0 < span.groups; g0 += kBlock * kAdamUnroll) {
-        uint32_t i[kAdamUnroll], keep[kAdamUnroll];
-        float4 p[kAdamUnroll], g[kAdamUnroll], m[kAdamUnroll], v[kAdamUnroll];
+// One element, or four, of the four arrays.
+template <int PT, int GT> struct Adam1 {
+    float p, g, m, v;
+    XSG_DEV void load(const AdamArrays& a, uint32_t i) {
+        p = load1<PT>(a.p, i);
+        g = load1<GT>(a.g, i);
+        m = load1<XSG_DTYPE_F32>(a.m, i);
+        v = load1<XSG_DTYPE_F32>(a.v, i);
+    }
+    XSG_DEV void update(const AdamTerms& s) { s.update(p, g, m, v); }
+    XSG_DEV void store(const AdamArrays& a, uint32_t i) const {
+        store1<PT>(a.p, i, p);
+        store1<XSG_DTYPE_F32>(a.m, i, m);
+        store1<XSG_DTYPE_F32>(a.v, i, v);
+    }
+};
+template <int PT, int GT, bool STREAM> struct Adam4 {
+    f32x4 p, g, m, v;
+    XSG_DEV void load(const AdamArrays& a, uint32_t i) {
+        p = load4<PT, STREAM>(a.p, i);
+        g = load4<GT, STREAM>(a.g, i);
+        m = load4<XSG_DTYPE_F32, STREAM>(a.m, i);
+        v = load4<XSG_DTYPE_F32, STREAM>(a.v, i);
+    }
+    XSG_DEV void update(const AdamTerms& s) {
 #pragma unroll
-        for (int u = 0; u < kAdamUnroll; ++u) {
-            i[u] = span.head + 4 * (g0 + u * kBlock);
-            keep[u] = g0 + u * kBlock < span.groups ? (MASK ? mask.four(i[u]) : 15u) : 0u;
-        }
-#pragma unroll
-        for (int u = 0; u < kAdamUnroll; ++u) {
-            if (keep[u]) {
-                p[u] = load4<PT>(a.p, i[u]);
-                g[u] = load4<GT>(a.g, i[u]);
-                m[u] = load4<XSG_DTYPE_F32>(a.m, i[u]);
-                v[u] = load4<XSG_DTYPE_F32>(a.v, i[u]);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kAdamUnroll; ++u) {
-            if (!keep[u]) continue;
-            s.update(p[u].x, g[u].x, m[u].x, v[u].x);
-            s.update(p[u].y, g[u].y, m[u].y, v[u].y);
-            s.update(p[u].z, g[u].z, m[u].z, v[u].z);
-            s.update(p[u].w, g[u].w, m[u].w, v[u].w);
-            if (keep[u] == 15u) {
-                store4<PT>(a.p, i[u], p[u]);
-                store4<XSG_DTYPE_F32>(a.m, i[u], m[u]);
-                store4<XSG_DTYPE_F32>(a.v, i[u], v[u]);
-            } else {
-                const float pe[4] = {p[u].x, p[u].y, p[u].z, p[u].w}, me[4] = {m[u].x, m[u].y, m[u].z, m[u].w},
-                            ve[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (!((keep[u] >> k) & 1)) continue;
-                    store1<PT>(a.p, i[u] + k, pe[k]);
-                    a.m[i[u] + k] = me[k];
-                    a.v[i[u] + k] = ve[k];
-                }
-            }
+        for (int k = 0; k < 4; ++k) {
+            float pk = p[k], mk = m[k], vk = v[k];
+            s.update(pk, g[k], mk, vk);
+            p[k] = pk;
+            m[k] = mk;
+            v[k] = vk;
         }
     }
-    if (threadIdx.x < span.head && (!MASK || mask.one(threadIdx.x))) adam_one<PT, GT>(a, s, threadIdx.x);
-    for (uint32_t i = span.tail_at() + threadIdx.x, end = span.tail_at() + span.tail; i < end; i += kBlock)
-        if (!MASK || mask.one(i)) adam_one<PT, GT>(a, s, i);
+    XSG_DEV void store(const AdamArrays& a, uint32_t i, uint32_t keep) const {
+        store4<PT, STREAM>(a.p, i, p, keep);
+        store4<XSG_DTYPE_F32, STREAM>(a.m, i, m, keep);
+        store4<XSG_DTYPE_F32, STREAM>(a.v, i, v, keep);
+    }
+};
+
+template <int PT, int GT, bool MASK, bool STREAM>
+XSG_DEV void chunk_adam(const AdamArrays& a, const AdamTerms& s, const ChunkSpan& span, const ChunkMask& mask) {
+    for_chunk<MASK, kAdamUnroll>(span, mask, [&](uint32_t i) {
+        Adam1<PT, GT> x;
+        x.load(a, i);
+        x.update(s);
+        x.store(a, i);
+    }, [&](const uint32_t* i, const uint32_t* keep, auto all) {
+        Adam4<PT, GT, STREAM> x[kAdamUnroll];
+#pragma unroll
+        for (int u = 0; u < kAdamUnroll; ++u)
+            if (all.value || keep[u]) x[u].load(a, i[u]);
+#pragma unroll
+        for (int u = 0; u < kAdamUnroll; ++u) {
+            if (!(all.value || keep[u])) continue;
+            x[u].update(s);
+            x[u].store(a, i[u], all.value ? 15u : keep[u]);
+        }
+    });
 }
 
-template <int PT, int GT>
+template <int PT, int GT, bool STREAM>
 XSG_DEV void rows_adam(const AdamArrays& a, const AdamTerms& s, uint32_t count, bool whole, const ChunkMask& mask) {
     if (whole) {
         for_kept_rows<4, kAdamUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
-            float4 p[kAdamUnroll], g[kAdamUnroll], m[kAdamUnroll], v[kAdamUnroll];
+            Adam4<PT, GT, STREAM> x[kAdamUnroll];
+#pragma unroll
+            for (int u = 0; u < kAdamUnroll; ++u)
+                if (on[u]) x[u].load(a, i[u]);
 #pragma unroll
             for (int u = 0; u < kAdamUnroll; ++u) {
                 if (!on[u]) continue;
-                p[u] = load4<PT>(a.p, i[u]);
-                g[u] = load4<GT>(a.g, i[u]);
-                m[u] = load4<XSG_DTYPE_F32>(a.m, i[u]);
-                v[u] = load4<XSG_DTYPE_F32>(a.v, i[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < kAdamUnroll; ++u) {
-                if (!on[u]) continue;
-                s.update(p[u].x, g[u].x, m[u].x, v[u].x);
-                s.update(p[u].y, g[u].y, m[u].y, v[u].y);
-                s.update(p[u].z, g[u].z, m[u].z, v[u].z);
-                s.update(p[u].w, g[u].w, m[u].w, v[u].w);
-                store4<PT>(a.p, i[u], p[u]);
-                store4<XSG_DTYPE_F32>(a.m, i[u], m[u]);
-                store4<XSG_DTYPE_F32>(a.v, i[u], v[u]);
+                x[u].update(s);
+                x[u].store(a, i[u], 15u);
             }
         });
     } else {
-        for_kept_rows<1, 4>(mask, count, [&](const uint32_t* i, const bool* on) {
-            float p[4], g[4], m[4], v[4];
+        for_kept_rows<1, kUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
+            Adam1<PT, GT> x[kUnroll];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (!on[u]) continue;
-                p[u] = load1<PT>(a.p, i[u]);
-                g[u] = load1<GT>(a.g, i[u]);
-                m[u] = a.m[i[u]];
-                v[u] = a.v[i[u]];
-            }
+            for (int u = 0; u < kUnroll; ++u)
+                if (on[u]) x[u].load(a, i[u]);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < kUnroll; ++u) {
                 if (!on[u]) continue;
-                s.update(p[u], g[u], m[u], v[u]);
-                store1<PT>(a.p, i[u], p[u]);
-                a.m[i[u]] = m[u];
-                a.v[i[u]] = v[u];
+                x[u].update(s);
+                x[u].store(a, i[u]);
             }
         });
     }
 }
 
-// parts.n < 0: no norm. The counter already counts this step; it is taken back where the step is not taken.
-template <typename L>
-__global__ __launch_bounds__(kBlock) void adam_kernel(L list, AdamScalars s, NormParts parts, int64_t* step,
-                                                      float* __restrict__ total) {
-    const int b = blockIdx.x;
-    AdamTerms terms;
-    terms.c = 1.0f;
-    if (parts.n >= 0) {
-        const double norm = norm_of(parts.partial, parts.n, parts.norm);
-        if (total && b == 0 && threadIdx.x == 0) *total = (float)norm;
-        if (s.skip_nonfinite && !(norm < (double)INFINITY)) {
-            if (b == 0 && threadIdx.x == 0) *step -= 1;   // no other workgroup reads the counter in this case
-            return;
-        }
-        if (s.clip) terms.c = clip_factor(norm, s.max_norm, kAdamClipEps);
-    }
-    if (b >= list.chunks) return;
+// F32: every parameter and gradient is float32
+template <bool F32, bool STREAM, typename L>
+__global__ __launch_bounds__(kBlock) void adam_kernel(L list, AdamScalars s, StepSource source) {
+    const StepTerms now = source.terms();
+    const int b = list.chunks - 1 - (int)blockIdx.x;
+    if (!now.taken || b < 0) return;
     const int t = find_tensor(list, b);
-    const auto& e = list.entry[t];
+    const auto& e = list.at(t);
     const Chunk chunk(list, e, b, t);
-    const double k = (double)*step;
-    // 1 - beta^k without the cancellation
-    terms.rate = (float)(e.lr / -expm1(k * s.log_beta1));
-    terms.root = (float)(1.0 / sqrt(-expm1(k * s.log_beta2)));
+    AdamTerms terms;
+    terms.c = now.c;
+    terms.rate = e.lr * now.over1;
+    terms.root = now.root;
     terms.beta2 = s.beta2;
     terms.one_minus_beta1 = s.one_minus_beta1;
     terms.one_minus_beta2 = s.one_minus_beta2;
     terms.eps = s.eps;
     terms.keep = e.keep;
-    const int pt = e.pdtype, gt = e.gdtype;
+    const int pt = F32 ? XSG_DTYPE_F32 : e.pdtype, gt = F32 ? XSG_DTYPE_F32 : e.gdtype;
     const AdamArrays a{at(e.param, chunk.base, pt), at(e.gradient, chunk.base, gt), e.avg + chunk.base,
                        e.sq + chunk.base};
     const uint32_t phase = phase_of(a.p, pt);
@@ -708,22 +794,26 @@ __global__ __launch_bounds__(kBlock) void adam_kernel(L list, AdamScalars s, Nor
     __shared__ uint16_t listed[kBlock / 64 * kRowBatch];
     mask.list = listed;
     if (e.mask) mask.open(e.mask, chunk.base, e.row, e.magic, e.shift);
-    with_type(pt, [&](auto p) {
-        with_type(gt, [&](auto g) {
-            if (!e.mask) chunk_adam<p.value, g.value, false>(a, terms, span, mask);
-            else if (mask.row > kShortRow) chunk_adam<p.value, g.value, true>(a, terms, span, mask);
-            else rows_adam<p.value, g.value>(a, terms, chunk.count, whole, mask);
-        });
-    });
+    const auto run = [&](auto p, auto g) {
+        if (!e.mask) chunk_adam<p.value, g.value, false, STREAM>(a, terms, span, mask);
+        else if (mask.row > kShortRow) chunk_adam<p.value, g.value, true, STREAM>(a, terms, span, mask);
+        else rows_adam<p.value, g.value, STREAM>(a, terms, chunk.count, whole, mask);
+    };
+    if constexpr (F32) {
+        const std::integral_constant<int, XSG_DTYPE_F32> f32;
+        run(f32, f32);
+    } else {
+        with_type(pt, [&](auto p) { with_type(gt, [&](auto g) { run(p, g); }); });
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host
-int64_t chunk_for(int64_t elements) {
+int64_t chunk_for(int64_t elements, bool writes_far) {
     int64_t c = (elements + kTargetChunks - 1) / kTargetChunks;
     c = (c + kChunkUnit - 1) / kChunkUnit * kChunkUnit;
-    return std::min(std::max(c, kChunkUnit), kMaxChunk);
+    return std::min(std::max(c, kChunkUnit), writes_far ? kWriteChunk : kMaxChunk);
 }
-int64_t chunks_of(int64_t numel, int64_t chunk) { return (numel + chunk - 1) / chunk; }
+int64_t chunks_of(int64_t numel, int64_t size) { return (numel + size - 1) / size; }
 
 int check_dtype(int dtype, const char* who, int i) {
     if (dtype != XSG_DTYPE_F32 && dtype != XSG_DTYPE_BF16 && dtype != XSG_DTYPE_F16)
@@ -768,28 +858,45 @@ AdamEntry entry_of(const xsg_adam_tensor& x) {
 }
 template <typename T> using EntryOf = decltype(entry_of(std::declval<const T&>()));
 
-// How a call is cut, and where things lie in its workspace: one double for a reduced norm, then (256 bytes on)
-// a partial sum per chunk, then a long list's table.
+int64_t touched(const xsg_grad_tensor& x) { return x.numel * type_size(x.dtype); }
+int64_t touched(const xsg_adam_tensor& x) { return x.numel * (type_size(x.param_dtype) + type_size(x.grad_dtype) + 8); }
+bool all_f32(const xsg_grad_tensor& x) { return x.dtype == XSG_DTYPE_F32; }
+bool all_f32(const xsg_adam_tensor& x) { return x.param_dtype == XSG_DTYPE_F32 && x.grad_dtype == XSG_DTYPE_F32; }
+
+// calls f with the flag as a constant
+template <typename F> void with_flag(bool flag, F&& f) {
+    if (flag) f(std::true_type{});
+    else f(std::false_type{});
+}
+
+// How a call is cut, and where things lie in its workspace: the step's terms, then (256 bytes on) the partial
+// sums, of `each` chunks in a row, then a long list's table.
 struct Plan {
-    int64_t elements = 0, chunk = 0, chunks = 0;
-    bool table = false;
+    int64_t elements = 0, bytes_touched = 0, chunk = 0, masked_chunk = 0, chunks = 0, each = 1, parts = 0;
+    bool table = false, f32 = true, stream = false;
     size_t first_at = 0, entry_at = 0, bytes = 0;
 };
 
 size_t aligned(size_t x) { return (x + 255) / 256 * 256; }
 
-template <typename T> int make_plan(const T* ts, int n, const char* who, bool norm, Plan* p) {
+template <typename T> int make_plan(const T* ts, int n, const char* who, bool norm, bool writes, Plan* p) {
     if (n < 0 || (n > 0 && !ts)) return xsg_fail(XSG_ERR_INVALID, "%s: null or negative list of tensors", who);
     for (int i = 0; i < n; ++i) {
         if (ts[i].numel < 0) return xsg_fail(XSG_ERR_INVALID, "%s: tensor %d has a negative size", who, i);
         if (ts[i].numel > kMaxElements - p->elements) return xsg_fail(XSG_ERR_INVALID, "%s: too many elements", who);
         p->elements += ts[i].numel;
+        p->bytes_touched += touched(ts[i]);
+        p->f32 = p->f32 && all_f32(ts[i]);
     }
-    p->chunk = chunk_for(p->elements);
-    for (int i = 0; i < n; ++i) p->chunks += chunks_of(ts[i].numel, p->chunk);
-    if (p->chunks > kMaxChunk) return xsg_fail(XSG_ERR_INVALID, "%s: too many tensors", who);
+    p->stream = p->bytes_touched > kCacheBytes;
+    p->chunk = chunk_for(p->elements, writes && p->stream);
+    p->masked_chunk = writes && p->stream ? kMaskedChunks * p->chunk : p->chunk;
+    for (int i = 0; i < n; ++i) p->chunks += chunks_of(ts[i].numel, ts[i].mask ? p->masked_chunk : p->chunk);
+    if (p->chunks > kMaxChunks) return xsg_fail(XSG_ERR_INVALID, "%s: too many tensors", who);
+    if (writes) p->each = std::max<int64_t>((p->chunks + kTargetChunks - 1) / kTargetChunks, 1);
+    p->parts = (p->chunks + p->each - 1) / p->each;
     p->table = n > kInline<EntryOf<T>>;
-    p->bytes = norm ? 256 + aligned((size_t)p->chunks * sizeof(double)) : 0;
+    p->bytes = norm ? 256 + aligned((size_t)p->parts * sizeof(double)) : 0;
     if (p->table) {
         p->first_at = p->bytes;
         p->entry_at = p->first_at + aligned(((size_t)n + 1) * sizeof(int32_t));
@@ -803,11 +910,12 @@ template <typename T> void fill_inline(const T* ts, int n, const Plan& p, Inline
     for (int i = 0; i < n; ++i) {
         list->entry[i] = entry_of(ts[i]);
         list->first[i] = at;
-        at += (int32_t)chunks_of(ts[i].numel, p.chunk);
+        at += (int32_t)chunks_of(ts[i].numel, ts[i].mask ? p.masked_chunk : p.chunk);
     }
     list->first[n] = at;
     list->n = n;
     list->chunk = (int32_t)p.chunk;
+    list->masked_chunk = (int32_t)p.masked_chunk;
     list->chunks = at;
 }
 
@@ -824,7 +932,7 @@ int send_table(const T* ts, int n, const Plan& p, void* ws, hipStream_t s, Table
         for (piece.n = 0; piece.n < kInline<E> && i < n; ++i, ++piece.n) {
             piece.entry[piece.n] = entry_of(ts[i]);
             piece.first[piece.n] = at;
-            at += (int32_t)chunks_of(ts[i].numel, p.chunk);
+            at += (int32_t)chunks_of(ts[i].numel, ts[i].mask ? p.masked_chunk : p.chunk);
         }
         const bool last = i == n && piece.n < kInline<E>;
         if (last) piece.first[piece.n] = at;
@@ -832,7 +940,7 @@ int send_table(const T* ts, int n, const Plan& p, void* ws, hipStream_t s, Table
         XSG_TRY_LAUNCH("table");
         if (last) break;
     }
-    *list = TableList<E>{entry, first, n, (int32_t)p.chunk, at};
+    *list = TableList<E>{entry, first, n, (int32_t)p.chunk, (int32_t)p.masked_chunk, at};
     return XSG_OK;
 }
 
@@ -869,20 +977,31 @@ template <typename F> void with_norm(int norm, F&& f) {
 
 double* partials(void* ws) { return (double*)((char*)ws + 256); }
 
-template <typename L>
-int launch_partials(const L& list, int norm, void* ws, int64_t* step, hipStream_t s) {
+template <bool STREAM, typename L>
+int launch_partials(const L& list, int norm, const Plan& p, void* ws, int64_t* step, hipStream_t s) {
+    const int blocks = std::max<int>((int)p.parts, 1);
     with_norm(norm, [&](auto kind) {
-        norm_partial_kernel<kind.value><<<std::max(list.chunks, 1), kBlock, 0, s>>>(list, partials(ws), step);
+        norm_partial_kernel<kind.value, STREAM><<<blocks, kBlock, 0, s>>>(list, (int)p.each, partials(ws), step);
     });
     return xsg_launch_status("grad_norm");
 }
 
-// the partial sums as the next launch's workgroups join them
-int join_parts(int chunks, int norm, void* ws, hipStream_t s, NormParts* parts) {
-    *parts = NormParts{partials(ws), chunks, norm};
-    if (chunks <= kJoinMax) return XSG_OK;
-    norm_reduce_kernel<<<1, kBlock, 0, s>>>(partials(ws), chunks, norm, (double*)ws);
-    *parts = NormParts{(const double*)ws, 1, norm};
+// the norm (where the rule has one) and the step's terms, for the launch behind
+template <typename L>
+int make_terms(const L& list, const StepRule& rule, const Plan& p, void* ws, int64_t* step, float* total, hipStream_t s,
+               StepSource* source) {
+    *source = StepSource{rule, nullptr, 0, step, total, nullptr};
+    if (rule.norm < 0) {
+        adam_count_kernel<<<1, 1, 0, s>>>(step);
+        return xsg_launch_status("adam_step");
+    }
+    const int rc = launch_partials<false>(list, rule.norm, p, ws, step, s);
+    if (rc != XSG_OK) return rc;
+    source->partial = partials(ws);
+    source->n = (int)p.parts;
+    if (p.each == 1) return XSG_OK;
+    step_terms_kernel<<<1, kBlock, 0, s>>>(rule, partials(ws), (int)p.parts, step, total, (StepTerms*)ws);
+    source->ready = (const StepTerms*)ws;
     return xsg_launch_status("grad_norm");
 }
 
@@ -890,13 +1009,13 @@ int join_parts(int chunks, int norm, void* ws, hipStream_t s, NormParts* parts) 
 
 extern "C" size_t xsg_grad_norm_workspace_bytes(const xsg_grad_tensor* ts, int n) {
     Plan p;
-    return make_plan(ts, n, "grad_norm", true, &p) == XSG_OK ? p.bytes : 0;
+    return make_plan(ts, n, "grad_norm", true, false, &p) == XSG_OK ? p.bytes : 0;
 }
 
 extern "C" int xsg_grad_norm(const xsg_grad_tensor* ts, int n, int norm, float* total, float* each, void* workspace,
                              xsg_stream_t stream) {
     Plan p;
-    int rc = make_plan(ts, n, "grad_norm", true, &p);
+    int rc = make_plan(ts, n, "grad_norm", true, false, &p);
     if (rc == XSG_OK) rc = check_list(ts, n, norm, "grad_norm");
     if (rc != XSG_OK) return rc;
     if (!total || !workspace) return xsg_fail(XSG_ERR_INVALID, "grad_norm: null output or workspace");
@@ -904,7 +1023,8 @@ extern "C" int xsg_grad_norm(const xsg_grad_tensor* ts, int n, int norm, float* 
     if (rc != XSG_OK) return rc;
     const hipStream_t s = (hipStream_t)stream;
     return with_list(ts, n, p, workspace, s, [&](const auto& list) {
-        const int status = launch_partials(list, norm, workspace, nullptr, s);
+        const int status = p.stream ? launch_partials<true>(list, norm, p, workspace, nullptr, s)
+                                    : launch_partials<false>(list, norm, p, workspace, nullptr, s);
         if (status != XSG_OK) return status;
         const double* const partial = partials(workspace);
         if (each) norm_each_kernel<<<n + 1, kBlock, 0, s>>>(list, partial, norm, total, each);
@@ -913,10 +1033,15 @@ extern "C" int xsg_grad_norm(const xsg_grad_tensor* ts, int n, int norm, float* 
     });
 }
 
+extern "C" size_t xsg_clip_grads_workspace_bytes(const xsg_grad_tensor* ts, int n) {
+    Plan p;
+    return make_plan(ts, n, "clip_grads", true, true, &p) == XSG_OK ? p.bytes : 0;
+}
+
 extern "C" int xsg_clip_grads(const xsg_grad_tensor* ts, int n, int norm, double max_norm, double eps, float* total,
                               void* workspace, xsg_stream_t stream) {
     Plan p;
-    int rc = make_plan(ts, n, "clip_grads", true, &p);
+    int rc = make_plan(ts, n, "clip_grads", true, true, &p);
     if (rc == XSG_OK) rc = check_list(ts, n, norm, "clip_grads");
     if (rc != XSG_OK) return rc;
     if (!(max_norm >= 0.0) || !(eps >= 0.0))
@@ -926,19 +1051,20 @@ extern "C" int xsg_clip_grads(const xsg_grad_tensor* ts, int n, int norm, double
     if (rc != XSG_OK) return rc;
     const hipStream_t s = (hipStream_t)stream;
     return with_list(ts, n, p, workspace, s, [&](const auto& list) {
-        int status = launch_partials(list, norm, workspace, nullptr, s);
+        const StepRule rule{max_norm, eps, 0.0, 0.0, norm, 1, 0};
+        StepSource source;
+        const int status = make_terms(list, rule, p, workspace, nullptr, total, s, &source);
         if (status != XSG_OK) return status;
-        NormParts parts;
-        status = join_parts(list.chunks, norm, workspace, s, &parts);
-        if (status != XSG_OK) return status;
-        clip_scale_kernel<<<std::max(list.chunks, 1), kBlock, 0, s>>>(list, parts, max_norm, eps, total);
+        with_flag(p.stream, [&](auto stream) {
+            clip_scale_kernel<stream.value><<<std::max(list.chunks, 1), kBlock, 0, s>>>(list, source);
+        });
         return xsg_launch_status("clip_grads");
     });
 }
 
 extern "C" size_t xsg_adam_step_workspace_bytes(const xsg_adam_tensor* ts, int n, const xsg_adam_options* o) {
     Plan p;
-    return o && make_plan(ts, n, "adam_step", o->clip || o->skip_nonfinite, &p) == XSG_OK ? p.bytes : 0;
+    return o && make_plan(ts, n, "adam_step", o->clip || o->skip_nonfinite, true, &p) == XSG_OK ? p.bytes : 0;
 }
 
 extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_options* o, int64_t* step, float* total,
@@ -946,7 +1072,7 @@ extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_op
     if (!o || !step) return xsg_fail(XSG_ERR_INVALID, "adam_step: null options or step counter");
     const bool needs_norm = o->clip || o->skip_nonfinite;
     Plan p;
-    int rc = make_plan(ts, n, "adam_step", needs_norm, &p);
+    int rc = make_plan(ts, n, "adam_step", needs_norm, true, &p);
     if (rc != XSG_OK) return rc;
     if (!(o->beta1 >= 0.0 && o->beta1 < 1.0 && o->beta2 >= 0.0 && o->beta2 < 1.0))
         return xsg_fail(XSG_ERR_INVALID, "adam_step: betas %g and %g must lie in [0, 1)", o->beta1, o->beta2);
@@ -967,29 +1093,20 @@ extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_op
         rc = xsg_check_workspace(workspace, "adam_step");
         if (rc != XSG_OK) return rc;
     }
-    AdamScalars a;
-    a.log_beta1 = log(o->beta1);   // beta 0: -inf, and 1 - beta^k is 1
-    a.log_beta2 = log(o->beta2);
-    a.beta2 = (float)o->beta2;
-    a.one_minus_beta1 = (float)(1.0 - o->beta1);
-    a.one_minus_beta2 = (float)(1.0 - o->beta2);
-    a.eps = (float)o->eps;
-    a.clip = o->clip;
-    a.skip_nonfinite = o->skip_nonfinite;
-    a.max_norm = o->max_norm;
+    const AdamScalars a{(float)o->beta2, (float)(1.0 - o->beta1), (float)(1.0 - o->beta2), (float)o->eps};
+    // beta 0: the logarithm is -inf, and 1 - beta^t is 1
+    const StepRule rule{o->max_norm, kAdamClipEps, log(o->beta1), log(o->beta2), needs_norm ? o->norm : -1, o->clip,
+                        o->skip_nonfinite};
     const hipStream_t s = (hipStream_t)stream;
     return with_list(ts, n, p, workspace, s, [&](const auto& list) {
-        NormParts parts{nullptr, -1, o->norm};
-        int status;
-        if (needs_norm) {
-            status = launch_partials(list, o->norm, workspace, step, s);
-            if (status == XSG_OK) status = join_parts(list.chunks, o->norm, workspace, s, &parts);
-        } else {
-            adam_count_kernel<<<1, 1, 0, s>>>(step);
-            status = xsg_launch_status("adam_step");
-        }
+        StepSource source;
+        const int status = make_terms(list, rule, p, workspace, step, total, s, &source);
         if (status != XSG_OK) return status;
-        adam_kernel<<<std::max(list.chunks, 1), kBlock, 0, s>>>(list, a, parts, step, total);
+        with_flag(p.f32, [&](auto f32) {
+            with_flag(p.stream, [&](auto stream) {
+                adam_kernel<f32.value, stream.value><<<std::max(list.chunks, 1), kBlock, 0, s>>>(list, a, source);
+            });
+        });
         return xsg_launch_status("adam_step");
     });
 }

@@ -725,7 +725,7 @@ Tensor clip_grads_(const std::vector<Tensor>& tensors, double max_norm, double n
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(tensors[0].device());
     Tensor total = at::empty({}, tensors[0].options().dtype(at::kFloat));
     const int n = (int)a.list.size();
-    Tensor ws = workspace(tensors[0], xsg_grad_norm_workspace_bytes(a.list.data(), n));
+    Tensor ws = workspace(tensors[0], xsg_clip_grads_workspace_bytes(a.list.data(), n));
     check_rc(xsg_clip_grads(a.list.data(), n, kind, max_norm, eps, total.data_ptr<float>(), ws.data_ptr(),
                             stream_of(tensors[0])));
     for (size_t i = 0; i < tensors.size(); ++i) {
@@ -804,12 +804,11 @@ OptT adam_step_(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
     const bool normed = o.clip || o.skip_nonfinite;
     Tensor total, ws;
-    if (normed) {
-        total = at::empty({}, params[0].options().dtype(at::kFloat));
-        ws = workspace(params[0], xsg_adam_step_workspace_bytes(list.data(), (int)n, &o));
-    }
+    if (normed) total = at::empty({}, params[0].options().dtype(at::kFloat));
+    const size_t bytes = xsg_adam_step_workspace_bytes(list.data(), (int)n, &o);
+    if (bytes > 0) ws = workspace(params[0], bytes);
     check_rc(xsg_adam_step(list.data(), (int)n, &o, step.data_ptr<int64_t>(),
-                           normed ? total.data_ptr<float>() : nullptr, normed ? ws.data_ptr() : nullptr,
+                           normed ? total.data_ptr<float>() : nullptr, bytes > 0 ? ws.data_ptr() : nullptr,
                            stream_of(params[0])));
     for (size_t i = 0; i < n; ++i) {
         mark_written(params[i]);
