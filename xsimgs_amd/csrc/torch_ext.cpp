@@ -601,7 +601,8 @@ std::tuple<Tensor, Tensor> radix_sort_pairs(const Tensor& keys, const Tensor& va
 // ------------------------------------------------------------------ training step
 // Extensions: the global gradient norm, clipping by it and the Adam update (optim.hip). Lists of tensors of
 // float32, bfloat16 or float16 on one GPU; masks: empty, or one optional packed mask per tensor over the rows
-// of its first dimension.
+// of its first dimension. The lists are read from Python's own: they can hold thousands of tensors, and a
+// tensor's conversion costs more than its share of the kernels.
 int norm_kind(double norm_type) {
     if (norm_type == 2.0) return XSG_NORM_L2;
     if (norm_type == 1.0) return XSG_NORM_L1;
@@ -619,17 +620,23 @@ int dtype_of(const Tensor& t, const char* what, size_t i) {
     }
 }
 
+const Tensor& tensor_at(const py::list& list, size_t i, const char* what) {
+    PyObject* const o = PyList_GET_ITEM(list.ptr(), (Py_ssize_t)i);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), what, " ", i, " must be a tensor");
+    return THPVariable_Unpack(o);
+}
+
 void check_listed(const Tensor& t, const at::Device& device, const char* what, size_t i) {
-    TORCH_CHECK(t.defined() && t.layout() == at::kStrided, what, " ", i, " must be a strided tensor");
+    TORCH_CHECK(t.layout() == at::kStrided, what, " ", i, " must be a strided tensor");
     TORCH_CHECK(t.is_cuda(), "xsimgs_amd ops take GPU tensors (got ", what, " ", i, " on ", t.device(), ")");
     TORCH_CHECK(t.device() == device, "All tensors must be on the same device");
 }
 
 // the mask of tensor i, or null
-const uint32_t* mask_of(const std::vector<OptT>& masks, size_t i, const Tensor& t, int64_t* rows) {
+const uint32_t* mask_of(const py::list& masks, size_t i, const Tensor& t, int64_t* rows) {
     *rows = 0;
-    if (masks.empty() || !masks[i].has_value()) return nullptr;
-    const Tensor& m = *masks[i];
+    if (masks.size() == 0 || PyList_GET_ITEM(masks.ptr(), (Py_ssize_t)i) == Py_None) return nullptr;
+    const Tensor& m = tensor_at(masks, i, "mask");
     TORCH_CHECK(m.scalar_type() == at::kUInt32 || m.scalar_type() == at::kInt, "Packed mask must be UInt32 tensor");
     TORCH_CHECK(m.device() == t.device(), "All tensors must be on the same device");
     TORCH_CHECK(m.is_contiguous(), "All tensors must be contiguous");
@@ -639,116 +646,169 @@ const uint32_t* mask_of(const std::vector<OptT>& masks, size_t i, const Tensor& 
     return (const uint32_t*)m.data_ptr();
 }
 
-// t itself where its elements lie densely (in row order, under a mask), else a dense copy
-Tensor dense_of(const Tensor& t, bool masked) {
-    return (masked ? t.is_contiguous() : t.is_non_overlapping_and_dense()) ? t : t.contiguous();
+// Whether t's elements lie densely (in row order, under a mask); else the kernels take a dense copy.
+bool is_dense(const Tensor& t, bool masked) {
+    return t.is_contiguous() || (!masked && t.is_non_overlapping_and_dense());
 }
 
 struct GradArgs {
-    std::vector<Tensor> held;   // what the pointers point into
     std::vector<xsg_grad_tensor> list;
+    std::vector<std::pair<size_t, Tensor>> copies;   // of the tensors that are not dense
 };
 
-GradArgs grad_args(const std::vector<Tensor>& tensors, const std::vector<OptT>& masks) {
-    TORCH_CHECK(!tensors.empty(), "an empty list of tensors has no device");
-    TORCH_CHECK(masks.empty() || masks.size() == tensors.size(), "masks must hold one entry per tensor");
+GradArgs grad_args(const py::list& tensors, const py::list& masks) {
+    const size_t n = tensors.size();
+    TORCH_CHECK(n > 0, "an empty list of tensors has no device");
+    TORCH_CHECK(masks.size() == 0 || masks.size() == n, "masks must hold one entry per tensor");
     GradArgs a;
-    a.held.reserve(tensors.size());
-    a.list.resize(tensors.size());
-    for (size_t i = 0; i < tensors.size(); ++i) {
-        const Tensor& t = tensors[i];
-        check_listed(t, tensors[0].device(), "tensor", i);
+    a.list.resize(n);
+    const at::Device device = tensor_at(tensors, 0, "tensor").device();
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor& t = tensor_at(tensors, i, "tensor");
+        check_listed(t, device, "tensor", i);
         xsg_grad_tensor& x = a.list[i];
         x.dtype = dtype_of(t, "tensor", i);
         x.mask = mask_of(masks, i, t, &x.rows);
-        a.held.push_back(dense_of(t, x.mask != nullptr));
-        x.data = a.held[i].data_ptr();
         x.numel = t.numel();
+        if (!is_dense(t, x.mask != nullptr)) a.copies.emplace_back(i, t.contiguous());
+        x.data = (a.copies.empty() || a.copies.back().first != i ? t : a.copies.back().second).data_ptr();
     }
     return a;
 }
 
-// No two written arrays of a call may overlap, nor a written and a read one: the kernels would race.
-struct Span {
-    uintptr_t lo, hi;
-    bool written;
-};
+// No two written arrays of a call may overlap, nor a written and a read one: the kernels would race. The spans
+// are put in order of their addresses by counting digits of 11 bits (a comparison sort costs more than the
+// launches where there are thousands).
+struct Spans {
+    struct Span {
+        uint64_t lo;
+        uint64_t size_written;   // 2 * bytes + whether it is written
+    };
+    std::vector<Span> spans;
 
-void add_span(std::vector<Span>& spans, const Tensor& t, bool written) {
-    const auto lo = reinterpret_cast<uintptr_t>(t.data_ptr());
-    if (t.numel() > 0) spans.push_back({lo, lo + t.numel() * t.element_size(), written});
-}
-
-void check_no_overlap(std::vector<Span>& spans) {
-    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
-    uintptr_t any = 0, written = 0;   // ends of what came before
-    for (const Span& s : spans) {
-        TORCH_CHECK(s.lo >= (s.written ? any : written),
-                    "the tensors overlap in memory: each one that is written must be given once");
-        any = std::max(any, s.hi);
-        if (s.written) written = std::max(written, s.hi);
+    void add(const void* data, size_t bytes, bool written) {
+        if (bytes > 0) spans.push_back({reinterpret_cast<uintptr_t>(data), 2 * (uint64_t)bytes + written});
     }
-}
+    void sort() {
+        const auto less = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+        if (std::is_sorted(spans.begin(), spans.end(), less)) return;
+        if (spans.size() < 128) return std::sort(spans.begin(), spans.end(), less);
+        uint64_t any = 0;
+        for (const Span& s : spans) any |= s.lo ^ spans[0].lo;   // bits in which the addresses differ
+        std::vector<Span> other(spans.size());
+        for (int shift = 0; shift < 64 && (any >> shift) != 0; shift += 11) {
+            if (((any >> shift) & 2047) == 0) continue;
+            uint32_t at[2048] = {};
+            for (const Span& s : spans) ++at[(s.lo >> shift) & 2047];
+            uint32_t sum = 0;
+            for (uint32_t& k : at) {
+                const uint32_t count = k;
+                k = sum;
+                sum += count;
+            }
+            for (const Span& s : spans) other[at[(s.lo >> shift) & 2047]++] = s;
+            spans.swap(other);
+        }
+    }
+    void check() {
+        sort();
+        uint64_t any = 0, written = 0;   // ends of what came before
+        for (const Span& s : spans) {
+            TORCH_CHECK(s.lo >= (s.size_written & 1 ? any : written),
+                        "the tensors overlap in memory: each one that is written must be given once");
+            const uint64_t hi = s.lo + (s.size_written >> 1);
+            any = std::max(any, hi);
+            if (s.size_written & 1) written = std::max(written, hi);
+        }
+    }
+};
 
 void mark_written(const Tensor& t) {   // autograd notices what it saved before
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-std::tuple<Tensor, OptT> grad_norm(const std::vector<Tensor>& tensors, double norm_type,
-                                   const std::vector<OptT>& masks, bool per_tensor) {
+std::tuple<Tensor, OptT> grad_norm(const py::list& tensors, double norm_type, const py::list& masks,
+                                   bool per_tensor) {
     const int kind = norm_kind(norm_type);
     at::NoGradGuard no_grad;
     GradArgs a = grad_args(tensors, masks);
-    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(tensors[0].device());
-    const auto opts = tensors[0].options().dtype(at::kFloat);
+    const Tensor& like = tensor_at(tensors, 0, "tensor");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(like.device());
+    const auto opts = like.options().dtype(at::kFloat);
     const int n = (int)a.list.size();
     Tensor total = at::empty({}, opts), each;
     if (per_tensor) each = at::empty({n}, opts);
-    Tensor ws = workspace(tensors[0], xsg_grad_norm_workspace_bytes(a.list.data(), n));
+    Tensor ws = workspace(like, xsg_grad_norm_workspace_bytes(a.list.data(), n));
     check_rc(xsg_grad_norm(a.list.data(), n, kind, total.data_ptr<float>(),
-                           per_tensor ? each.data_ptr<float>() : nullptr, ws.data_ptr(), stream_of(tensors[0])));
+                           per_tensor ? each.data_ptr<float>() : nullptr, ws.data_ptr(), stream_of(like)));
     return {total, per_tensor ? OptT(each) : OptT()};
 }
 
-Tensor clip_grads_(const std::vector<Tensor>& tensors, double max_norm, double norm_type, double eps,
-                   const std::vector<OptT>& masks) {
+Tensor clip_grads_(const py::list& tensors, double max_norm, double norm_type, double eps, const py::list& masks) {
     const int kind = norm_kind(norm_type);
     at::NoGradGuard no_grad;
     GradArgs a = grad_args(tensors, masks);
-    std::vector<Span> spans;
-    for (size_t i = 0; i < tensors.size(); ++i) {
-        TORCH_CHECK(at::has_internal_overlap(tensors[i]) != at::MemOverlap::Yes, "tensor ", i,
-                    " has elements that share memory and cannot be scaled in place");
-        if (a.held[i].is_same(tensors[i])) add_span(spans, tensors[i], true);
+    const size_t n = a.list.size();
+    Spans spans;
+    size_t copied = 0;
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor& t = tensor_at(tensors, i, "tensor");
+        if (copied < a.copies.size() && a.copies[copied].first == i) {
+            ++copied;
+            TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, "tensor ", i,
+                        " has elements that share memory and cannot be scaled in place");
+        } else {
+            spans.add(a.list[i].data, a.list[i].numel * t.element_size(), true);
+        }
     }
-    check_no_overlap(spans);
-    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(tensors[0].device());
-    Tensor total = at::empty({}, tensors[0].options().dtype(at::kFloat));
-    const int n = (int)a.list.size();
-    Tensor ws = workspace(tensors[0], xsg_clip_grads_workspace_bytes(a.list.data(), n));
-    check_rc(xsg_clip_grads(a.list.data(), n, kind, max_norm, eps, total.data_ptr<float>(), ws.data_ptr(),
-                            stream_of(tensors[0])));
-    for (size_t i = 0; i < tensors.size(); ++i) {
-        if (a.held[i].is_same(tensors[i])) mark_written(tensors[i]);
-        else tensors[i].copy_(a.held[i]);
-    }
+    spans.check();
+    const Tensor& like = tensor_at(tensors, 0, "tensor");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(like.device());
+    Tensor total = at::empty({}, like.options().dtype(at::kFloat));
+    Tensor ws = workspace(like, xsg_clip_grads_workspace_bytes(a.list.data(), (int)n));
+    check_rc(xsg_clip_grads(a.list.data(), (int)n, kind, max_norm, eps, total.data_ptr<float>(), ws.data_ptr(),
+                            stream_of(like)));
+    for (size_t i = 0; i < n; ++i) mark_written(tensor_at(tensors, i, "tensor"));
+    for (const auto& [i, copy] : a.copies) tensor_at(tensors, i, "tensor").copy_(copy);
     return total;
 }
 
 bool same_layout(const Tensor& a, const Tensor& b) {
-    return a.sizes() == b.sizes() && (a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()));
+    return a.sizes() == b.sizes() && ((a.is_contiguous() && b.is_contiguous()) || a.strides() == b.strides());
 }
 
-OptT adam_step_(const std::vector<Tensor>& params, const std::vector<Tensor>& grads,
-                const std::vector<Tensor>& exp_avgs, const std::vector<Tensor>& exp_avg_sqs, const Tensor& step,
-                const std::vector<double>& lr, const std::vector<double>& weight_decay, double beta1, double beta2,
+// a number, or one per tensor
+struct Rates {
+    double same = 0.0;
+    std::vector<double> each;
+    Rates(const py::object& value, size_t n, const char* name) {
+        if (PyList_Check(value.ptr())) {
+            TORCH_CHECK_VALUE((size_t)PyList_GET_SIZE(value.ptr()) == n, name, " must be a number or hold one per tensor: ",
+                              PyList_GET_SIZE(value.ptr()), " for ", n);
+            each.resize(n);
+            for (size_t i = 0; i < n; ++i) each[i] = number(PyList_GET_ITEM(value.ptr(), (Py_ssize_t)i));
+        } else {
+            same = number(value.ptr());
+        }
+    }
+    static double number(PyObject* o) {
+        const double v = PyFloat_AsDouble(o);
+        if (v == -1.0 && PyErr_Occurred()) throw py::error_already_set();
+        return v;
+    }
+    double operator[](size_t i) const { return each.empty() ? same : each[i]; }
+};
+
+OptT adam_step_(const py::list& params, const py::list& grads, const py::list& exp_avgs, const py::list& exp_avg_sqs,
+                const Tensor& step, const py::object& lr, const py::object& weight_decay, double beta1, double beta2,
                 double eps, const std::optional<double>& max_norm, double norm_type, bool skip_nonfinite,
-                const std::vector<OptT>& masks) {
+                const py::list& masks) {
     const size_t n = params.size();
     TORCH_CHECK(n > 0, "an empty list of tensors has no device");
-    TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && lr.size() == n &&
-                    weight_decay.size() == n && (masks.empty() || masks.size() == n),
-                "params, grads, exp_avgs, exp_avg_sqs, lr, weight_decay and masks must hold one entry per tensor");
+    TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n &&
+                    (masks.size() == 0 || masks.size() == n),
+                "params, grads, exp_avgs, exp_avg_sqs and masks must hold one entry per tensor");
+    const Rates lrs(lr, n, "lr"), decays(weight_decay, n, "weight_decay");
     xsg_adam_options o{};
     o.beta1 = beta1;
     o.beta2 = beta2;
@@ -757,18 +817,19 @@ OptT adam_step_(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     o.max_norm = max_norm.value_or(0.0);
     o.skip_nonfinite = skip_nonfinite;
     o.norm = norm_kind(norm_type);
-    const at::Device device = params[0].device();
+    const Tensor& like = tensor_at(params, 0, "parameter");
+    const at::Device device = like.device();
     TORCH_CHECK(step.scalar_type() == at::kLong && step.numel() == 1 && step.device() == device,
                 "step must be one int64 value on the parameters' device");
     at::NoGradGuard no_grad;
     std::vector<xsg_adam_tensor> list(n);
     std::vector<Tensor> held;
-    std::vector<Span> spans;
-    spans.reserve(4 * n + 1);
-    add_span(spans, step, true);
+    Spans spans;
+    spans.spans.reserve(4 * n + 1);
+    spans.add(step.data_ptr(), sizeof(int64_t), true);
     for (size_t i = 0; i < n; ++i) {
-        const Tensor &p = params[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
-        Tensor g = grads[i];
+        const Tensor &p = tensor_at(params, i, "parameter"), &m = tensor_at(exp_avgs, i, "exp_avg"),
+                     &v = tensor_at(exp_avg_sqs, i, "exp_avg_sq"), &g = tensor_at(grads, i, "gradient");
         check_listed(p, device, "parameter", i);
         check_listed(g, device, "gradient", i);
         check_listed(m, device, "exp_avg", i);
@@ -777,43 +838,43 @@ OptT adam_step_(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
         x.param_dtype = dtype_of(p, "parameter", i);
         x.grad_dtype = dtype_of(g, "gradient", i);
         x.mask = mask_of(masks, i, p, &x.rows);
-        TORCH_CHECK(x.mask ? p.is_contiguous() : p.is_non_overlapping_and_dense(), "parameter ", i, " must be ",
+        TORCH_CHECK(is_dense(p, x.mask != nullptr), "parameter ", i, " must be ",
                     x.mask ? "contiguous under a mask" : "dense in memory");
         TORCH_CHECK(m.scalar_type() == at::kFloat && v.scalar_type() == at::kFloat, "moments ", i,
                     " must be float32 tensors");
         TORCH_CHECK(same_layout(m, p) && same_layout(v, p), "moments ", i,
                     " must have their parameter's sizes and strides");
         TORCH_CHECK(g.sizes() == p.sizes(), "gradient ", i, " must have its parameter's sizes");
+        x.grad = g.data_ptr();
         if (!same_layout(g, p)) {
-            g = at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g);
-            held.push_back(g);
+            held.push_back(at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g));
+            x.grad = held.back().data_ptr();
         }
         x.param = p.data_ptr();
-        x.grad = g.data_ptr();
         x.exp_avg = m.data_ptr<float>();
         x.exp_avg_sq = v.data_ptr<float>();
         x.numel = p.numel();
-        x.lr = lr[i];
-        x.weight_decay = weight_decay[i];
-        add_span(spans, p, true);
-        add_span(spans, m, true);
-        add_span(spans, v, true);
-        add_span(spans, g, false);
+        x.lr = lrs[i];
+        x.weight_decay = decays[i];
+        spans.add(x.param, x.numel * p.element_size(), true);
+        spans.add(x.exp_avg, x.numel * sizeof(float), true);
+        spans.add(x.exp_avg_sq, x.numel * sizeof(float), true);
+        spans.add(x.grad, x.numel * g.element_size(), false);
     }
-    check_no_overlap(spans);
+    spans.check();
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
     const bool normed = o.clip || o.skip_nonfinite;
     Tensor total, ws;
-    if (normed) total = at::empty({}, params[0].options().dtype(at::kFloat));
+    if (normed) total = at::empty({}, like.options().dtype(at::kFloat));
     const size_t bytes = xsg_adam_step_workspace_bytes(list.data(), (int)n, &o);
-    if (bytes > 0) ws = workspace(params[0], bytes);
+    if (bytes > 0) ws = workspace(like, bytes);
     check_rc(xsg_adam_step(list.data(), (int)n, &o, step.data_ptr<int64_t>(),
                            normed ? total.data_ptr<float>() : nullptr, bytes > 0 ? ws.data_ptr() : nullptr,
-                           stream_of(params[0])));
+                           stream_of(like)));
     for (size_t i = 0; i < n; ++i) {
-        mark_written(params[i]);
-        mark_written(exp_avgs[i]);
-        mark_written(exp_avg_sqs[i]);
+        mark_written(tensor_at(params, i, "parameter"));
+        mark_written(tensor_at(exp_avgs, i, "exp_avg"));
+        mark_written(tensor_at(exp_avg_sqs, i, "exp_avg_sq"));
     }
     mark_written(step);
     return normed ? OptT(total) : OptT();

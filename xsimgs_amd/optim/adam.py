@@ -8,13 +8,8 @@ from .. import _C
 from .clip import listed_masks
 
 
-def _per_tensor(value, n: int, name: str) -> list:
-    if isinstance(value, (int, float)):
-        return [float(value)] * n
-    value = [float(v) for v in value]
-    if len(value) != n:
-        raise ValueError(f"{name} must be a number or hold one per tensor: {len(value)} for {n}")
-    return value
+def _rates(value):
+    return value if isinstance(value, (int, float)) else list(value)
 
 
 def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -32,11 +27,10 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     before clipping (with ``max_norm`` or ``skip_nonfinite``, else None). Parameters and gradients are float32,
     bfloat16 or float16; moments are float32 tensors of their parameter's sizes and strides."""
     params = list(params)
-    n = len(params)
-    return _C.adam_step_(params, list(grads), list(exp_avgs), list(exp_avg_sqs), step, _per_tensor(lr, n, "lr"),
-                         _per_tensor(weight_decay, n, "weight_decay"), float(betas[0]), float(betas[1]), float(eps),
+    return _C.adam_step_(params, list(grads), list(exp_avgs), list(exp_avg_sqs), step, _rates(lr),
+                         _rates(weight_decay), float(betas[0]), float(betas[1]), float(eps),
                          None if max_norm is None else float(max_norm), float(norm_type), bool(skip_nonfinite),
-                         listed_masks(masks, n))
+                         listed_masks(masks, len(params)))
 
 
 class Adam(torch.optim.Optimizer):
