@@ -96,7 +96,18 @@ template <int DT, bool STREAM> XSG_DEV void store4(void* p, uint32_t i, f32x4 x,
     for (int k = 0; k < 4; ++k)
         if ((keep >> k) & 1) store1<DT>(p, i + k, x[k]);
 }
+// What tensors of a long list have in common: most of it has few kinds.
+struct EntryKind {
+    uint32_t row, magic;
+    float lr, keep;
+    uint8_t shift, dtype, gdtype;
+    bool operator==(const EntryKind& o) const {
+        return row == o.row && lr == o.lr && keep == o.keep && dtype == o.dtype && gdtype == o.gdtype;
+    }
+};
+
 struct GradEntry {
+    static constexpr int kPointers = 1;
     void* data;
     int64_t numel;
     const uint32_t* mask;
@@ -104,9 +115,21 @@ struct GradEntry {
     uint8_t shift, dtype;
     XSG_HD const void* grad() const { return data; }
     XSG_HD int grad_dtype() const { return dtype; }
+    EntryKind kind() const { return EntryKind{row, magic, 0.0f, 0.0f, shift, dtype, 0}; }
+    void pointers(uint64_t* to) const { to[0] = (uint64_t)data; }
+    XSG_DEV void set(const uint64_t* ptr, int64_t numel_, const uint32_t* mask_, const EntryKind& k) {
+        data = (void*)ptr[0];
+        numel = numel_;
+        mask = mask_;
+        row = k.row;
+        magic = k.magic;
+        shift = k.shift;
+        dtype = k.dtype;
+    }
 };
 
 struct AdamEntry {
+    static constexpr int kPointers = 4;
     void* param;
     const void* gradient;
     float *avg, *sq;
@@ -117,6 +140,28 @@ struct AdamEntry {
     uint8_t shift, pdtype, gdtype;
     XSG_HD const void* grad() const { return gradient; }
     XSG_HD int grad_dtype() const { return gdtype; }
+    EntryKind kind() const { return EntryKind{row, magic, lr, keep, shift, pdtype, gdtype}; }
+    void pointers(uint64_t* to) const {
+        to[0] = (uint64_t)param;
+        to[1] = (uint64_t)gradient;
+        to[2] = (uint64_t)avg;
+        to[3] = (uint64_t)sq;
+    }
+    XSG_DEV void set(const uint64_t* ptr, int64_t numel_, const uint32_t* mask_, const EntryKind& k) {
+        param = (void*)ptr[0];
+        gradient = (const void*)ptr[1];
+        avg = (float*)ptr[2];
+        sq = (float*)ptr[3];
+        numel = numel_;
+        mask = mask_;
+        row = k.row;
+        magic = k.magic;
+        lr = k.lr;
+        keep = k.keep;
+        shift = k.shift;
+        pdtype = k.dtype;
+        gdtype = k.gdtype;
+    }
 };
 
 template <typename E> constexpr int kInline = kArgumentBytes / (sizeof(E) + 4);
@@ -147,23 +192,48 @@ template <typename E> struct TableList {
     }
     XSG_DEV int32_t first_of(int t) const { return get<int32_t>(first, 4 * t); }
 };
-// a piece of a table on its way to the workspace
+// A piece of a long list on its way to the workspace: pointers, first chunk, and a word of a tensor's size (48
+// bits), kind and mask (8 bits each; 0: no mask).
 template <typename E> struct TablePiece {
-    E entry[kInline<E>];
-    int32_t first[kInline<E>];
-    int32_t n;
+    static constexpr int kKinds = 16, kMasks = E::kPointers == 1 ? 48 : 24;
+    static constexpr int kSpace = kArgumentBytes - kKinds * sizeof(EntryKind) - kMasks * 8 - 24;
+    static constexpr int kMax = kSpace / (8 * E::kPointers + 12);
+    static_assert(kMax <= kBlock, "a thread to a tensor");
+    uint64_t pointer[kMax][E::kPointers];
+    uint64_t word[kMax];
+    const uint32_t* mask[kMasks];
+    EntryKind kind[kKinds];
+    int32_t first[kMax];
+    int32_t n, kinds, masks, end;   // end: the list's number of chunks with its last piece, else -1
 };
 static_assert(sizeof(InlineList<GradEntry>) <= 3920 && sizeof(InlineList<AdamEntry>) <= 3920 &&
+                  sizeof(TablePiece<GradEntry>) <= 3920 && sizeof(TablePiece<AdamEntry>) <= 3920 &&
                   sizeof(GradEntry) % 8 == 0 && sizeof(AdamEntry) % 8 == 0,
-              "lists share 4 KB with the other arguments and are copied by words");
+              "lists share 4 KB with the other arguments; entries are loaded by words");
 
 template <typename E>
 __global__ __launch_bounds__(kBlock) void table_kernel(TablePiece<E> piece, E* __restrict__ entry,
-                                                       int32_t* __restrict__ first, int last) {
-    const uint64_t* const from = reinterpret_cast<const uint64_t*>(piece.entry);
-    uint64_t* const to = reinterpret_cast<uint64_t*>(entry);
-    for (int i = threadIdx.x; i < piece.n * (int)(sizeof(E) / 8); i += kBlock) to[i] = from[i];
-    if (threadIdx.x < piece.n + last) first[threadIdx.x] = piece.first[threadIdx.x];
+                                                       int32_t* __restrict__ first) {
+    __shared__ EntryKind kind[TablePiece<E>::kKinds];
+    __shared__ const uint32_t* mask[TablePiece<E>::kMasks];
+    const int i = threadIdx.x;
+    if (i < piece.kinds) kind[i] = piece.kind[i];
+    if (i < piece.masks) mask[i] = piece.mask[i];
+    const int mine = min(i, piece.n - 1);
+    const uint64_t word = piece.word[mine];
+    uint64_t pointer[E::kPointers];
+#pragma unroll
+    for (int k = 0; k < E::kPointers; ++k) pointer[k] = piece.pointer[mine][k];
+    const int32_t chunk = piece.first[mine];
+    __syncthreads();
+    if (i < piece.n) {
+        const int m = (int)(word >> 56);
+        E e;
+        e.set(pointer, (int64_t)(word & (((uint64_t)1 << 48) - 1)), m ? mask[m - 1] : nullptr, kind[(word >> 48) & 255]);
+        entry[i] = e;
+        first[i] = chunk;
+    }
+    if (piece.end >= 0 && i == 0) first[piece.n] = piece.end;
 }
 
 XSG_HD uint32_t type_size(int dtype) { return dtype == XSG_DTYPE_F32 ? 4 : 2; }
@@ -311,8 +381,10 @@ XSG_DEV void for_chunk(const ChunkSpan& span, const ChunkMask& mask, One&& one, 
         if (!MASK || mask.one(k)) one(k);
 }
 
-constexpr int kUnroll = 4;       // groups in flight per thread: of one array
-constexpr int kAdamUnroll = 2;   // and of four
+constexpr int kUnroll = 4;   // groups in flight per thread and array
+// An update of four arrays has as many where it streams (4 M Gaussians 1251 us, with two 1267), two where the
+// caches answer and more wavefronts do better.
+template <bool STREAM> constexpr int kAdamUnroll = STREAM ? 4 : 2;
 
 // Under a mask of short rows each wavefront lists the kept rows of its share of the chunk (a mask word a lane, so
 // up to 2048 rows for one load's latency) and then walks their elements alone, VEC at a time, so that lanes are
@@ -625,8 +697,8 @@ XSG_DEV void rows_scale(void* p, float c, uint32_t count, bool whole, const Chun
 template <bool STREAM, typename L>
 __global__ __launch_bounds__(kBlock) void clip_scale_kernel(L list, StepSource source) {
     const float c = source.terms().c;
-    const int b = list.chunks - 1 - (int)blockIdx.x;
-    if (c == 1.0f || b < 0) return;   // the values stay as they are
+    const int b = blockIdx.x;
+    if (c == 1.0f || b >= list.chunks) return;   // the values stay as they are
     const int t = find_tensor(list, b);
     const auto& e = list.at(t);
     const Chunk chunk(list, e, b, t);
@@ -668,6 +740,13 @@ struct AdamArrays {
     const void* g;
     float *m, *v;
 };
+
+XSG_DEV AdamTerms adam_terms(const StepTerms& now, const AdamScalars& s, float lr, float keep) {
+    return AdamTerms{s.beta2, s.one_minus_beta1, s.one_minus_beta2, s.eps, now.c, lr * now.over1, now.root, keep};
+}
+XSG_DEV AdamArrays adam_arrays(const AdamEntry& e, int64_t base) {
+    return AdamArrays{at(e.param, base, e.pdtype), at(e.gradient, base, e.gdtype), e.avg + base, e.sq + base};
+}
 
 // One element, or four, of the four arrays.
 template <int PT, int GT> struct Adam1 {
@@ -712,18 +791,18 @@ template <int PT, int GT, bool STREAM> struct Adam4 {
 
 template <int PT, int GT, bool MASK, bool STREAM>
 XSG_DEV void chunk_adam(const AdamArrays& a, const AdamTerms& s, const ChunkSpan& span, const ChunkMask& mask) {
-    for_chunk<MASK, kAdamUnroll>(span, mask, [&](uint32_t i) {
+    for_chunk<MASK, kAdamUnroll<STREAM>>(span, mask, [&](uint32_t i) {
         Adam1<PT, GT> x;
         x.load(a, i);
         x.update(s);
         x.store(a, i);
     }, [&](const uint32_t* i, const uint32_t* keep, auto all) {
-        Adam4<PT, GT, STREAM> x[kAdamUnroll];
+        Adam4<PT, GT, STREAM> x[kAdamUnroll<STREAM>];
 #pragma unroll
-        for (int u = 0; u < kAdamUnroll; ++u)
+        for (int u = 0; u < kAdamUnroll<STREAM>; ++u)
             if (all.value || keep[u]) x[u].load(a, i[u]);
 #pragma unroll
-        for (int u = 0; u < kAdamUnroll; ++u) {
+        for (int u = 0; u < kAdamUnroll<STREAM>; ++u) {
             if (!(all.value || keep[u])) continue;
             x[u].update(s);
             x[u].store(a, i[u], all.value ? 15u : keep[u]);
@@ -734,26 +813,26 @@ XSG_DEV void chunk_adam(const AdamArrays& a, const AdamTerms& s, const ChunkSpan
 template <int PT, int GT, bool STREAM>
 XSG_DEV void rows_adam(const AdamArrays& a, const AdamTerms& s, uint32_t count, bool whole, const ChunkMask& mask) {
     if (whole) {
-        for_kept_rows<4, kAdamUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
-            Adam4<PT, GT, STREAM> x[kAdamUnroll];
+        for_kept_rows<4, kAdamUnroll<STREAM>>(mask, count, [&](const uint32_t* i, const bool* on) {
+            Adam4<PT, GT, STREAM> x[kAdamUnroll<STREAM>];
 #pragma unroll
-            for (int u = 0; u < kAdamUnroll; ++u)
+            for (int u = 0; u < kAdamUnroll<STREAM>; ++u)
                 if (on[u]) x[u].load(a, i[u]);
 #pragma unroll
-            for (int u = 0; u < kAdamUnroll; ++u) {
+            for (int u = 0; u < kAdamUnroll<STREAM>; ++u) {
                 if (!on[u]) continue;
                 x[u].update(s);
                 x[u].store(a, i[u], 15u);
             }
         });
     } else {
-        for_kept_rows<1, kUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
-            Adam1<PT, GT> x[kUnroll];
+        for_kept_rows<1, kAdamUnroll<STREAM>>(mask, count, [&](const uint32_t* i, const bool* on) {
+            Adam1<PT, GT> x[kAdamUnroll<STREAM>];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
+            for (int u = 0; u < kAdamUnroll<STREAM>; ++u)
                 if (on[u]) x[u].load(a, i[u]);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
+            for (int u = 0; u < kAdamUnroll<STREAM>; ++u) {
                 if (!on[u]) continue;
                 x[u].update(s);
                 x[u].store(a, i[u]);
@@ -766,23 +845,14 @@ XSG_DEV void rows_adam(const AdamArrays& a, const AdamTerms& s, uint32_t count, 
 template <bool F32, bool STREAM, typename L>
 __global__ __launch_bounds__(kBlock) void adam_kernel(L list, AdamScalars s, StepSource source) {
     const StepTerms now = source.terms();
-    const int b = list.chunks - 1 - (int)blockIdx.x;
-    if (!now.taken || b < 0) return;
+    const int b = blockIdx.x;
+    if (!now.taken || b >= list.chunks) return;
     const int t = find_tensor(list, b);
     const auto& e = list.at(t);
     const Chunk chunk(list, e, b, t);
-    AdamTerms terms;
-    terms.c = now.c;
-    terms.rate = e.lr * now.over1;
-    terms.root = now.root;
-    terms.beta2 = s.beta2;
-    terms.one_minus_beta1 = s.one_minus_beta1;
-    terms.one_minus_beta2 = s.one_minus_beta2;
-    terms.eps = s.eps;
-    terms.keep = e.keep;
+    const AdamTerms terms = adam_terms(now, s, e.lr, e.keep);
     const int pt = F32 ? XSG_DTYPE_F32 : e.pdtype, gt = F32 ? XSG_DTYPE_F32 : e.gdtype;
-    const AdamArrays a{at(e.param, chunk.base, pt), at(e.gradient, chunk.base, gt), e.avg + chunk.base,
-                       e.sq + chunk.base};
+    const AdamArrays a = adam_arrays(e, chunk.base);
     const uint32_t phase = phase_of(a.p, pt);
     ChunkSpan span(chunk.count, phase);
     if (phase != phase_of(a.g, gt) || phase != phase_of(a.m, XSG_DTYPE_F32) || phase != phase_of(a.v, XSG_DTYPE_F32)) {
@@ -807,13 +877,151 @@ __global__ __launch_bounds__(kBlock) void adam_kernel(L list, AdamScalars s, Ste
     }
 }
 
+// A short list of few chunks (poses, biases, a head's weights): one workgroup does the whole call, a chunk to a
+// wavefront, so that there is one launch, which is most of such a call's time.
+// 16 chunks of 1024 elements: norm 5.8 us against 8.4 in two launches, clip 6.0 against 8.8; 24: 8.2 either way; 24
+// tensors of 4: 5.9. The update does more to an element: 24 tensors of 4 take 8.4 us against 9.7, 8 of 1024 take
+// 12.1 against 9.5.
+constexpr int kSmallBlock = 1024;
+constexpr int kSmallChunks = 64;                  // of tensors of up to kSmallTensor elements
+constexpr int kOneRound = kSmallBlock / 64;       // of longer ones, not for an update
+constexpr int64_t kSmallTensor = 256;
+
+enum SmallOp { kSmallNorm, kSmallClip, kSmallAdam };
+
+template <int UNROLL, typename F> XSG_DEV void for_lanes(const Chunk& chunk, const ChunkMask& mask, bool masked, F&& f) {
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t i0 = lane; i0 < chunk.count; i0 += 64 * UNROLL) {
+        uint32_t i[UNROLL];
+        bool on[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            i[u] = i0 + 64 * u;
+            on[u] = i[u] < chunk.count && (!masked || mask.one(i[u]));
+        }
+        f(i, on);
+    }
+}
+
+template <int NORM, int OP, typename E>
+__global__ __launch_bounds__(kSmallBlock) void small_kernel(InlineList<E> list, StepRule rule, AdamScalars s,
+                                                            int64_t* step, float* __restrict__ total,
+                                                            float* __restrict__ each) {
+    __shared__ double part[kSmallChunks];
+    __shared__ StepTerms shared;
+    __shared__ float corrections[2];
+    const int wave = threadIdx.x >> 6;
+    const double count = OP == kSmallAdam ? (double)(*step + 1) : 0.0;   // before it may change
+    if (OP == kSmallAdam && wave == kSmallBlock / 64 - 1) {
+        corrections[0] = (float)(-1.0 / expm1(count * rule.log_beta1));
+        corrections[1] = (float)(1.0 / sqrt(-expm1(count * rule.log_beta2)));
+    }
+    if (OP != kSmallAdam || rule.norm >= 0) {
+        for (int b = wave; b < list.chunks; b += kSmallBlock / 64) {
+            const int t = find_tensor(list, b);
+            const E& e = list.at(t);
+            const Chunk chunk(list, e, b, t);
+            const void* p = at(e.grad(), chunk.base, e.grad_dtype());
+            ChunkMask mask;
+            if (e.mask) mask.open(e.mask, chunk.base, e.row, e.magic, e.shift);
+            Accum<NORM> acc[kUnroll];
+            with_type(e.grad_dtype(), [&](auto dt) {
+                for_lanes<kUnroll>(chunk, mask, e.mask != nullptr, [&](const uint32_t* i, const bool* on) {
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u)
+                        if (on[u]) acc[u].add(load1<dt.value>(p, i[u]));
+                });
+            });
+#pragma unroll
+            for (int u = 1; u < kUnroll; ++u) acc[0].join(acc[u]);
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) acc[0].join(acc[0].shuffled(d));
+            if ((threadIdx.x & 63) == 0) part[b] = acc[0].value();
+        }
+    }
+    __syncthreads();
+    if (OP == kSmallNorm && each && threadIdx.x >= 64 && threadIdx.x - 64 < list.n) {
+        const int t = threadIdx.x - 64;
+        Accum<NORM> acc;
+        for (int b = list.first_of(t); b < list.first_of(t + 1); ++b) acc.join_value(part[b]);
+        each[t] = (float)acc.finish();
+    }
+    if (threadIdx.x < 64) {
+        StepTerms terms{1.0f, 1.0f, 1.0f, 1};
+        if (OP != kSmallAdam || rule.norm >= 0) {
+            Accum<NORM> acc;
+            if (threadIdx.x < list.chunks) acc.join_value(part[threadIdx.x]);
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) acc.join(acc.shuffled(d));
+            const double norm = acc.finish();
+            if (threadIdx.x == 0 && total) *total = (float)norm;
+            if (rule.clip) terms.c = clip_factor(norm, rule.max_norm, rule.clip_eps);
+            terms.taken = !rule.skip_nonfinite || norm < (double)INFINITY;
+        }
+        if (threadIdx.x == 0) {
+            if (OP == kSmallAdam && terms.taken) *step += 1;
+            shared = terms;
+        }
+    }
+    if (OP == kSmallNorm) return;
+    __syncthreads();
+    StepTerms now = shared;
+    if (OP == kSmallAdam) {
+        now.over1 = corrections[0];
+        now.root = corrections[1];
+    }
+    if (OP == kSmallClip ? now.c == 1.0f : !now.taken) return;
+    for (int b = wave; b < list.chunks; b += kSmallBlock / 64) {
+        const int t = find_tensor(list, b);
+        const E& e = list.at(t);
+        const Chunk chunk(list, e, b, t);
+        ChunkMask mask;
+        if (e.mask) mask.open(e.mask, chunk.base, e.row, e.magic, e.shift);
+        if constexpr (OP == kSmallClip) {
+            void* p = at(e.data, chunk.base, e.dtype);
+            with_type(e.dtype, [&](auto dt) {
+                for_lanes<kUnroll>(chunk, mask, e.mask != nullptr, [&](const uint32_t* i, const bool* on) {
+                    float x[kUnroll];
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u)
+                        if (on[u]) x[u] = load1<dt.value>(p, i[u]);
+#pragma unroll
+                    for (int u = 0; u < kUnroll; ++u)
+                        if (on[u]) store1<dt.value>(p, i[u], x[u] * now.c);
+                });
+            });
+        } else if constexpr (OP == kSmallAdam) {
+            const AdamTerms terms = adam_terms(now, s, e.lr, e.keep);
+            const AdamArrays a = adam_arrays(e, chunk.base);
+            with_type(e.pdtype, [&](auto pt) {
+                with_type(e.gdtype, [&](auto gt) {
+                    for_lanes<kUnroll>(chunk, mask, e.mask != nullptr, [&](const uint32_t* i, const bool* on) {
+                        Adam1<pt.value, gt.value> x[kUnroll];
+#pragma unroll
+                        for (int u = 0; u < kUnroll; ++u)
+                            if (on[u]) x[u].load(a, i[u]);
+#pragma unroll
+                        for (int u = 0; u < kUnroll; ++u) {
+                            if (!on[u]) continue;
+                            x[u].update(terms);
+                            x[u].store(a, i[u]);
+                        }
+                    });
+                });
+            });
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ host
+int64_t chunks_of(int64_t numel, int64_t size) {
+    return numel <= size ? (numel > 0 ? 1 : 0) : (numel + size - 1) / size;
+}
 int64_t chunk_for(int64_t elements, bool writes_far) {
     int64_t c = (elements + kTargetChunks - 1) / kTargetChunks;
     c = (c + kChunkUnit - 1) / kChunkUnit * kChunkUnit;
     return std::min(std::max(c, kChunkUnit), writes_far ? kWriteChunk : kMaxChunk);
 }
-int64_t chunks_of(int64_t numel, int64_t size) { return (numel + size - 1) / size; }
 
 int check_dtype(int dtype, const char* who, int i) {
     if (dtype != XSG_DTYPE_F32 && dtype != XSG_DTYPE_BF16 && dtype != XSG_DTYPE_F16)
@@ -835,7 +1043,8 @@ int check_rows(int64_t numel, const void* mask, int64_t rows, const char* who, i
 
 // rows of a mask: d = 2^shift needs no magic; else magic = floor(2^32 (2^shift - d) / d) + 1, 2^(shift-1) < d < 2^shift
 RowDiv row_div(int64_t numel, const void* mask, int64_t rows) {
-    const uint32_t d = mask && numel ? (uint32_t)(numel / rows) : 1u;
+    if (!mask || numel == 0) return RowDiv{1, 1, 0};
+    const uint32_t d = (uint32_t)(numel / rows);
     uint32_t shift = 0;
     while (((uint64_t)1 << shift) < d) ++shift;
     return RowDiv{d, (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift};
@@ -922,25 +1131,36 @@ template <typename T> void fill_inline(const T* ts, int n, const Plan& p, Inline
 template <typename T>
 int send_table(const T* ts, int n, const Plan& p, void* ws, hipStream_t s, TableList<EntryOf<T>>* list) {
     using E = EntryOf<T>;
+    using Piece = TablePiece<E>;
     int32_t* const first = (int32_t*)((char*)ws + p.first_at);
     E* const entry = (E*)((char*)ws + p.entry_at);
-    TablePiece<E> piece;
-    int32_t at = 0;
-    // first[n], the end, goes as one more tensor's first chunk
-    for (int i = 0; i <= n;) {
+    Piece piece;
+    int64_t chunks = 0;
+    for (int i = 0; i < n;) {
         const int i0 = i;
-        for (piece.n = 0; piece.n < kInline<E> && i < n; ++i, ++piece.n) {
-            piece.entry[piece.n] = entry_of(ts[i]);
-            piece.first[piece.n] = at;
-            at += (int32_t)chunks_of(ts[i].numel, ts[i].mask ? p.masked_chunk : p.chunk);
+        int kinds = 0, masks = 0;
+        for (piece.n = 0; piece.n < Piece::kMax && i < n; ++i, ++piece.n) {
+            const E e = entry_of(ts[i]);
+            const EntryKind kind = e.kind();
+            int k = 0, m = masks;   // a mask is mostly the last tensor's
+            while (k < kinds && !(piece.kind[k] == kind)) ++k;
+            while (e.mask && m > 0 && piece.mask[m - 1] != e.mask) --m;
+            if (k == Piece::kKinds || (e.mask && m == 0 && masks == Piece::kMasks)) break;
+            if (k == kinds) piece.kind[kinds++] = kind;
+            if (!e.mask) m = 0;
+            else if (m == 0) piece.mask[(m = ++masks) - 1] = e.mask;
+            e.pointers(piece.pointer[piece.n]);
+            piece.word[piece.n] = (uint64_t)e.numel | (uint64_t)k << 48 | (uint64_t)m << 56;
+            piece.first[piece.n] = (int32_t)chunks;
+            chunks += chunks_of(e.numel, e.mask ? p.masked_chunk : p.chunk);
         }
-        const bool last = i == n && piece.n < kInline<E>;
-        if (last) piece.first[piece.n] = at;
-        table_kernel<E><<<1, kBlock, 0, s>>>(piece, entry + i0, first + i0, last);
+        piece.kinds = kinds;
+        piece.masks = masks;
+        piece.end = i == n ? (int32_t)chunks : -1;
+        table_kernel<E><<<1, kBlock, 0, s>>>(piece, entry + i0, first + i0);
         XSG_TRY_LAUNCH("table");
-        if (last) break;
     }
-    *list = TableList<E>{entry, first, n, (int32_t)p.chunk, (int32_t)p.masked_chunk, at};
+    *list = TableList<E>{entry, first, n, (int32_t)p.chunk, (int32_t)p.masked_chunk, (int32_t)chunks};
     return XSG_OK;
 }
 
@@ -987,6 +1207,23 @@ int launch_partials(const L& list, int norm, const Plan& p, void* ws, int64_t* s
 }
 
 // the norm (where the rule has one) and the step's terms, for the launch behind
+template <int OP, typename T> bool is_small(const T* ts, int n, const Plan& p) {
+    if (p.table || p.chunks > kSmallChunks) return false;
+    return (OP != kSmallAdam && p.chunks <= kOneRound) ||
+           std::all_of(ts, ts + n, [](const T& x) { return x.numel <= kSmallTensor; });
+}
+
+template <int OP, typename T>
+int launch_small(const T* ts, int n, const Plan& p, const StepRule& rule, const AdamScalars& a, int64_t* step,
+                 float* total, float* each, hipStream_t s) {
+    InlineList<EntryOf<T>> list;
+    fill_inline(ts, n, p, &list);
+    with_norm(rule.norm, [&](auto kind) {
+        small_kernel<kind.value, OP><<<1, kSmallBlock, 0, s>>>(list, rule, a, step, total, each);
+    });
+    return xsg_launch_status("small list");
+}
+
 template <typename L>
 int make_terms(const L& list, const StepRule& rule, const Plan& p, void* ws, int64_t* step, float* total, hipStream_t s,
                StepSource* source) {
@@ -1022,6 +1259,9 @@ extern "C" int xsg_grad_norm(const xsg_grad_tensor* ts, int n, int norm, float* 
     rc = xsg_check_workspace(workspace, "grad_norm");
     if (rc != XSG_OK) return rc;
     const hipStream_t s = (hipStream_t)stream;
+    if (is_small<kSmallNorm>(ts, n, p))
+        return launch_small<kSmallNorm>(ts, n, p, StepRule{0.0, 0.0, 0.0, 0.0, norm, 0, 0}, AdamScalars{}, nullptr, total,
+                                        each, s);
     return with_list(ts, n, p, workspace, s, [&](const auto& list) {
         const int status = p.stream ? launch_partials<true>(list, norm, p, workspace, nullptr, s)
                                     : launch_partials<false>(list, norm, p, workspace, nullptr, s);
@@ -1050,8 +1290,10 @@ extern "C" int xsg_clip_grads(const xsg_grad_tensor* ts, int n, int norm, double
     rc = xsg_check_workspace(workspace, "clip_grads");
     if (rc != XSG_OK) return rc;
     const hipStream_t s = (hipStream_t)stream;
+    const StepRule rule{max_norm, eps, 0.0, 0.0, norm, 1, 0};
+    if (is_small<kSmallClip>(ts, n, p))
+        return launch_small<kSmallClip>(ts, n, p, rule, AdamScalars{}, nullptr, total, nullptr, s);
     return with_list(ts, n, p, workspace, s, [&](const auto& list) {
-        const StepRule rule{max_norm, eps, 0.0, 0.0, norm, 1, 0};
         StepSource source;
         const int status = make_terms(list, rule, p, workspace, nullptr, total, s, &source);
         if (status != XSG_OK) return status;
@@ -1098,6 +1340,7 @@ extern "C" int xsg_adam_step(const xsg_adam_tensor* ts, int n, const xsg_adam_op
     const StepRule rule{o->max_norm, kAdamClipEps, log(o->beta1), log(o->beta2), needs_norm ? o->norm : -1, o->clip,
                         o->skip_nonfinite};
     const hipStream_t s = (hipStream_t)stream;
+    if (is_small<kSmallAdam>(ts, n, p)) return launch_small<kSmallAdam>(ts, n, p, rule, a, step, total, nullptr, s);
     return with_list(ts, n, p, workspace, s, [&](const auto& list) {
         StepSource source;
         const int status = make_terms(list, rule, p, workspace, step, total, s, &source);
