@@ -558,7 +558,13 @@ __global__ __launch_bounds__(kBlock) void norm_partial_kernel(L list, int each, 
 
 template <int NORM> XSG_DEV Accum<NORM> join_partials(const double* __restrict__ partial, int n) {
     Accum<NORM> acc;
-    for (int i = threadIdx.x; i < n; i += kBlock) acc.join_value(partial[i]);
+    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * kBlock) {   // other XCDs wrote them: one far latency for eight
+        double v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = i0 + u * kBlock < n ? partial[i0 + u * kBlock] : 0.0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) acc.join_value(v[u]);
+    }
     return block_join<NORM>(acc);
 }
 

@@ -723,6 +723,10 @@ struct Spans {
     }
 };
 
+// Workspace on the current device and stream, from the allocator that tensors come from (making a tensor of it
+// costs more than the memory, and these calls can be shorter than 10 us).
+c10::DataPtr scratch(size_t bytes) { return c10::GetAllocator(c10::kCUDA)->allocate(bytes); }
+
 void mark_written(const Tensor& t) {   // autograd notices what it saved before
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -738,9 +742,9 @@ std::tuple<Tensor, OptT> grad_norm(const py::list& tensors, double norm_type, co
     const int n = (int)a.list.size();
     Tensor total = at::empty({}, opts), each;
     if (per_tensor) each = at::empty({n}, opts);
-    Tensor ws = workspace(like, xsg_grad_norm_workspace_bytes(a.list.data(), n));
+    const c10::DataPtr ws = scratch(xsg_grad_norm_workspace_bytes(a.list.data(), n));
     check_rc(xsg_grad_norm(a.list.data(), n, kind, total.data_ptr<float>(),
-                           per_tensor ? each.data_ptr<float>() : nullptr, ws.data_ptr(), stream_of(like)));
+                           per_tensor ? each.data_ptr<float>() : nullptr, ws.get(), stream_of(like)));
     return {total, per_tensor ? OptT(each) : OptT()};
 }
 
@@ -765,8 +769,8 @@ Tensor clip_grads_(const py::list& tensors, double max_norm, double norm_type, d
     const Tensor& like = tensor_at(tensors, 0, "tensor");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(like.device());
     Tensor total = at::empty({}, like.options().dtype(at::kFloat));
-    Tensor ws = workspace(like, xsg_clip_grads_workspace_bytes(a.list.data(), (int)n));
-    check_rc(xsg_clip_grads(a.list.data(), (int)n, kind, max_norm, eps, total.data_ptr<float>(), ws.data_ptr(),
+    const c10::DataPtr ws = scratch(xsg_clip_grads_workspace_bytes(a.list.data(), (int)n));
+    check_rc(xsg_clip_grads(a.list.data(), (int)n, kind, max_norm, eps, total.data_ptr<float>(), ws.get(),
                             stream_of(like)));
     for (size_t i = 0; i < n; ++i) mark_written(tensor_at(tensors, i, "tensor"));
     for (const auto& [i, copy] : a.copies) tensor_at(tensors, i, "tensor").copy_(copy);
@@ -864,13 +868,11 @@ OptT adam_step_(const py::list& params, const py::list& grads, const py::list& e
     spans.check();
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
     const bool normed = o.clip || o.skip_nonfinite;
-    Tensor total, ws;
+    Tensor total;
     if (normed) total = at::empty({}, like.options().dtype(at::kFloat));
-    const size_t bytes = xsg_adam_step_workspace_bytes(list.data(), (int)n, &o);
-    if (bytes > 0) ws = workspace(like, bytes);
+    const c10::DataPtr ws = scratch(xsg_adam_step_workspace_bytes(list.data(), (int)n, &o));
     check_rc(xsg_adam_step(list.data(), (int)n, &o, step.data_ptr<int64_t>(),
-                           normed ? total.data_ptr<float>() : nullptr, bytes > 0 ? ws.data_ptr() : nullptr,
-                           stream_of(like)));
+                           normed ? total.data_ptr<float>() : nullptr, ws.get(), stream_of(like)));
     for (size_t i = 0; i < n; ++i) {
         mark_written(tensor_at(params, i, "parameter"));
         mark_written(tensor_at(exp_avgs, i, "exp_avg"));
