@@ -832,13 +832,13 @@ XSG_DEV void rows_adam(const AdamArrays& a, const AdamTerms& s, uint32_t count, 
             }
         });
     } else {
-        for_kept_rows<1, kAdamUnroll<STREAM>>(mask, count, [&](const uint32_t* i, const bool* on) {
-            Adam1<PT, GT> x[kAdamUnroll<STREAM>];
+        for_kept_rows<1, kUnroll>(mask, count, [&](const uint32_t* i, const bool* on) {
+            Adam1<PT, GT> x[kUnroll];
 #pragma unroll
-            for (int u = 0; u < kAdamUnroll<STREAM>; ++u)
+            for (int u = 0; u < kUnroll; ++u)
                 if (on[u]) x[u].load(a, i[u]);
 #pragma unroll
-            for (int u = 0; u < kAdamUnroll<STREAM>; ++u) {
+            for (int u = 0; u < kUnroll; ++u) {
                 if (!on[u]) continue;
                 x[u].update(s);
                 x[u].store(a, i[u]);
