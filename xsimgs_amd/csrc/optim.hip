@@ -18,12 +18,15 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int64_t kChunkUnit = 1024;      // chunks are multiples of this many elements
-constexpr int64_t kTargetChunks = 2048;   // of a call whose tensors are long enough: every CU's eight workgroups
+// Workgroups that share out the elements of a call whose tensors are long enough. Dense tensors stream best from
+// four long runs to a CU (4 M Gaussians: clip 442 us, 456 with eight), under masks the lists of rows are latency that
+// eight hide (1 M with 14 % kept: norm 19 us, 27 with four).
+constexpr int64_t kDenseChunks = 1024, kMaskedChunks = 2048;
 // Longest chunk of a call that writes more than the caches hold: many short workgroups follow each other through
 // memory, where few long ones write in as many places at once (an update of 236 M elements: 2048 chunks 1310 us,
 // 57618 chunks 1230, around the caches 1145).
 constexpr int64_t kWriteChunk = 4096;
-constexpr int64_t kMaskedChunks = 4;      // such chunks to one of a masked tensor
+constexpr int64_t kMaskedFactor = 4;      // such chunks to one of a masked tensor, of which little is kept
 constexpr int64_t kMaxChunk = 1 << 26;    // offsets inside a chunk are 32-bit, in bytes
 constexpr int64_t kCacheBytes = (int64_t)256 << 20;   // of the last-level cache
 constexpr int64_t kMaxRow = 1 << 30;      // and so are rows under a mask
@@ -1023,8 +1026,8 @@ __global__ __launch_bounds__(kSmallBlock) void small_kernel(InlineList<E> list, 
 int64_t chunks_of(int64_t numel, int64_t size) {
     return numel <= size ? (numel > 0 ? 1 : 0) : (numel + size - 1) / size;
 }
-int64_t chunk_for(int64_t elements, bool writes_far) {
-    int64_t c = (elements + kTargetChunks - 1) / kTargetChunks;
+int64_t chunk_for(int64_t elements, int64_t target, bool writes_far) {
+    int64_t c = (elements + target - 1) / target;
     c = (c + kChunkUnit - 1) / kChunkUnit * kChunkUnit;
     return std::min(std::max(c, kChunkUnit), writes_far ? kWriteChunk : kMaxChunk);
 }
@@ -1097,6 +1100,7 @@ size_t aligned(size_t x) { return (x + 255) / 256 * 256; }
 template <typename T> int make_plan(const T* ts, int n, const char* who, bool norm, bool writes, Plan* p) {
     if (n < 0 || (n > 0 && !ts)) return xsg_fail(XSG_ERR_INVALID, "%s: null or negative list of tensors", who);
     int64_t grad_bytes = 0;
+    bool masked = false;
     for (int i = 0; i < n; ++i) {
         if (ts[i].numel < 0) return xsg_fail(XSG_ERR_INVALID, "%s: tensor %d has a negative size", who, i);
         if (ts[i].numel > kMaxElements - p->elements) return xsg_fail(XSG_ERR_INVALID, "%s: too many elements", who);
@@ -1104,15 +1108,17 @@ template <typename T> int make_plan(const T* ts, int n, const char* who, bool no
         p->bytes_touched += touched(ts[i]);
         grad_bytes += ts[i].numel * type_size(grad_of(ts[i]).dtype);
         p->f32 = p->f32 && all_f32(ts[i]);
+        masked = masked || ts[i].mask;
     }
     p->stream = p->bytes_touched > kCacheBytes;
     // a call that writes gains nothing from it (4 M Gaussians: clip 454 us either way, update 1249 and 1280)
     p->stream_norm = !writes && grad_bytes > kCacheBytes;
-    p->chunk = chunk_for(p->elements, writes && p->stream);
-    p->masked_chunk = writes && p->stream ? kMaskedChunks * p->chunk : p->chunk;
+    const int64_t target = masked ? kMaskedChunks : kDenseChunks;
+    p->chunk = chunk_for(p->elements, target, writes && p->stream);
+    p->masked_chunk = writes && p->stream ? kMaskedFactor * p->chunk : p->chunk;
     for (int i = 0; i < n; ++i) p->chunks += chunks_of(ts[i].numel, ts[i].mask ? p->masked_chunk : p->chunk);
     if (p->chunks > kMaxChunks) return xsg_fail(XSG_ERR_INVALID, "%s: too many tensors", who);
-    if (writes) p->each = std::max<int64_t>((p->chunks + kTargetChunks - 1) / kTargetChunks, 1);
+    if (writes) p->each = std::max<int64_t>((p->chunks + target - 1) / target, 1);
     p->parts = (p->chunks + p->each - 1) / p->each;
     p->table = n > kInline<EntryOf<T>>;
     p->bytes = norm ? 256 + aligned((size_t)p->parts * sizeof(double)) : 0;
