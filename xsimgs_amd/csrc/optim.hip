@@ -6,7 +6,8 @@
 // travels in the kernels' arguments (no copy from the host, and a captured graph holds it by value): a short one
 // in the arguments of each kernel, a long one piece by piece into the workspace, so that each pass stays one
 // launch over all tensors. Sums are held in 64 bits and added in a fixed order, so a call's results are the
-// same bits each time.
+// same bits each time. Scaling and update are computed in 32 bits and rounded once, to the type the tensor has;
+// moments stay in 32 bits, since squares of half-precision gradients would fall out of 16 (1e-4 squared).
 #include <math.h>
 
 #include <algorithm>
@@ -31,7 +32,8 @@ constexpr int64_t kMaxChunk = 1 << 26;    // offsets inside a chunk are 32-bit, 
 constexpr int64_t kCacheBytes = (int64_t)256 << 20;   // of the last-level cache
 constexpr int64_t kMaxRow = 1 << 30;      // and so are rows under a mask
 constexpr int64_t kMaxElements = (int64_t)1 << 41;
-constexpr int64_t kMaxChunks = 1 << 30;
+constexpr int64_t kMaxChunks = (1 << 24) - 1;   // a launch of one workgroup each holds fewer than 2^32 threads
+constexpr int64_t kFarChunks = 1 << 22;         // of long writing calls, beside a last short one of every tensor
 constexpr int kArgumentBytes = 3900;      // of a list, beside the other arguments in 4 KB
 
 // Division of n < 2^31 by the row length: (mulhi(n, magic) + n) >> shift
@@ -214,6 +216,7 @@ static_assert(sizeof(InlineList<GradEntry>) <= 3920 && sizeof(InlineList<AdamEnt
                   sizeof(GradEntry) % 8 == 0 && sizeof(AdamEntry) % 8 == 0,
               "lists share 4 KB with the other arguments; entries are loaded by words");
 
+// 2.1 us a piece, a launch's and an argument's latency: 505 tensors take four pieces (gradients) or seven (updates).
 template <typename E>
 __global__ __launch_bounds__(kBlock) void table_kernel(TablePiece<E> piece, E* __restrict__ entry,
                                                        int32_t* __restrict__ first) {
@@ -392,7 +395,8 @@ template <bool STREAM> constexpr int kAdamUnroll = STREAM ? 4 : 2;
 
 // Under a mask of short rows each wavefront lists the kept rows of its share of the chunk (a mask word a lane, so
 // up to 2048 rows for one load's latency) and then walks their elements alone, VEC at a time, so that lanes are
-// busy and loads in flight however few rows are kept.
+// busy and loads in flight however few rows are kept (1 M Gaussians with 14 % kept: norm 41 -> 24 us against a look
+// at every group of four, the update's kernel 119 -> 86).
 // many(i[], on[]): UNROLL units of VEC elements from element i, of which those not on are left out.
 constexpr uint32_t kShortRow = 128;
 
@@ -530,6 +534,8 @@ struct Chunk {
     }
 };
 
+// Bound by its reads: 236 M float32 166 us (5.7 TB/s), 59 M 35 us (in part from the last-level cache); 1 M
+// Gaussians with 14 % kept 17 us, of which the list of rows is most.
 // A workgroup sums `each` chunks in a row. `step`, unless null, counts one step more; the launches behind this
 // one read it.
 template <int NORM, bool STREAM, typename L>
@@ -705,6 +711,7 @@ XSG_DEV void rows_scale(void* p, float c, uint32_t count, bool whole, const Chun
     }
 }
 
+// x <- c x, bound by reads and writes: 236 M float32 268 us (7.0 TB/s of both). One chunk a workgroup.
 template <bool STREAM, typename L>
 __global__ __launch_bounds__(kBlock) void clip_scale_kernel(L list, StepSource source) {
     const int b = blockIdx.x, t = find_tensor(list, b);   // while the partial sums are on their way
@@ -851,6 +858,8 @@ XSG_DEV void rows_adam(const AdamArrays& a, const AdamTerms& s, uint32_t count, 
     }
 }
 
+// The update, bound by four reads and three writes of an element: 236 M float32 1060 us (6.2 TB/s), 1 M Gaussians
+// with 14 % kept 80 us (412 MB moved in sectors of 64 bytes, 5.1 TB/s).
 // F32: every parameter and gradient is float32
 template <bool F32, bool STREAM, typename L>
 __global__ __launch_bounds__(kBlock) void adam_kernel(L list, AdamScalars s, StepSource source) {
@@ -1027,9 +1036,8 @@ int64_t chunks_of(int64_t numel, int64_t size) {
     return numel <= size ? (numel > 0 ? 1 : 0) : (numel + size - 1) / size;
 }
 int64_t chunk_for(int64_t elements, int64_t target, bool writes_far) {
-    int64_t c = (elements + target - 1) / target;
-    c = (c + kChunkUnit - 1) / kChunkUnit * kChunkUnit;
-    return std::min(std::max(c, kChunkUnit), writes_far ? kWriteChunk : kMaxChunk);
+    const auto share = [&](int64_t of) { return ((elements + of - 1) / of + kChunkUnit - 1) / kChunkUnit * kChunkUnit; };
+    return std::min(std::max(share(target), kChunkUnit), writes_far ? std::max(kWriteChunk, share(kFarChunks)) : kMaxChunk);
 }
 
 int check_dtype(int dtype, const char* who, int i) {
