@@ -292,7 +292,7 @@ typedef struct {
 typedef struct {
     double beta1, beta2, eps;
     int clip;               /* 1: gradients count as scaled by min(1, max_norm / (norm + 1e-6)) */
-    int skip_nonfinite;     /* 1: a norm that is not finite leaves everything, the counter too, as it is */
+    int skip_nonfinite;     /* 1: a norm that is not finite in float32 leaves everything, the counter too, as it is */
     int norm;               /* XSG_NORM_*, with either of the above */
     double max_norm;
 } xsg_adam_options;

@@ -639,7 +639,7 @@ XSG_DEV StepTerms step_terms(const StepRule& rule, const double* __restrict__ pa
         const bool first = blockIdx.x == 0 && threadIdx.x == 0;
         if (first && total) *total = (float)norm;
         if (rule.clip) terms.c = clip_factor(norm, rule.max_norm, rule.clip_eps);
-        if (rule.skip_nonfinite && !(norm < (double)INFINITY)) {
+        if (rule.skip_nonfinite && !((float)norm < INFINITY)) {   // by the norm as the caller has it
             if (first) *step -= 1;
             terms.taken = 0;
         }
@@ -974,7 +974,7 @@ __global__ __launch_bounds__(kSmallBlock) void small_kernel(InlineList<E> list, 
             const double norm = acc.finish();
             if (threadIdx.x == 0 && total) *total = (float)norm;
             if (rule.clip) terms.c = clip_factor(norm, rule.max_norm, rule.clip_eps);
-            terms.taken = !rule.skip_nonfinite || norm < (double)INFINITY;
+            terms.taken = !rule.skip_nonfinite || (float)norm < INFINITY;   // by the norm as the caller has it
         }
         if (threadIdx.x == 0) {
             if (OP == kSmallAdam && terms.taken) *step += 1;

@@ -23,9 +23,9 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
 
     ``step``: one int64 value on the GPU, which then holds t. ``lr`` and ``weight_decay``: a number, or one per
     tensor. ``masks`` as in ``grad_norm`` (rows out of the mask do not change, and do not count in the norm).
-    ``skip_nonfinite``: a norm that is not finite leaves everything as it is, ``step`` too. Returns the norm
-    before clipping (with ``max_norm`` or ``skip_nonfinite``, else None). Parameters and gradients are float32,
-    bfloat16 or float16; moments are float32 tensors of their parameter's sizes and strides."""
+    ``skip_nonfinite``: a norm that is not finite (as returned, in float32) leaves everything as it is, ``step``
+    too. Returns the norm before clipping (with ``max_norm`` or ``skip_nonfinite``, else None). Parameters and
+    gradients are float32, bfloat16 or float16; moments are float32 tensors of their parameter's sizes and strides."""
     params = list(params)
     return _C.adam_step_(params, list(grads), list(exp_avgs), list(exp_avg_sqs), step, _rates(lr),
                          _rates(weight_decay), float(betas[0]), float(betas[1]), float(eps),
