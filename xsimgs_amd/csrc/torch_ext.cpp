@@ -641,7 +641,9 @@ const uint32_t* mask_of(const py::list& masks, size_t i, const Tensor& t, int64_
     TORCH_CHECK(m.device() == t.device(), "All tensors must be on the same device");
     TORCH_CHECK(m.is_contiguous(), "All tensors must be contiguous");
     TORCH_CHECK(t.dim() >= 1, "a masked tensor needs a first dimension of rows (tensor ", i, " has none)");
-    TORCH_CHECK(m.numel() * 32 >= t.size(0), "Packed mask size mismatch with tensor ", i, " of ", t.size(0), " rows");
+    // more words than the rows need are another tensor's, or another dimension's: their bits mean other rows
+    TORCH_CHECK(m.numel() == (t.size(0) + 31) / 32, "Packed mask size mismatch with tensor ", i, ": ", m.numel(),
+                " words for ", t.size(0), " rows");
     *rows = t.size(0);
     return (const uint32_t*)m.data_ptr();
 }
