@@ -72,3 +72,82 @@ def test_sh_of_the_second_layout_by_rows(dev, n):
     got = optim.adam_step_(p, g, m, v, step, lr=1e-2, eps=1e-15, max_norm=0.5 * norm, masks=_pack(keep.numpy()).to(dev))
     _close(got, norm, 2 * U)
     _check_update((p, m, v), before, 12, [1e-2] * rows, [0.0] * rows, 0.5 * norm / (norm + 1e-6), [keep] * rows)
+
+
+def _scene(kind):
+    from xsimgs_amd import synthetic
+
+    if kind == "lidar":
+        return synthetic.make_cfg3(seed=4, n=4000, width=128, n_beams=16)
+    if kind == "camera":
+        sc = synthetic.make_cfg0(seed=2, n=3000, width=96, height=64)
+        sc.means[:500, 0] += 900.0   # beside the image
+    else:
+        sc = synthetic.make_cfg4(seed=4, n=6000, n_blobs=40)
+        sc.cameras = synthetic.rig_cameras(80, 48, 63.0)[:3]   # a half of the circle
+        sc.means[:500, 2] += 900.0   # above it
+    return sc
+
+
+@pytest.mark.parametrize("kind", ["camera", "rig", "lidar"])
+def test_train_frame_updates_what_it_says(dev, kind):
+    """Two steps of a frame, a rig and a lidar beside float64: the scene's parameters under their mask, and
+    beside them parameters without dimensions and of the Gaussians' number, which no mask may hold back."""
+    from xsimgs_amd import frame
+
+    sc = _scene(kind)
+    st = frame.prepare(sc, dev)
+    gen = torch.Generator().manual_seed(1)
+    cams = sc.cameras if kind == "rig" else sc.cameras[:1]
+    shape = ((len(cams),) if kind == "rig" else ()) + (cams[0].height, cams[0].width)
+    channels = 2 if kind == "lidar" else 3
+    image = [(1e-3 * torch.randn(*s, generator=gen)).to(dev) for s in ((*shape, channels), shape, shape)]
+    exposure, table = torch.nn.Parameter(torch.tensor(0.5, device=dev)), torch.nn.Parameter(torch.ones(sc.n, device=dev))
+    opt = frame.make_optimizer(st, max_norm=1e-2)
+    opt.add_param_group(dict(params=[exposure, table], lr=1e-2, name="others"))
+    assert len(opt.param_groups) == 6
+    params = [p for group in opt.param_groups for p in group["params"]]
+    rates = [group["lr"] for group in opt.param_groups for _ in group["params"]]
+    moments = [[torch.zeros(p.shape) for p in params] for _ in range(2)]
+    own = [torch.tensor(3e-3), torch.randn(sc.n, generator=gen) * 1e-3]
+    for t in (1, 2):
+        old = [p.detach().cpu().clone() for p in params]
+        exposure.grad, table.grad = (x.to(dev) for x in own)
+        out = frame.train_frame(st, opt, image, rig=kind == "rig")
+        grads = [out["grads"][group["name"]].cpu() for group in opt.param_groups[:5]] + own
+        keep = torch.ones(sc.n, dtype=torch.bool)
+        if kind != "lidar":
+            seen = (out["radii"] > 0).all(-1).cpu()
+            keep = seen.any(0) if kind == "rig" else seen
+            assert 0 < int(keep.sum()) <= sc.n - 500
+            assert not any(bool(g[~keep].any()) for g in grads[:5])
+        norm = _norm64([_f64(g) for g in grads], 2.0)
+        _close(out["grad_norm"], norm, 2 * U)
+        now = [[p.detach() for p in params]] + [[opt.state[p][k] for p in params] for k in ("exp_avg", "exp_avg_sq")]
+        everything = torch.ones(sc.n, dtype=torch.bool)
+        keeps = [keep] * 5 + [torch.ones((), dtype=torch.bool), everything]
+        _check_update(now, (old, grads, *moments), t, rates, [0.0] * 7, min(1.0, 1e-2 / (norm + 1e-6)), keeps)
+        assert exposure.grad is None and table.grad is None and st.means.grad is not None
+        assert float(exposure.detach()) != float(old[5]) and not bool((table.detach().cpu() == old[6]).any())
+        moments = [[x.cpu().clone() for x in xs] for xs in now[1:]]
+
+
+def test_train_frame_with_a_pose(dev):
+    """A camera's position beside the scene: its gradient is this frame's alone, not a sum over the steps."""
+    from xsimgs_amd import frame
+
+    st = frame.prepare(_scene("camera"), dev)
+    position = st.cams[0].pose.t.requires_grad_()
+    gen = torch.Generator().manual_seed(1)
+    image = [torch.randn(*s, generator=gen).to(dev) for s in ((64, 96, 3), (64, 96), (64, 96))]
+    opt = frame.make_optimizer(st, rates=dict.fromkeys(frame.RATES, 0.0))
+    opt.add_param_group(dict(params=[position], lr=0.0))
+    frame.render_frame(st, backward=True, grads=image)
+    once = position.grad.clone()
+    assert bool(once.any())
+    position.grad = None
+    for t in (1, 2, 3):
+        frame.train_frame(st, opt, image)
+        # equal gradients: m is (1 - beta1^t) times them, but for the order of the frame's sums
+        m = opt.state[position]["exp_avg"]
+        assert bool(((m - (1 - 0.9 ** t) * once).abs() <= 1e-4 * once.abs().max()).all()), t

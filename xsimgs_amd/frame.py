@@ -205,7 +205,9 @@ def train_frame(st: FrameState, optimizer: Adam, grads, cam_index: int = 0, rig:
     """One training step: the frame (of one camera, or of the whole rig) forward and backward, then the
     optimizer's update with whatever clipping it carries. In a regular tiling only the Gaussians that some
     tile can hold are updated (their packed mask from the projection's radii; the others' gradients are
-    zeros, their momentum rests). Returns the frame's outputs and ``grad_norm`` before clipping."""
+    zeros, their momentum rests). Parameters beside the scene's (a pose, an exposure) are updated whole, from
+    what the frame's backward and the caller's own before this call gave them; these gradients count for one
+    step and are cleared behind it. Returns the frame's outputs and ``grad_norm`` before clipping."""
     zero_grads(st)
     if rig:
         out = render_rig(st, backward=True, grads=grads)
@@ -214,13 +216,21 @@ def train_frame(st: FrameState, optimizer: Adam, grads, cam_index: int = 0, rig:
     masks = None
     if rig or st.scene.cameras[cam_index].kind in REGULAR_TILING:
         mask = packed_visibility_mask(out["radii"].detach().contiguous())
-        masks = {p: mask for group in optimizer.param_groups for p in group["params"] if p.shape[0] == st.scene.n}
+        masks = {t: mask for t in _leaves(st)}
     optimizer.step(masks=masks)
     out["grad_norm"] = optimizer.grad_norm
+    scene = {id(t) for t in _leaves(st)}
+    for group in optimizer.param_groups:
+        for p in group["params"]:
+            if id(p) not in scene:
+                p.grad = None
     return out
 
 
+def _leaves(st: FrameState) -> list:
+    return [t for t in (st.means, st.log_scales, st.quats, st.opacity_logits, st.sh, st.colors) if t is not None]
+
+
 def zero_grads(st: FrameState) -> None:
-    for t in (st.means, st.log_scales, st.quats, st.opacity_logits, st.sh, st.colors):
-        if t is not None:
-            t.grad = None
+    for t in _leaves(st):
+        t.grad = None
