@@ -1,0 +1,80 @@
+"""What ``optim.Adam`` keeps over copies, pickles and checkpoints, and what it refuses to take up. CPU only: the
+native update is replaced by float64 arithmetic on the same arguments."""
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+
+from xsimgs_amd import optim
+
+OPTIONS = dict(betas=(0.8, 0.95), eps=1e-7, max_norm=0.5, norm_type=1.0, skip_nonfinite=True)
+
+
+@pytest.fixture(autouse=True)
+def calls(monkeypatch):
+    """The arguments of each update, which is computed as adam_step_ documents it."""
+    seen = []
+
+    def update(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas, eps, weight_decay, max_norm, norm_type,
+               skip_nonfinite, masks):
+        seen.append(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_norm=max_norm, norm_type=norm_type,
+                         skip_nonfinite=skip_nonfinite, masks=masks))
+        norm = torch.linalg.vector_norm(torch.cat([g.double().reshape(-1) for g in grads]), norm_type)
+        c = 1.0 if max_norm is None else min(1.0, max_norm / (float(norm) + 1e-6))
+        step += 1
+        t = int(step)
+        for p, g, m, v, rate, decay in zip(params, grads, exp_avgs, exp_avg_sqs, lr, weight_decay):
+            assert m.dtype == v.dtype == torch.float32
+            g = c * g.double()
+            m.copy_(betas[0] * m.double() + (1 - betas[0]) * g)
+            v.copy_(betas[1] * v.double() + (1 - betas[1]) * g * g)
+            root = (v.double() / (1 - betas[1] ** t)).sqrt() + eps
+            p.copy_(p.double() * (1 - rate * decay) - rate / (1 - betas[0] ** t) * m.double() / root)
+        return norm.float() if max_norm is not None or skip_nonfinite else None
+
+    monkeypatch.setattr("xsimgs_amd.optim.adam.adam_step_", update)
+    return seen
+
+
+def _params():
+    g = torch.Generator().manual_seed(5)
+    return [torch.nn.Parameter(torch.randn(s, generator=g)) for s in ((6, 3), (4,))] + \
+           [torch.nn.Parameter(torch.randn(7, generator=g).bfloat16())]
+
+
+def _optimizer(ps, **options):
+    return optim.Adam([dict(params=ps[:1], lr=1e-2, name="means"), dict(params=ps[1:], weight_decay=0.1)], lr=3e-3,
+                      **options)
+
+
+def _run(opt, ts):
+    ps = [p for group in opt.param_groups for p in group["params"]]
+    for t in ts:
+        for i, p in enumerate(ps):
+            p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(10 * t + i)).to(p.dtype)
+        opt.step()
+    return [p.detach().clone() for p in ps]
+
+
+@pytest.mark.parametrize("steps", [0, 2])
+@pytest.mark.parametrize("how", ["copy", "pickle", "save"])
+def test_copies_go_on_alike(calls, how, steps):
+    opt = _optimizer(_params(), **OPTIONS)
+    _run(opt, range(steps))
+    if how == "copy":
+        other = copy.deepcopy(opt)
+    elif how == "pickle":
+        other = pickle.loads(pickle.dumps(opt))
+    else:
+        torch.save(opt, file := io.BytesIO())
+        file.seek(0)
+        other = torch.load(file, weights_only=False)
+    assert {k: getattr(other, k) for k in OPTIONS} == OPTIONS
+    assert (other.step_count is None) == (steps == 0) and (steps == 0 or int(other.step_count) == steps)
+    want = _run(opt, range(steps, steps + 2))
+    assert steps == 0 or int(other.step_count) == steps   # its own counter, not the first one's
+    got = _run(other, range(steps, steps + 2))
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and int(other.step_count) == int(opt.step_count) == steps + 2
+    assert calls[-1] == calls[-3] and torch.equal(other.grad_norm, opt.grad_norm)

@@ -49,6 +49,11 @@ class Adam(torch.optim.Optimizer):
         self.step_count = None   # int64 [1] on the parameters' GPU, from the first step on
         self.grad_norm = None
 
+    def __getstate__(self):
+        """What a copy or a pickle takes along: the base class knows its own attributes only."""
+        own = ("betas", "eps", "max_norm", "norm_type", "skip_nonfinite", "step_count", "grad_norm")
+        return dict(super().__getstate__(), **{k: getattr(self, k) for k in own})
+
     def add_param_group(self, param_group):
         if shared := {"betas", "eps", "max_norm", "norm_type", "skip_nonfinite"} & set(param_group):
             raise ValueError(f"{sorted(shared)} hold for the whole optimizer; a group may set lr and weight_decay")
