@@ -78,3 +78,33 @@ def test_copies_go_on_alike(calls, how, steps):
     got = _run(other, range(steps, steps + 2))
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and int(other.step_count) == int(opt.step_count) == steps + 2
     assert calls[-1] == calls[-3] and torch.equal(other.grad_norm, opt.grad_norm)
+
+
+@pytest.mark.parametrize("through_file", [False, True])
+def test_a_state_dict_brings_the_options(calls, through_file):
+    """A resumed run goes on with what was saved, whatever the optimizer was built with."""
+    opt = _optimizer(_params(), **OPTIONS)
+    _run(opt, range(2))
+    saved = opt.state_dict()
+    if through_file:
+        torch.save(saved, file := io.BytesIO())
+        file.seek(0)
+        saved = torch.load(file, weights_only=True)
+    kept = copy.deepcopy(saved)
+    other = _optimizer([torch.nn.Parameter(p.detach().clone()) for g in opt.param_groups for p in g["params"]],
+                       betas=(0.5, 0.5), eps=1e-3)
+    other.load_state_dict(saved)
+    assert {k: getattr(other, k) for k in OPTIONS} == OPTIONS
+    got = _run(other, [2, 3])
+    for i, state in saved["state"].items():   # the other optimizer's steps write nothing of what was saved
+        assert all(torch.equal(state[k], kept["state"][i][k]) for k in state)
+    assert int(saved["step"]) == 2
+    assert all(torch.equal(a, b) for a, b in zip(got, _run(opt, [2, 3]))) and calls[-1] == calls[-3]
+
+
+def test_a_state_dict_without_options_leaves_them():
+    opt = _optimizer(_params(), **OPTIONS)
+    _run(opt, [0])
+    other = _optimizer(_params(), betas=(0.5, 0.5), max_norm=2.0)
+    other.load_state_dict({k: v for k, v in opt.state_dict().items() if k != "options"})
+    assert other.betas == (0.5, 0.5) and other.max_norm == 2.0 and not other.skip_nonfinite and int(other.step_count) == 1

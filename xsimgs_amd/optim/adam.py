@@ -33,6 +33,9 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
                          listed_masks(masks, len(params)))
 
 
+_OPTIONS = ("betas", "eps", "max_norm", "norm_type", "skip_nonfinite")   # of a whole optimizer
+
+
 class Adam(torch.optim.Optimizer):
     """Adam over ``adam_step_``. Groups carry their own ``lr`` and ``weight_decay``; betas, eps, ``max_norm``,
     ``norm_type`` and ``skip_nonfinite`` hold for the whole optimizer, whose tensors are one list with one norm
@@ -51,11 +54,10 @@ class Adam(torch.optim.Optimizer):
 
     def __getstate__(self):
         """What a copy or a pickle takes along: the base class knows its own attributes only."""
-        own = ("betas", "eps", "max_norm", "norm_type", "skip_nonfinite", "step_count", "grad_norm")
-        return dict(super().__getstate__(), **{k: getattr(self, k) for k in own})
+        return dict(super().__getstate__(), **{k: getattr(self, k) for k in (*_OPTIONS, "step_count", "grad_norm")})
 
     def add_param_group(self, param_group):
-        if shared := {"betas", "eps", "max_norm", "norm_type", "skip_nonfinite"} & set(param_group):
+        if shared := set(_OPTIONS) & set(param_group):
             raise ValueError(f"{sorted(shared)} hold for the whole optimizer; a group may set lr and weight_decay")
         super().add_param_group(param_group)
 
@@ -90,11 +92,16 @@ class Adam(torch.optim.Optimizer):
         return loss
 
     def state_dict(self):
-        return dict(super().state_dict(), step=None if self.step_count is None else self.step_count.clone())
+        """The base class's, with the step counter and the options that hold for the whole optimizer."""
+        return dict(super().state_dict(), step=None if self.step_count is None else self.step_count.clone(),
+                    options={k: getattr(self, k) for k in _OPTIONS})
 
     def load_state_dict(self, state_dict):
-        """The moments come back in float32 (the base class would give them their parameter's type)."""
-        super().load_state_dict({k: v for k, v in state_dict.items() if k != "step"})
+        """Options are taken over as the groups' rates are (a dict without any leaves those of this optimizer).
+        The moments come back in float32 (the base class would give them their parameter's type)."""
+        super().load_state_dict({k: v for k, v in state_dict.items() if k not in ("step", "options")})
+        for k, v in state_dict.get("options", {}).items():
+            setattr(self, k, tuple(v) if k == "betas" else v)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
