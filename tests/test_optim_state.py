@@ -108,3 +108,16 @@ def test_a_state_dict_without_options_leaves_them():
     other = _optimizer(_params(), betas=(0.5, 0.5), max_norm=2.0)
     other.load_state_dict({k: v for k, v in opt.state_dict().items() if k != "options"})
     assert other.betas == (0.5, 0.5) and other.max_norm == 2.0 and not other.skip_nonfinite and int(other.step_count) == 1
+
+
+def test_a_state_dict_is_of_one_time():
+    """Moments and counter in a dict belong together, also after further steps of its optimizer."""
+    opt = _optimizer(_params())
+    _run(opt, range(2))
+    saved = opt.state_dict()
+    now = _run(opt, [2])
+    params = [torch.nn.Parameter(p.clone()) for p in now]
+    other = _optimizer(params)
+    other.load_state_dict(saved)
+    assert int(other.step_count) == int(opt.step_count) == 3
+    assert all(torch.equal(a, b) for a, b in zip(_run(other, [3]), _run(opt, [3])))

@@ -92,9 +92,9 @@ class Adam(torch.optim.Optimizer):
         return loss
 
     def state_dict(self):
-        """The base class's, with the step counter and the options that hold for the whole optimizer."""
-        return dict(super().state_dict(), step=None if self.step_count is None else self.step_count.clone(),
-                    options={k: getattr(self, k) for k in _OPTIONS})
+        """The base class's, with the step counter and the options that hold for the whole optimizer. The counter
+        is the optimizer's own tensor, as the moments are: copy the dict to keep it over further steps."""
+        return dict(super().state_dict(), step=self.step_count, options={k: getattr(self, k) for k in _OPTIONS})
 
     def load_state_dict(self, state_dict):
         """Options are taken over as the groups' rates are (a dict without any leaves those of this optimizer).
