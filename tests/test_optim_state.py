@@ -121,3 +121,46 @@ def test_a_state_dict_is_of_one_time():
     other.load_state_dict(saved)
     assert int(other.step_count) == int(opt.step_count) == 3
     assert all(torch.equal(a, b) for a, b in zip(_run(other, [3]), _run(opt, [3])))
+
+
+@pytest.mark.parametrize("steps", [0, 2])
+@pytest.mark.parametrize("other", [torch.optim.Adam, torch.optim.AdamW, torch.optim.SGD])
+def test_another_optimizers_state_dict_is_refused(other, steps):
+    """Warm moments with a counter that starts again would be corrected as a first step's; nothing changes."""
+    ps = _params()
+    foreign = other([dict(params=ps[:1]), dict(params=ps[1:])], lr=0.1)
+    _run(foreign, range(steps))
+    opt = _optimizer(_params())
+    _run(opt, [0])
+    before = copy.deepcopy(opt.state_dict())
+    with pytest.raises(ValueError, match="state dict of this optimizer"):
+        opt.load_state_dict(foreign.state_dict())
+    after = opt.state_dict()
+    assert after["param_groups"] == before["param_groups"] and int(after["step"]) == 1
+    for i, state in before["state"].items():
+        assert state.keys() == after["state"][i].keys()
+        assert all(torch.equal(state[k], after["state"][i][k]) for k in state)
+    if other is torch.optim.Adam and steps:   # in this optimizer's form its moments and count go on
+        theirs = foreign.state_dict()
+        opt.load_state_dict(dict(before, step=torch.tensor([steps]), state={
+            i: {k: v[k] for k in ("exp_avg", "exp_avg_sq")} for i, v in theirs["state"].items()}))
+        assert int(opt.step_count) == steps
+        first = opt.param_groups[0]["params"][0]
+        assert torch.equal(opt.state[first]["exp_avg"], theirs["state"][0]["exp_avg"])
+
+
+def test_a_state_dict_with_a_part_missing_is_refused():
+    opt = _optimizer(_params())
+    _run(opt, [0])
+    whole = opt.state_dict()
+    for part in (dict(whole, step=None), {k: v for k, v in whole.items() if k != "step"},
+                 dict(whole, state={0: dict(exp_avg=torch.zeros(6, 3))})):
+        with pytest.raises(ValueError, match="state dict of this optimizer"):
+            _optimizer(_params()).load_state_dict(part)
+    narrow = copy.deepcopy(whole)
+    narrow["state"][0]["exp_avg"] = narrow["state"][0]["exp_avg"][:1]   # would fit by repetition
+    with pytest.raises(ValueError, match="not of its sizes"):
+        opt.load_state_dict(narrow)
+    fresh = _optimizer(_params())
+    fresh.load_state_dict(_optimizer(_params()).state_dict())   # before a first step there is none of it
+    assert fresh.step_count is None and not fresh.state

@@ -98,12 +98,22 @@ class Adam(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Options are taken over as the groups' rates are (a dict without any leaves those of this optimizer).
-        The moments come back in float32 (the base class would give them their parameter's type)."""
+        The moments come back in float32 (the base class would give them their parameter's type). Another
+        optimizer's dict is refused: torch.optim.Adam's, say, counts each parameter's steps and holds options
+        that mean something else here. Its moments can come in a dict of this form, where all its counts agree."""
+        moments = {"exp_avg", "exp_avg_sq"}
+        states = [set(v) for v in state_dict["state"].values() if v]
+        if "step" not in state_dict or any(s != moments for s in states) or (states and state_dict["step"] is None):
+            raise ValueError("not a state dict of this optimizer: it has exp_avg and exp_avg_sq for each parameter and "
+                             "one step counter (step) beside them")
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            if any(v.shape != p.shape for v in state_dict["state"].get(i, {}).values()):
+                raise ValueError(f"the moments of parameter {i} are not of its sizes {tuple(p.shape)}")
         super().load_state_dict({k: v for k, v in state_dict.items() if k not in ("step", "options")})
         for k, v in state_dict.get("options", {}).items():
             setattr(self, k, tuple(v) if k == "betas" else v)
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
             for k, v in state_dict["state"].get(i, {}).items():
                 self.state[p][k] = torch.empty_like(p, dtype=torch.float32).copy_(v)
