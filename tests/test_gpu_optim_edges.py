@@ -151,3 +151,17 @@ def test_train_frame_with_a_pose(dev):
         # equal gradients: m is (1 - beta1^t) times them, but for the order of the frame's sums
         m = opt.state[position]["exp_avg"]
         assert bool(((m - (1 - 0.9 ** t) * once).abs() <= 1e-4 * once.abs().max()).all()), t
+
+
+def test_rates_on_the_gpu_are_refused(dev):
+    from xsimgs_amd import optim
+
+    x = torch.ones(4, device=dev)
+    far = torch.tensor([0.1], device=dev)
+    for name in ("lr", "weight_decay"):
+        with pytest.raises(ValueError, match=f"{name} must be a number"):
+            optim.adam_step_([x], [x.clone()], [x.clone()], [x.clone()], torch.zeros(1, dtype=torch.int64, device=dev),
+                             **dict(dict(lr=1e-3), **{name: far}))
+        with pytest.raises(ValueError, match=f"{name} must be a number"):
+            optim.Adam([torch.nn.Parameter(x)], **{name: far[0]})
+    assert bool((x == 1).all())

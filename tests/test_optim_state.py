@@ -164,3 +164,31 @@ def test_a_state_dict_with_a_part_missing_is_refused():
     fresh = _optimizer(_params())
     fresh.load_state_dict(_optimizer(_params()).state_dict())   # before a first step there is none of it
     assert fresh.step_count is None and not fresh.state
+
+
+@pytest.mark.parametrize("name", ["lr", "weight_decay"])
+def test_rates_on_another_device_are_refused(calls, name):
+    """Reading one back would wait for the GPU in every step. (A device without memory stands for the GPU.)"""
+    far, near = torch.empty((), device="meta"), torch.tensor(0.25)
+    ps = _params()
+    with pytest.raises(ValueError, match=f"{name} must be a number"):
+        optim.Adam(ps, **{name: far})
+    opt = _optimizer(ps)
+    opt.param_groups[1][name] = far
+    with pytest.raises(ValueError, match=f"{name} must be a number"):
+        _run(opt, [0])
+    assert not calls and not opt.state
+    opt.param_groups[1][name] = near
+    _run(opt, [0])
+    assert calls[0][name] == [opt.param_groups[0][name], 0.25, 0.25]
+    opt = optim.Adam(ps, **{name: near})   # a tensor that its owner changes
+    near.fill_(0.5)
+    _run(opt, [0])
+    assert calls[1][name] == [0.5] * 3
+    x = torch.ones(4)
+    from xsimgs_amd import _C
+    for value in (far, [far]):
+        args = dict(lr=1e-3, weight_decay=0.0, beta1=0.9, beta2=0.99, eps=1e-8, max_norm=None, norm_type=2.0,
+                    skip_nonfinite=False, masks=[])
+        with pytest.raises(ValueError, match=f"{name} must be a number"):
+            _C.adam_step_([x], [x], [x], [x], torch.zeros(1, dtype=torch.int64), **dict(args, **{name: value}))

@@ -792,12 +792,14 @@ struct Rates {
             TORCH_CHECK_VALUE((size_t)PyList_GET_SIZE(value.ptr()) == n, name, " must be a number or hold one per tensor: ",
                               PyList_GET_SIZE(value.ptr()), " for ", n);
             each.resize(n);
-            for (size_t i = 0; i < n; ++i) each[i] = number(PyList_GET_ITEM(value.ptr(), (Py_ssize_t)i));
+            for (size_t i = 0; i < n; ++i) each[i] = number(PyList_GET_ITEM(value.ptr(), (Py_ssize_t)i), name);
         } else {
-            same = number(value.ptr());
+            same = number(value.ptr(), name);
         }
     }
-    static double number(PyObject* o) {
+    static double number(PyObject* o, const char* name) {
+        TORCH_CHECK_VALUE(!THPVariable_Check(o) || THPVariable_Unpack(o).is_cpu(), name,
+                          " must be a number or a tensor on the CPU: one on the GPU would be read back");
         const double v = PyFloat_AsDouble(o);
         if (v == -1.0 && PyErr_Occurred()) throw py::error_already_set();
         return v;

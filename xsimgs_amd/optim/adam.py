@@ -12,6 +12,12 @@ def _rates(value):
     return value if isinstance(value, (int, float)) else list(value)
 
 
+def _number(value, name) -> float:
+    if isinstance(value, torch.Tensor) and value.device.type != "cpu":
+        raise ValueError(f"{name} must be a number or a tensor on the CPU: one on {value.device} would be read back")
+    return float(value)
+
+
 def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay=0.0, max_norm: float | None = None, norm_type: float = 2.0,
                skip_nonfinite: bool = False, masks=None):
@@ -22,7 +28,7 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
         p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
 
     ``step``: one int64 value on the GPU, which then holds t. ``lr`` and ``weight_decay``: a number, or one per
-    tensor. ``masks`` as in ``grad_norm`` (rows out of the mask do not change, and do not count in the norm).
+    tensor (not on the GPU: they would be read back). ``masks`` as in ``grad_norm`` (rows out of the mask do not change, and do not count in the norm).
     ``skip_nonfinite``: a norm that is not finite (as returned, in float32) leaves everything as it is, ``step``
     too. Returns the norm before clipping (with ``max_norm`` or ``skip_nonfinite``, else None). Parameters and
     gradients are float32, bfloat16 or float16; moments are float32 tensors of their parameter's sizes and strides."""
@@ -44,7 +50,7 @@ class Adam(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-15, weight_decay: float = 0.0, *,
                  max_norm: float | None = None, norm_type: float = 2.0, skip_nonfinite: bool = False):
-        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
+        if _number(lr, "lr") < 0.0 or eps < 0.0 or _number(weight_decay, "weight_decay") < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
             raise ValueError("lr, eps and weight_decay must not be negative, betas must lie in [0, 1)")
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay))
         self.betas, self.eps = tuple(betas), eps
@@ -70,11 +76,12 @@ class Adam(torch.optim.Optimizer):
                 loss = closure()
         params, lr, decay = [], [], []
         for group in self.param_groups:
+            rate, share = _number(group["lr"], "lr"), _number(group["weight_decay"], "weight_decay")
             for p in group["params"]:
                 if p.grad is not None:
                     params.append(p)
-                    lr.append(float(group["lr"]))
-                    decay.append(float(group["weight_decay"]))
+                    lr.append(rate)
+                    decay.append(share)
         self.grad_norm = None
         if not params:
             return loss
