@@ -1,5 +1,6 @@
 """The training step's operators and optimizer at the edges of what they take."""
 import math
+import random
 
 import pytest
 import torch
@@ -165,3 +166,61 @@ def test_rates_on_the_gpu_are_refused(dev):
         with pytest.raises(ValueError, match=f"{name} must be a number"):
             optim.Adam([torch.nn.Parameter(x)], **{name: far[0]})
     assert bool((x == 1).all())
+
+
+def _places(t, base):
+    """The bytes of base that t's elements lie in, each as often as it has an element there."""
+    at = torch.zeros((), dtype=torch.int64)
+    for size, stride in zip(t.shape, t.stride()):
+        at = at.unsqueeze(-1) + torch.arange(size) * stride
+    first = t.data_ptr() - base.data_ptr() + at.reshape(-1) * t.element_size()
+    return (first.unsqueeze(-1) + torch.arange(t.element_size())).reshape(-1).tolist()
+
+
+def test_strided_tensors_that_share_elements_are_refused(dev):
+    from xsimgs_amd import optim
+
+    base = torch.ones(40, 30, device=dev)
+    flat = base.view(-1)
+    for ts in ([base[:, :5], base[:, 4:9]], [base, base[:, 3]], [base[:, 3], base], [base[:, 3:9], base[7, :4]],
+               [base[:, ::2].t(), base[5:6, 4]], [base[::2], base.t()[:, 2:3]], [flat[::6], flat[10::4]],
+               [flat[1::2], flat.view(torch.int16).view(torch.float16)[3::400]]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            optim.clip_grads_(ts, 1e-3)
+    for t in (flat.as_strided((5, 7), (2, 3)), flat.as_strided((4, 3), (1, 1)), flat.as_strided((3, 3, 2), (10, 0, 1))):
+        with pytest.raises(RuntimeError, match="share memory"):
+            optim.clip_grads_([flat[1000:], t], 1e-3)
+    assert bool((base == 1).all())
+    # between each other's elements, in steps of other sizes and with elements of another type
+    parts = [flat[::4], flat[2::4], base[:, 1:20:2][::2], base[:, 21::2][1::2],
+             base[1::2, 1:20].view(torch.float16)[:, ::4].t()]
+    assert optim.clip_grads_(parts, 1e9).isfinite()
+
+
+def test_strided_tensors_any_way(dev):
+    """Small views at random, of one buffer and two element sizes: refused exactly where elements are shared."""
+    from xsimgs_amd import optim
+
+    rng, told = random.Random(5), {True: 0, False: 0}
+    for _ in range(300):
+        base = torch.ones(64, device=dev)
+        ts = []
+        for _ in range(rng.randint(1, 3)):
+            buffer = base if rng.random() < 0.7 else base.view(torch.float16)
+            sizes = [rng.randint(1, 4) for _ in range(rng.randint(1, 3))]
+            strides = [rng.randint(1, 12) for _ in sizes]
+            reach = sum((n - 1) * s for n, s in zip(sizes, strides))
+            if reach < buffer.numel():
+                ts.append(buffer.as_strided(sizes, strides, rng.randrange(buffer.numel() - reach)))
+        if not ts:
+            continue
+        places = [i for t in ts for i in _places(t, base)]
+        shared = len(set(places)) < len(places)
+        told[shared] += 1
+        if shared:
+            with pytest.raises(RuntimeError, match="overlap|share memory"):
+                optim.clip_grads_(ts, 1e-3)
+            assert bool((base == 1).all())
+        else:
+            optim.clip_grads_(ts, 1e9)
+    assert min(told.values()) > 60, told

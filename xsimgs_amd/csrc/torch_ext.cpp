@@ -2,12 +2,13 @@
 // xsimgs_amd C-ABI. This file validates and allocates exactly as the reference ops do, then calls
 // the HIP kernels through include/xsimgs_amd.h on the current stream of the input's device.
 #include <torch/extension.h>
-#include <ATen/MemoryOverlap.h>
+#include <c10/util/SmallVector.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 #include <optional>
 #include <string>
 #include <vector>
@@ -725,6 +726,103 @@ struct Spans {
     }
 };
 
+// Whether sum of step[k] x[k] = target with 0 <= x[k] <= last[k], by search from the largest step down: what the
+// smaller ones can still add up to, and their common divisor, leave few values of each x to look at where steps
+// nest as a tensor's do. A search that grows too long is taken to have found one.
+struct Steps {
+    struct Term {
+        int64_t step, last;
+    };
+    c10::SmallVector<Term, 16> terms;
+    c10::SmallVector<int64_t, 17> most, divisor;   // of terms[k] and those behind it
+    int budget = 100000;
+
+    void add(int64_t step, int64_t last) {
+        if (last > 0) terms.push_back({step, last});
+    }
+    bool reach(int64_t target) {
+        std::sort(terms.begin(), terms.end(), [](const Term& a, const Term& b) { return a.step > b.step; });
+        size_t kept = 0;
+        for (const Term& t : terms) {
+            if (kept > 0 && terms[kept - 1].step == t.step) terms[kept - 1].last += t.last;
+            else terms[kept++] = t;
+        }
+        terms.resize(kept);
+        most.assign(kept + 1, 0);
+        divisor.assign(kept + 1, 0);
+        for (size_t k = kept; k-- > 0;) {
+            most[k] = most[k + 1] + terms[k].step * terms[k].last;
+            divisor[k] = std::gcd(divisor[k + 1], terms[k].step);
+        }
+        return search(0, target);
+    }
+    bool search(size_t k, int64_t target) {
+        if (target < 0 || target > most[k]) return false;
+        if (target == 0) return true;
+        if (target % divisor[k] != 0) return false;
+        const int64_t step = terms[k].step, over = target - most[k + 1];
+        const int64_t hi = std::min(terms[k].last, target / step);
+        for (int64_t x = over > 0 ? (over + step - 1) / step : 0; x <= hi; ++x)
+            if (--budget < 0 || search(k + 1, target - x * step)) return true;
+        return false;
+    }
+};
+
+// Where a tensor's elements lie: from lo on, in steps of its strides.
+struct Lattice {
+    uint64_t lo, hi;   // bytes
+    int64_t size;      // of an element
+    bool dense;
+    c10::SmallVector<Steps::Term, 8> terms;   // in elements
+
+    Lattice(const Tensor& t, bool dense_)
+        : lo(reinterpret_cast<uintptr_t>(t.data_ptr())), hi(lo), size((int64_t)t.element_size()), dense(dense_) {
+        if (t.numel() == 0) return;
+        if (dense) {
+            terms.push_back({1, t.numel() - 1});
+        } else {
+            for (int64_t d = 0; d < t.dim(); ++d)
+                if (t.size(d) > 1) terms.push_back({t.stride(d), t.size(d) - 1});
+        }
+        std::sort(terms.begin(), terms.end(), [](const auto& a, const auto& b) { return a.step > b.step; });
+        hi += size;
+        for (const auto& x : terms) hi += x.step * x.last * size;
+    }
+    // two different indices, one place: their difference, with its first part that is not 0 positive, adds up to 0
+    bool meets_itself() const {
+        if (!terms.empty() && terms.back().step == 0) return true;
+        int64_t behind = 0;
+        for (size_t k = terms.size(); k-- > 0; behind += terms[k].step * terms[k].last) {
+            if (terms[k].step > behind) continue;
+            Steps steps;
+            steps.add(terms[k].step, terms[k].last - 1);
+            for (size_t j = k + 1; j < terms.size(); ++j) steps.add(terms[j].step, 2 * terms[j].last);
+            if (steps.reach(behind - terms[k].step)) return true;
+        }
+        return false;
+    }
+    // a place of both: this one's index forward and the other's backward from its last element
+    bool meets(const Lattice& o) const {
+        const int64_t apart = (int64_t)(o.lo - lo), length = (int64_t)(o.hi - o.lo);
+        const bool alike = size == o.size && apart % size == 0;   // else byte by byte
+        const int64_t unit = alike ? 1 : size, other = alike ? 1 : o.size;
+        Steps steps;
+        for (const auto& x : terms) steps.add(x.step * unit, x.last);
+        for (const auto& x : o.terms) steps.add(x.step * other, x.last);
+        if (!alike) steps.add(1, size + o.size - 2);
+        return steps.reach(alike ? apart / size + length / size - 1 : apart + length - 1);
+    }
+};
+
+// Strided tensors may lie between each other's elements; none may share one.
+void check_apart(std::vector<Lattice>& list) {
+    std::sort(list.begin(), list.end(), [](const Lattice& a, const Lattice& b) { return a.lo < b.lo; });
+    for (size_t i = 0; i < list.size(); ++i)
+        for (size_t j = i + 1; j < list.size() && list[j].lo < list[i].hi; ++j)
+            TORCH_CHECK((list[i].dense && list[j].dense) || !list[i].meets(list[j]),
+                        "the tensors overlap in memory: each one that is written must be given once");
+}
+
 // Workspace on the current device and stream, from the allocator that tensors come from (making a tensor of it
 // costs more than the memory, and these calls can be shorter than 10 us).
 c10::DataPtr scratch(size_t bytes) { return c10::GetAllocator(c10::kCUDA)->allocate(bytes); }
@@ -756,17 +854,21 @@ Tensor clip_grads_(const py::list& tensors, double max_norm, double norm_type, d
     GradArgs a = grad_args(tensors, masks);
     const size_t n = a.list.size();
     Spans spans;
+    std::vector<Lattice> written;   // of all tensors, where some are strided
     size_t copied = 0;
     for (size_t i = 0; i < n; ++i) {
         const Tensor& t = tensor_at(tensors, i, "tensor");
-        if (copied < a.copies.size() && a.copies[copied].first == i) {
+        const bool strided = copied < a.copies.size() && a.copies[copied].first == i;
+        if (strided) {
             ++copied;
-            TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, "tensor ", i,
+            TORCH_CHECK(!Lattice(t, false).meets_itself(), "tensor ", i,
                         " has elements that share memory and cannot be scaled in place");
         } else {
             spans.add(a.list[i].data, a.list[i].numel * t.element_size(), true);
         }
+        if (!a.copies.empty() && t.numel() > 0) written.emplace_back(t, !strided);
     }
+    check_apart(written);
     spans.check();
     const Tensor& like = tensor_at(tensors, 0, "tensor");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(like.device());
