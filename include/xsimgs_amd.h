@@ -277,6 +277,12 @@ size_t xsg_clip_grads_workspace_bytes(const xsg_grad_tensor* tensors, int n);
 int xsg_clip_grads(const xsg_grad_tensor* tensors, int n, int norm, double max_norm, double eps, float* total,
                    void* workspace, xsg_stream_t stream);
 
+/* Writes a dense copy back into the strided tensor that it was made of: element i of src, counted in row order
+ * over sizes[dims], goes to its place in dst (strides in elements; no two of one place), where its bits differ and
+ * its row is in the mask. Elements of 2 or 4 bytes, up to 16 dimensions, mask and rows as above. */
+int xsg_write_back(void* dst, const void* src, int64_t numel, int element_bytes, int dims, const int64_t* sizes,
+                   const int64_t* strides, const uint32_t* mask, int64_t rows, xsg_stream_t stream);
+
 typedef struct {
     void* param;
     const void* grad;

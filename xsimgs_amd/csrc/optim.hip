@@ -733,6 +733,35 @@ __global__ __launch_bounds__(kBlock) void clip_scale_kernel(L list, StepSource s
     });
 }
 
+// Elements of a strided tensor that took their turn in a dense copy. Rows out of the mask are not touched (they may be
+// another stream's to write meanwhile), and what did not change is not written. An element a lane and turn, its place
+// by a division for each dimension left.
+constexpr int kMaxDims = 16;
+struct Strides {
+    int64_t size[kMaxDims], stride[kMaxDims];
+    int dims;
+};
+
+template <typename T, typename I>
+__global__ __launch_bounds__(kBlock) void write_back_kernel(T* __restrict__ dst, const T* __restrict__ src, I numel,
+                                                            Strides at, const uint32_t* __restrict__ mask, I row) {
+    for (I i = (I)blockIdx.x * kBlock + threadIdx.x; i < numel; i += (I)gridDim.x * kBlock) {
+        if (mask) {
+            const I r = i / row;
+            if (!((mask[r >> 5] >> (r & 31)) & 1u)) continue;
+        }
+        I rest = i;
+        int64_t place = 0;
+        for (int d = at.dims - 1; d >= 0; --d) {
+            const I q = rest / (I)at.size[d];
+            place += (int64_t)(rest - q * (I)at.size[d]) * at.stride[d];
+            rest = q;
+        }
+        const T x = src[i];
+        if (dst[place] != x) dst[place] = x;
+    }
+}
+
 struct AdamScalars {
     float beta2, one_minus_beta1, one_minus_beta2, eps;
 };
@@ -1326,6 +1355,43 @@ extern "C" int xsg_clip_grads(const xsg_grad_tensor* ts, int n, int norm, double
         });
         return xsg_launch_status("clip_grads");
     });
+}
+
+extern "C" int xsg_write_back(void* dst, const void* src, int64_t numel, int element_bytes, int dims, const int64_t* sizes,
+                              const int64_t* strides, const uint32_t* mask, int64_t rows, xsg_stream_t stream) {
+    if (numel < 0 || numel > kMaxElements) return xsg_fail(XSG_ERR_INVALID, "write_back: %lld elements", (long long)numel);
+    if (dims < 0 || dims > kMaxDims || (dims > 0 && (!sizes || !strides)))
+        return xsg_fail(XSG_ERR_INVALID, "write_back: %d dimensions, more than %d or without sizes", dims, kMaxDims);
+    if (element_bytes != 2 && element_bytes != 4)
+        return xsg_fail(XSG_ERR_INVALID, "write_back: elements of %d bytes", element_bytes);
+    Strides at{};
+    at.dims = dims;
+    int64_t count = 1;
+    for (int d = 0; d < dims; ++d) {
+        at.size[d] = sizes[d];
+        at.stride[d] = strides[d];
+        if (sizes[d] < 0) count = -1;
+        if (count < 0) break;
+        count = sizes[d] > 0 && count > kMaxElements / sizes[d] ? kMaxElements + 1 : count * sizes[d];
+    }
+    if (count != numel)
+        return xsg_fail(XSG_ERR_INVALID, "write_back: sizes do not make %lld elements", (long long)numel);
+    const int rc = check_rows(numel, mask, rows, "write_back", 0);
+    if (rc != XSG_OK || numel == 0) return rc;
+    if (!dst || !src) return xsg_fail(XSG_ERR_INVALID, "write_back: null array");
+    const int blocks = (int)std::min<int64_t>((numel + kBlock - 1) / kBlock, 1 << 14);
+    const int64_t row = mask ? numel / rows : 1;
+    // indices of 32 bits where a turn past the last element stays within them
+    const bool narrow = numel <= ((int64_t)1 << 31);
+    const hipStream_t s = (hipStream_t)stream;
+    const auto launch = [&](auto element, auto index) {
+        using T = decltype(element);
+        using I = decltype(index);
+        write_back_kernel<T, I><<<blocks, kBlock, 0, s>>>((T*)dst, (const T*)src, (I)numel, at, mask, (I)row);
+    };
+    if (element_bytes == 4) narrow ? launch(uint32_t{}, uint32_t{}) : launch(uint32_t{}, uint64_t{});
+    else narrow ? launch(uint16_t{}, uint32_t{}) : launch(uint16_t{}, uint64_t{});
+    return xsg_launch_status("write_back");
 }
 
 extern "C" size_t xsg_adam_step_workspace_bytes(const xsg_adam_tensor* ts, int n, const xsg_adam_options* o) {

@@ -848,6 +848,23 @@ std::tuple<Tensor, OptT> grad_norm(const py::list& tensors, double norm_type, co
     return {total, per_tensor ? OptT(each) : OptT()};
 }
 
+// t from its dense copy; neighbouring dimensions that step alike go as one
+void write_back(const Tensor& t, const Tensor& copy, const xsg_grad_tensor& x) {
+    c10::SmallVector<int64_t, 8> sizes, strides;
+    for (int64_t d = 0; d < t.dim(); ++d) {
+        if (t.size(d) == 1) continue;
+        if (!sizes.empty() && strides.back() == t.size(d) * t.stride(d)) {
+            sizes.back() *= t.size(d);
+            strides.back() = t.stride(d);
+        } else {
+            sizes.push_back(t.size(d));
+            strides.push_back(t.stride(d));
+        }
+    }
+    check_rc(xsg_write_back(t.data_ptr(), copy.data_ptr(), t.numel(), (int)t.element_size(), (int)sizes.size(), sizes.data(),
+                            strides.data(), x.mask, x.rows, stream_of(t)));
+}
+
 Tensor clip_grads_(const py::list& tensors, double max_norm, double norm_type, double eps, const py::list& masks) {
     const int kind = norm_kind(norm_type);
     at::NoGradGuard no_grad;
@@ -877,7 +894,7 @@ Tensor clip_grads_(const py::list& tensors, double max_norm, double norm_type, d
     check_rc(xsg_clip_grads(a.list.data(), (int)n, kind, max_norm, eps, total.data_ptr<float>(), ws.get(),
                             stream_of(like)));
     for (size_t i = 0; i < n; ++i) mark_written(tensor_at(tensors, i, "tensor"));
-    for (const auto& [i, copy] : a.copies) tensor_at(tensors, i, "tensor").copy_(copy);
+    for (const auto& [i, copy] : a.copies) write_back(tensor_at(tensors, i, "tensor"), copy, a.list[i]);
     return total;
 }
 

@@ -35,7 +35,8 @@ def grad_norm(tensors, norm_type: float = 2.0, *, masks=None, per_tensor: bool =
 def clip_grads_(tensors, max_norm: float, norm_type: float = 2.0, *, eps: float = 1e-6, masks=None) -> torch.Tensor:
     """Scales ``tensors`` in place by min(1, max_norm / (norm + eps)) and returns the norm before. Where the
     factor is 1 nothing is written; a norm that is not finite acts as in torch.nn.utils.clip_grad_norm_
-    (NaN spreads, infinity zeros the finite values). No two tensors may share an element; strided ones may lie
+    (NaN spreads, infinity zeros the finite values). A tensor that is not dense (or, under a mask, not contiguous)
+    is worked on in a dense copy, which reads all of it; what changed is written back. No two tensors may share an element; strided ones may lie
     between each other's (should it take too long to tell, they are refused)."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     return _C.clip_grads_(tensors, float(max_norm), float(norm_type), float(eps), listed_masks(masks, len(tensors)))
