@@ -224,3 +224,25 @@ def test_strided_tensors_any_way(dev):
         else:
             optim.clip_grads_(ts, 1e9)
     assert min(told.values()) > 60, told
+
+
+@pytest.mark.parametrize("clip", [False, True])
+@pytest.mark.parametrize("lists", LISTS)
+def test_rate_and_correction_are_rounded_once(dev, lists, clip):
+    """Where everything else is exact in float32 (p = 0, m = g = v = 1, eps = 0, beta2 = 1/2 after many steps), a
+    step is the corrected rate itself: lr / (1 - beta1^t), rounded to the nearest float32."""
+    from xsimgs_amd import optim
+
+    sizes = LISTS[lists]
+    g, m, v = ([torch.ones(s, device=dev) for s in sizes] for _ in range(3))
+    rng = random.Random(3)
+    for _ in range(20 if lists != "many chunks" else 4):
+        t, beta1 = rng.randint(60, 200), rng.choice([0.9, 0.95, 0.99])
+        rates = [10 ** rng.uniform(-6, -1) for _ in sizes]
+        p = [torch.zeros(s, device=dev) for s in sizes]
+        step = torch.full((1,), t - 1, dtype=torch.int64, device=dev)
+        optim.adam_step_(p, g, m, v, step, lr=rates, betas=(beta1, 0.5), eps=0.0, max_norm=1e9 if clip else None)
+        assert all(bool((x == 1).all()) for xs in (m, v) for x in xs)
+        for x, lr in zip(p, rates):
+            want = torch.tensor(-lr / (1.0 - beta1 ** t), dtype=torch.float64).float()
+            assert bool((x.cpu() == want).all()), (lr, beta1, t, float(x.view(-1)[0]), float(want))

@@ -103,8 +103,9 @@ template <int DT, bool STREAM> XSG_DEV void store4(void* p, uint32_t i, f32x4 x,
 }
 // What tensors of a long list have in common: most of it has few kinds.
 struct EntryKind {
+    double lr;
     uint32_t row, magic;
-    float lr, keep;
+    float keep;
     uint8_t shift, dtype, gdtype;
     bool operator==(const EntryKind& o) const {
         return row == o.row && lr == o.lr && keep == o.keep && dtype == o.dtype && gdtype == o.gdtype;
@@ -120,7 +121,7 @@ struct GradEntry {
     uint8_t shift, dtype;
     XSG_HD const void* grad() const { return data; }
     XSG_HD int grad_dtype() const { return dtype; }
-    EntryKind kind() const { return EntryKind{row, magic, 0.0f, 0.0f, shift, dtype, 0}; }
+    EntryKind kind() const { return EntryKind{0.0, row, magic, 0.0f, shift, dtype, 0}; }
     void pointers(uint64_t* to) const { to[0] = (uint64_t)data; }
     XSG_DEV void set(const uint64_t* ptr, int64_t numel_, const uint32_t* mask_, const EntryKind& k) {
         data = (void*)ptr[0];
@@ -140,12 +141,13 @@ struct AdamEntry {
     float *avg, *sq;
     int64_t numel;
     const uint32_t* mask;
+    double lr;
     uint32_t row, magic;
-    float lr, keep;           // keep: 1 - lr * weight decay
+    float keep;               // 1 - lr * weight decay
     uint8_t shift, pdtype, gdtype;
     XSG_HD const void* grad() const { return gradient; }
     XSG_HD int grad_dtype() const { return gdtype; }
-    EntryKind kind() const { return EntryKind{row, magic, lr, keep, shift, pdtype, gdtype}; }
+    EntryKind kind() const { return EntryKind{lr, row, magic, keep, shift, pdtype, gdtype}; }
     void pointers(uint64_t* to) const {
         to[0] = (uint64_t)param;
         to[1] = (uint64_t)gradient;
@@ -609,8 +611,8 @@ XSG_DEV float clip_factor(double norm, double max_norm, double eps) {
 
 // What a call that writes takes from the norm and the step counter.
 struct StepTerms {
+    double over1;   // 1 / (1 - beta1^t); its product with a rate is rounded, not itself
     float c;        // the clip factor
-    float over1;    // 1 / (1 - beta1^t)
     float root;     // 1 / sqrt(1 - beta2^t)
     int taken;      // 0: the step is left out
 };
@@ -626,13 +628,14 @@ struct StepRule {
 // the step is not taken (what another one then made of it goes unused). The counter already counts this step.
 XSG_DEV StepTerms step_terms(const StepRule& rule, const double* __restrict__ partial, int n, int64_t* step,
                              float* __restrict__ total) {
-    StepTerms terms{1.0f, 1.0f, 1.0f, 1};
-    __shared__ float corrections[2];
+    StepTerms terms{1.0, 1.0f, 1.0f, 1};
+    __shared__ double over1;
+    __shared__ float root;
     // 1 - beta^t without the cancellation, in 64 bits not cheap: by the wavefront with the fewest partial sums
     if (step && threadIdx.x >= kBlock - 64) {
         const double t = (double)*step;
-        corrections[0] = (float)(-1.0 / expm1(t * rule.log_beta1));
-        corrections[1] = (float)(1.0 / sqrt(-expm1(t * rule.log_beta2)));
+        over1 = -1.0 / expm1(t * rule.log_beta1);
+        root = (float)(1.0 / sqrt(-expm1(t * rule.log_beta2)));
     }
     if (rule.norm >= 0) {
         const double norm = norm_of(partial, n, rule.norm);
@@ -647,8 +650,8 @@ XSG_DEV StepTerms step_terms(const StepRule& rule, const double* __restrict__ pa
         __syncthreads();
     }
     if (step) {
-        terms.over1 = corrections[0];
-        terms.root = corrections[1];
+        terms.over1 = over1;
+        terms.root = root;
     }
     return terms;
 }
@@ -787,8 +790,8 @@ struct AdamArrays {
     float *m, *v;
 };
 
-XSG_DEV AdamTerms adam_terms(const StepTerms& now, const AdamScalars& s, float lr, float keep) {
-    return AdamTerms{s.beta2, s.one_minus_beta1, s.one_minus_beta2, s.eps, now.c, lr * now.over1, now.root, keep};
+XSG_DEV AdamTerms adam_terms(const StepTerms& now, const AdamScalars& s, double lr, float keep) {
+    return AdamTerms{s.beta2, s.one_minus_beta1, s.one_minus_beta2, s.eps, now.c, (float)(lr * now.over1), now.root, keep};
 }
 XSG_DEV AdamArrays adam_arrays(const AdamEntry& e, int64_t base) {
     return AdamArrays{at(e.param, base, e.pdtype), at(e.gradient, base, e.gdtype), e.avg + base, e.sq + base};
@@ -956,12 +959,13 @@ __global__ __launch_bounds__(kSmallBlock) void small_kernel(InlineList<E> list, 
                                                             float* __restrict__ each) {
     __shared__ double part[kSmallChunks];
     __shared__ StepTerms shared;
-    __shared__ float corrections[2];
+    __shared__ double over1;
+    __shared__ float root;
     const int wave = threadIdx.x >> 6;
     const double count = OP == kSmallAdam ? (double)(*step + 1) : 0.0;   // before it may change
     if (OP == kSmallAdam && wave == kSmallBlock / 64 - 1) {
-        corrections[0] = (float)(-1.0 / expm1(count * rule.log_beta1));
-        corrections[1] = (float)(1.0 / sqrt(-expm1(count * rule.log_beta2)));
+        over1 = -1.0 / expm1(count * rule.log_beta1);
+        root = (float)(1.0 / sqrt(-expm1(count * rule.log_beta2)));
     }
     if (OP != kSmallAdam || rule.norm >= 0) {
         for (int b = wave; b < list.chunks; b += kSmallBlock / 64) {
@@ -994,7 +998,7 @@ __global__ __launch_bounds__(kSmallBlock) void small_kernel(InlineList<E> list, 
         each[t] = (float)acc.finish();
     }
     if (threadIdx.x < 64) {
-        StepTerms terms{1.0f, 1.0f, 1.0f, 1};
+        StepTerms terms{1.0, 1.0f, 1.0f, 1};
         if (OP != kSmallAdam || rule.norm >= 0) {
             Accum<NORM> acc;
             if (threadIdx.x < list.chunks) acc.join_value(part[threadIdx.x]);
@@ -1014,8 +1018,8 @@ __global__ __launch_bounds__(kSmallBlock) void small_kernel(InlineList<E> list, 
     __syncthreads();
     StepTerms now = shared;
     if (OP == kSmallAdam) {
-        now.over1 = corrections[0];
-        now.root = corrections[1];
+        now.over1 = over1;
+        now.root = root;
     }
     if (OP == kSmallClip ? now.c == 1.0f : !now.taken) return;
     for (int b = wave; b < list.chunks; b += kSmallBlock / 64) {
@@ -1107,8 +1111,8 @@ GradEntry entry_of(const xsg_grad_tensor& x) {
 }
 AdamEntry entry_of(const xsg_adam_tensor& x) {
     const RowDiv div = row_div(x.numel, x.mask, x.rows);
-    return AdamEntry{x.param, x.grad, x.exp_avg, x.exp_avg_sq, x.numel, x.numel ? x.mask : nullptr, div.row, div.magic,
-                     (float)x.lr, (float)(1.0 - x.lr * x.weight_decay), (uint8_t)div.shift, (uint8_t)x.param_dtype,
+    return AdamEntry{x.param, x.grad, x.exp_avg, x.exp_avg_sq, x.numel, x.numel ? x.mask : nullptr, x.lr, div.row, div.magic,
+                     (float)(1.0 - x.lr * x.weight_decay), (uint8_t)div.shift, (uint8_t)x.param_dtype,
                      (uint8_t)x.grad_dtype};
 }
 template <typename T> using EntryOf = decltype(entry_of(std::declval<const T&>()));
