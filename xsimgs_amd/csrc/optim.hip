@@ -27,7 +27,9 @@ constexpr int64_t kDenseChunks = 1024, kMaskedChunks = 2048;
 // memory, where few long ones write in as many places at once (an update of 236 M elements: 2048 chunks 1310 us,
 // 57618 chunks 1230, around the caches 1145).
 constexpr int64_t kWriteChunk = 4096;
-constexpr int64_t kMaskedFactor = 4;      // such chunks to one of a masked tensor, of which little is kept
+// Such chunks to one of a masked tensor, of which little is kept (1 M Gaussians with 14 % kept: one 148 us, two 119,
+// four and eight 114; 101 nodes with 40 %: one and two 148, four 151, eight 166).
+constexpr int64_t kMaskedFactor = 4;
 constexpr int64_t kMaxChunk = 1 << 26;    // offsets inside a chunk are 32-bit, in bytes
 constexpr int64_t kCacheBytes = (int64_t)256 << 20;   // of the last-level cache
 constexpr int64_t kMaxRow = 1 << 30;      // and so are rows under a mask
@@ -36,7 +38,8 @@ constexpr int64_t kMaxChunks = (1 << 24) - 1;   // a launch of one workgroup eac
 constexpr int64_t kFarChunks = 1 << 22;         // of long writing calls, beside a last short one of every tensor
 constexpr int kArgumentBytes = 3900;      // of a list, beside the other arguments in 4 KB
 
-// Division of n < 2^31 by the row length: (mulhi(n, magic) + n) >> shift
+// Division of n < 2^31 by the row length: (mulhi(n, magic) + n) >> shift, by the method of Granlund and Montgomery
+// ("Division by Invariant Integers using Multiplication", 1994)
 struct RowDiv {
     uint32_t row, magic;
     uint32_t shift;
@@ -890,8 +893,9 @@ XSG_DEV void rows_adam(const AdamArrays& a, const AdamTerms& s, uint32_t count, 
     }
 }
 
-// The update, bound by four reads and three writes of an element: 236 M float32 1060 us (6.2 TB/s), 1 M Gaussians
-// with 14 % kept 80 us (412 MB moved in sectors of 64 bytes, 5.1 TB/s).
+// The update, bound by four reads and three writes of an element: 236 M float32 1000 to 1080 us from card to card (6.6
+// to 6.1 TB/s), 1 M Gaussians with 14 % kept 77 to 80 us (412 MB moved in sectors of 64 bytes, 5.1 TB/s). Dense arrays
+// that are not aligned alike go one element at a time: 59 M with the parameters one element further 371 us, 288 aligned.
 // F32: every parameter and gradient is float32
 template <bool F32, bool STREAM, typename L>
 __global__ __launch_bounds__(kBlock) void adam_kernel(L list, AdamScalars s, StepSource source) {
@@ -1152,7 +1156,7 @@ template <typename T> int make_plan(const T* ts, int n, const char* who, bool no
         masked = masked || ts[i].mask;
     }
     p->stream = p->bytes_touched > kCacheBytes;
-    // a call that writes gains nothing from it (4 M Gaussians: clip 454 us either way, update 1249 and 1280)
+    // a call that writes loses by it (4 M Gaussians: clip 440 us, around the caches 446; update 1239 and 1271)
     p->stream_norm = !writes && grad_bytes > kCacheBytes;
     const int64_t target = masked ? kMaskedChunks : kDenseChunks;
     p->chunk = chunk_for(p->elements, target, writes && p->stream);
@@ -1264,7 +1268,6 @@ template <typename L> int launch_partials(const L& list, int norm, const Plan& p
     return xsg_launch_status("grad_norm");
 }
 
-// the norm (where the rule has one) and the step's terms, for the launch behind
 template <int OP, typename T> bool is_small(const T* ts, int n, const Plan& p) {
     if (p.table || p.chunks > kSmallChunks) return false;
     return (OP != kSmallAdam && p.chunks <= kOneRound) ||
@@ -1282,6 +1285,7 @@ int launch_small(const T* ts, int n, const Plan& p, const StepRule& rule, const 
     return xsg_launch_status("small list");
 }
 
+// the norm (where the rule has one) and the step's terms, for the launch behind
 template <typename L>
 int make_terms(const L& list, const StepRule& rule, const Plan& p, void* ws, int64_t* step, float* total, hipStream_t s,
                StepSource* source) {

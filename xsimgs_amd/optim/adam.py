@@ -1,7 +1,8 @@
 """Adam over many tensors in a few launches: decoupled weight decay, clipping by the global norm fused in (the
 factor stays on the GPU and the gradients are not rewritten), and the renderer's packed visibility mask, under
 which Gaussians out of view keep their parameters and moments. Moments are float32 whatever the parameter's
-type; the step counter lives on the GPU, so a step can be captured in a graph and replayed."""
+type; the step counter lives on the GPU, so a step can be captured in a graph and replayed (with the learning
+rates it was captured with, and not a first step, which makes moments and counter)."""
 import torch
 
 from .. import _C
@@ -45,8 +46,10 @@ _OPTIONS = ("betas", "eps", "max_norm", "norm_type", "skip_nonfinite")   # of a 
 class Adam(torch.optim.Optimizer):
     """Adam over ``adam_step_``. Groups carry their own ``lr`` and ``weight_decay``; betas, eps, ``max_norm``,
     ``norm_type`` and ``skip_nonfinite`` hold for the whole optimizer, whose tensors are one list with one norm
-    and one step counter (a parameter without a gradient sits a step out; bias correction goes by the
-    optimizer's count). ``grad_norm`` is the last step's norm before clipping, or None."""
+    and one step counter: a parameter without a gradient sits a step out, and bias correction goes by the
+    optimizer's count, not the parameter's as in torch.optim.Adam (one that joins late starts with corrections
+    near 1, so its first step is up to (1 - beta1) / sqrt(1 - beta2) rates long; an optimizer of its own starts
+    it as a new one). ``grad_norm`` is the last step's norm before clipping, or None."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-15, weight_decay: float = 0.0, *,
                  max_norm: float | None = None, norm_type: float = 2.0, skip_nonfinite: bool = False):
