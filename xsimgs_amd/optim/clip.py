@@ -4,8 +4,9 @@ of sizes (empty ones too) and strides; sums are held in 64 bits.
 
 ``masks``: None, one packed mask for every tensor, or a sequence with one (or None) per tensor. A packed mask
 (``packed_visibility_mask``, ``packed_mask_from_instances``: bit i % 32 of word i // 32) covers the rows of
-its tensor's first dimension and has the words that these need, no more; rows whose bit is 0 are neither read
-nor written, whatever they hold. (SH coefficients in the ``[3, K, N]`` layout go in as 3 K tensors, the rows of
+its tensor's first dimension and has the words that these need, no more (one word fits any 1 to 32 rows: below
+that a mask of other rows cannot be told); rows whose bit is 0 are neither read nor written, whatever they
+hold. (SH coefficients in the ``[3, K, N]`` layout go in as 3 K tensors, the rows of
 their ``view(3 * K, N)``, each under the mask.)"""
 import torch
 
