@@ -290,9 +290,13 @@ def _plain_norm(state):
     keep = torch.ones(b, pixels, 1, 1, dtype=torch.bool, device=DEV) if state["mask"] is None else state["mask"].view(b, pixels, 1, 1)
     n = torch.clamp(keep.sum(1, keepdim=True) * (c // g), min=1)
     grouped = torch.where(keep, x.reshape(b, pixels, g, c // g).float(), 0.0)
-    mean = grouped.sum((1, 3), keepdim=True) / n
+
+    def total(t, dims, keepdim=True):   # long sums in 64 bits
+        return t.sum(dims, keepdim=keepdim, dtype=torch.float64)
+
+    mean = (total(grouped, (1, 3)) / n).float()
     xh = torch.where(keep, grouped - mean, 0.0)
-    rstd = 1.0 / torch.sqrt(xh.square().sum((1, 3), keepdim=True) / n + EPS)
+    rstd = (1.0 / torch.sqrt(total(xh.square(), (1, 3)) / n + EPS)).float()
     xh = xh * rstd
     weight, bias = (state[k].detach().view(g, c // g) for k in ("weight", "bias"))
     y, slope = _act(xh * weight + bias, case["act"])
@@ -304,9 +308,10 @@ def _plain_norm(state):
     if not case.get("train"):
         return out
     dz = torch.where(keep, state["grad"].view(b, pixels, g, c // g).float() * slope, 0.0)
-    out["v_weight"], out["v_bias"] = (dz * xh).sum((0, 1)).view(c), dz.sum((0, 1)).view(c)
+    out["v_weight"], out["v_bias"] = (total(t, (0, 1), False).float().view(c) for t in (dz * xh, dz))
     dxh = dz * weight
-    dx = rstd * (dxh - dxh.sum((1, 3), keepdim=True) / n - xh * ((dxh * xh).sum((1, 3), keepdim=True) / n))
+    means = [(total(t, (1, 3)) / n).float() for t in (dxh, dxh * xh)]
+    dx = rstd * (dxh - means[0] - xh * means[1])
     out["v_x"] = torch.where(keep, dx, 0.0).to(x.dtype).view(x.shape)
     return out
 
