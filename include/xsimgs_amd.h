@@ -240,6 +240,72 @@ int xsg_activate_bwd(int64_t n, const float* scales, const float* opacities, con
                      const float* v_opacities, float* v_log_scales, float* v_opacity_logits,
                      xsg_stream_t stream);
 
+/* ------------------------------------------------- dropout and feature images
+ * Extensions, no reference counterpart. Draws come from a counter-based generator, so no mask is stored: value e
+ * of a call is a function of e, the seed and the stream. It is dropped where its 32 bits are below
+ * T = round(p 2^32); the upper 16 of them are half e % 2 (the lower half first) of word e % 8 / 2 of
+ * Philox4x32-10 with the seed's two words (lower first) as key and the counter (lower and upper word of e / 8,
+ * stream, 0), the lower 16 the same half and word under the counter (.., .., stream, 1). What is kept is
+ * multiplied by 1 / (1 - T / 2^32). XSG_DTYPE_* as below. */
+typedef struct {
+    double p;                  /* in [0, 1] */
+    uint64_t seed;
+    const uint64_t* seed_at;   /* NULL, or the seed's place on the device, read by the kernels */
+    uint32_t stream;
+} xsg_drop_desc;
+
+/* out = x (kept) / (1 - T / 2^32), 0 where dropped (whatever x holds there); draw i covers the `shared`
+ * consecutive elements from i * shared on (1: each element has its own; numel is a multiple of it). The backward
+ * is the same call on the gradient. out may be x. Rows of eight elements and more that are dropped are not read (but
+ * for up to seven elements beside a kept row). */
+int xsg_dropout(const xsg_drop_desc* drop, int dtype, int64_t numel, int64_t shared, const void* x, void* out,
+                xsg_stream_t stream);
+
+/* The draws themselves as a packed mask of (n + 31) / 32 words: bit i % 32 of word i / 32 set where value i is
+ * kept, zeros past n. */
+int xsg_drop_mask(const xsg_drop_desc* drop, int64_t n, uint32_t* out, xsg_stream_t stream);
+
+/* xsg_activate_fwd / _bwd with a share of the Gaussians dropped: opacities are sigmoid(opacity_logits) times draw
+ * i's factor. The backward takes the logits in place of the opacities. */
+int xsg_activate_drop_fwd(const xsg_drop_desc* drop, int64_t n, const float* log_scales, const float* opacity_logits,
+                          float* scales, float* opacities, xsg_stream_t stream);
+int xsg_activate_drop_bwd(const xsg_drop_desc* drop, int64_t n, const float* scales, const float* opacity_logits,
+                          const float* v_scales, const float* v_opacities, float* v_log_scales,
+                          float* v_opacity_logits, xsg_stream_t stream);
+
+#define XSG_ACT_NONE 0
+#define XSG_ACT_RELU 1
+#define XSG_ACT_SILU 2
+#define XSG_ACT_GELU 3     /* z Phi(z), by the error function */
+
+#define XSG_NORM_MAX_CHANNELS 4096
+
+/* Group norm of feature images, channels last, with an activation and dropout behind it: over each sample and
+ * each group of channels / groups consecutive channels, with mean and (biased) variance over the pixels in the
+ * mask, y = drop(act((x - mean) / sqrt(variance + eps) weight + bias)). Pixels out of the mask are not read; y
+ * and v_x are 0 there. */
+typedef struct {
+    int dtype;                        /* of x, y and their gradients */
+    int64_t batch, pixels;
+    int channels, groups;
+    const void* x;                    /* [batch, pixels, channels]; channels lie side by side */
+    int64_t batch_stride, pixel_stride;   /* of x, in elements; all other arrays are dense */
+    const void* weight;               /* [channels] or NULL (1) */
+    const void* bias;                 /* [channels] or NULL (0) */
+    int weight_dtype, bias_dtype;     /* XSG_DTYPE_F32 or x's */
+    const uint8_t* mask;              /* [batch, pixels], 0: out; NULL: every pixel */
+    int act;                          /* XSG_ACT_* */
+    double eps;
+    xsg_drop_desc drop;               /* value e is element e of the dense y */
+} xsg_norm_desc;
+
+/* stats [batch, groups, 4]: mean, 1 / sqrt(variance + eps), 1 / count (0 of none), 0; the backward takes them, and
+ * the same desc. weight and bias gradients in float32, either may be NULL, as may v_x. */
+size_t xsg_group_norm_act_workspace_bytes(const xsg_norm_desc* d, int backward);
+int xsg_group_norm_act_fwd(const xsg_norm_desc* d, void* y, float* stats, void* workspace, xsg_stream_t stream);
+int xsg_group_norm_act_bwd(const xsg_norm_desc* d, const float* stats, const void* v_y, void* v_x, float* v_weight,
+                           float* v_bias, void* workspace, xsg_stream_t stream);
+
 /* ---------------------------------------------------------- training step
  * Extensions, no reference counterpart: what a training step does behind the frame's backward. Every
  * call takes a list of tensors (an array on the host, read before the call returns); the lists travel in

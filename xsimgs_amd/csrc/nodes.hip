@@ -2,6 +2,7 @@
 // mask_radii_packed / SH, and the rigid per-instance copy of Gaussians into the frame's buffers
 // (reference csrc/nodes/gs_masking.cu, csrc/nodes/container.cu). One thread per element / Gaussian.
 #include "xsg_common.h"
+#include "xsg_random.h"
 
 namespace {
 
@@ -284,6 +285,61 @@ __global__ __launch_bounds__(kBlock) void activate_bwd_kernel(int64_t n3, int64_
     }
 }
 
+// The same with a share of the Gaussians dropped: a thread takes four scales, or the eight opacities of one block of
+// draws. The backward evaluates the sigmoid again: the dropped opacities do not tell it.
+template <typename F>
+XSG_DEV void act_drop_chunk(bool vec, const DropArgs& drop, int64_t block, int64_t n, const float* __restrict__ x,
+                            const float* __restrict__ v, float* __restrict__ out, F f) {
+    const int64_t i0 = 8 * block;
+    const uint32_t keep = Draws(drop).keep8((uint64_t)block);
+    if (vec && i0 + 8 <= n) {
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(x + i0 + h);
+            const float4 g = v ? *reinterpret_cast<const float4*>(v + i0 + h) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(out + i0 + h) =
+                make_float4(keep >> h & 1 ? f(a.x, g.x) : 0.0f, keep >> (h + 1) & 1 ? f(a.y, g.y) : 0.0f,
+                            keep >> (h + 2) & 1 ? f(a.z, g.z) : 0.0f, keep >> (h + 3) & 1 ? f(a.w, g.w) : 0.0f);
+        }
+    } else {
+        for (int j = 0; j < 8; ++j)
+            if (i0 + j < n) out[i0 + j] = keep >> j & 1 ? f(x[i0 + j], v ? v[i0 + j] : 0.0f) : 0.0f;
+    }
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(kBlock) void activate_drop_fwd_kernel(int64_t n3, int64_t n, DropArgs drop,
+                                                                   const float* __restrict__ log_scales,
+                                                                   const float* __restrict__ logits,
+                                                                   float* __restrict__ scales,
+                                                                   float* __restrict__ opacities) {
+    const int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x, q3 = (n3 + 3) >> 2;
+    if (q < q3)
+        act_chunk<VEC>(log_scales, scales, 4 * q, n3, act_exp);
+    else if (8 * (q - q3) < n)
+        act_drop_chunk(VEC, drop, q - q3, n, logits, nullptr, opacities,
+                       [&](float a, float) { return act_sigmoid(a) * drop.factor; });
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(kBlock) void activate_drop_bwd_kernel(int64_t n3, int64_t n, DropArgs drop,
+                                                                   const float* __restrict__ scales,
+                                                                   const float* __restrict__ logits,
+                                                                   const float* __restrict__ v_scales,
+                                                                   const float* __restrict__ v_opacities,
+                                                                   float* __restrict__ v_log_scales,
+                                                                   float* __restrict__ v_logits) {
+    const int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x, q3 = (n3 + 3) >> 2;
+    if (q < q3) {
+        if (v_scales) act_grad_chunk<VEC>(v_scales, scales, v_log_scales, 4 * q, n3, [](float a, float b) { return a * b; });
+    } else if (v_opacities && 8 * (q - q3) < n) {
+        act_drop_chunk(VEC, drop, q - q3, n, logits, v_opacities, v_logits, [&](float a, float g) {
+            const float s = act_sigmoid(a);
+            return g * drop.factor * ((1.0f - s) * s);
+        });
+    }
+}
+
 }  // namespace
 
 extern "C" int xsg_packed_mask_from_instances(int64_t n, const int32_t* instance_ids, const uint8_t* instance_mask,
@@ -409,5 +465,45 @@ extern "C" int xsg_activate_bwd(int64_t n, const float* scales, const float* opa
         activate_bwd_kernel<false><<<grid, kBlock, 0, s>>>(3 * n, n, scales, opacities, v_scales, v_opacities,
                                                            v_log_scales, v_opacity_logits);
     XSG_TRY_LAUNCH("activate_bwd");
+    return XSG_OK;
+}
+
+extern "C" int xsg_activate_drop_fwd(const xsg_drop_desc* drop, int64_t n, const float* log_scales,
+                                     const float* opacity_logits, float* scales, float* opacities,
+                                     xsg_stream_t stream) {
+    DropArgs d;
+    if (const int rc = drop_args(drop, d, "activate_drop_fwd")) return rc;
+    if (n < 0) return xsg_fail(XSG_ERR_INVALID, "activate_drop_fwd: negative size");
+    if (n == 0) return XSG_OK;
+    if (!log_scales || !opacity_logits || !scales || !opacities)
+        return xsg_fail(XSG_ERR_INVALID, "activate_drop_fwd: null tensor");
+    const unsigned grid = xsg_blocks((3 * n + 3) / 4 + (n + 7) / 8, kBlock);
+    const hipStream_t s = (hipStream_t)stream;
+    if (aligned16({log_scales, opacity_logits, scales, opacities}))
+        activate_drop_fwd_kernel<true><<<grid, kBlock, 0, s>>>(3 * n, n, d, log_scales, opacity_logits, scales, opacities);
+    else
+        activate_drop_fwd_kernel<false><<<grid, kBlock, 0, s>>>(3 * n, n, d, log_scales, opacity_logits, scales, opacities);
+    XSG_TRY_LAUNCH("activate_drop_fwd");
+    return XSG_OK;
+}
+
+extern "C" int xsg_activate_drop_bwd(const xsg_drop_desc* drop, int64_t n, const float* scales,
+                                     const float* opacity_logits, const float* v_scales, const float* v_opacities,
+                                     float* v_log_scales, float* v_opacity_logits, xsg_stream_t stream) {
+    DropArgs d;
+    if (const int rc = drop_args(drop, d, "activate_drop_bwd")) return rc;
+    if (n < 0) return xsg_fail(XSG_ERR_INVALID, "activate_drop_bwd: negative size");
+    if (n == 0 || (!v_scales && !v_opacities)) return XSG_OK;
+    if ((v_scales && (!scales || !v_log_scales)) || (v_opacities && (!opacity_logits || !v_opacity_logits)))
+        return xsg_fail(XSG_ERR_INVALID, "activate_drop_bwd: null tensor");
+    const unsigned grid = xsg_blocks((3 * n + 3) / 4 + (n + 7) / 8, kBlock);
+    const hipStream_t s = (hipStream_t)stream;
+    if (aligned16({scales, opacity_logits, v_scales, v_opacities, v_log_scales, v_opacity_logits}))
+        activate_drop_bwd_kernel<true><<<grid, kBlock, 0, s>>>(3 * n, n, d, scales, opacity_logits, v_scales, v_opacities,
+                                                               v_log_scales, v_opacity_logits);
+    else
+        activate_drop_bwd_kernel<false><<<grid, kBlock, 0, s>>>(3 * n, n, d, scales, opacity_logits, v_scales, v_opacities,
+                                                                v_log_scales, v_opacity_logits);
+    XSG_TRY_LAUNCH("activate_drop_bwd");
     return XSG_OK;
 }

@@ -1060,6 +1060,172 @@ std::tuple<Tensor, Tensor> activate_bwd(const Tensor& scales, const Tensor& opac
     return {v_log_scales, v_logits};
 }
 
+// ------------------------------------------------------------------ dropout and feature images (extensions)
+int dtype_code(const Tensor& t, const char* name) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return XSG_DTYPE_F32;
+        case at::kBFloat16: return XSG_DTYPE_BF16;
+        case at::kHalf: return XSG_DTYPE_F16;
+        default: TORCH_CHECK(false, name, " must be a float32, bfloat16 or float16 tensor, not ", t.scalar_type());
+    }
+}
+
+xsg_drop_desc drop_desc(double p, int64_t seed, const OptT& seed_at, int64_t stream, const c10::Device& device) {
+    TORCH_CHECK(p >= 0.0 && p <= 1.0, "a drop probability lies in [0, 1], not ", p);
+    TORCH_CHECK(stream >= 0 && stream <= 0x7fffffff, "stream must lie in [0, 2^31), not ", stream);
+    TORCH_CHECK(!seed_at.has_value() || (seed_at->scalar_type() == at::kLong && seed_at->numel() == 1),
+                "a seed tensor holds one int64");
+    TORCH_CHECK(!seed_at.has_value() || seed_at->device() == device, "the seed tensor must be on ", device);
+    return xsg_drop_desc{p, (uint64_t)seed,
+                         seed_at.has_value() ? (const uint64_t*)seed_at->data_ptr<int64_t>() : nullptr, (uint32_t)stream};
+}
+
+Tensor dropout(const Tensor& x, double p, int64_t seed, const OptT& seed_at, int64_t stream, int64_t shared) {
+    TORCH_CHECK(x.is_contiguous(), "x must be contiguous");
+    const int dt = dtype_code(x, "x");
+    const xsg_stream_t s = stream_of(x);
+    const auto d = drop_desc(p, seed, seed_at, stream, x.device());
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    Tensor out = at::empty(x.sizes(), x.options());
+    if (x.numel() == 0) return out;
+    check_rc(xsg_dropout(&d, dt, x.numel(), shared, x.data_ptr(), out.data_ptr(), s));
+    return out;
+}
+
+Tensor drop_mask(int64_t n, double p, int64_t seed, const OptT& seed_at, int64_t stream, const c10::Device& device) {
+    TORCH_CHECK(n >= 0, "n must not be negative");
+    TORCH_CHECK(device.is_cuda(), "xsimgs_amd ops take GPU tensors (got the device ", device, ")");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
+    Tensor out = at::empty({(n + 31) / 32}, at::TensorOptions().device(device).dtype(at::kUInt32));
+    const auto d = drop_desc(p, seed, seed_at, stream, out.device());
+    check_rc(xsg_drop_mask(&d, n, (uint32_t*)out.data_ptr(), stream_of(out)));
+    return out;
+}
+
+std::tuple<Tensor, Tensor> activate_drop_fwd(const Tensor& log_scales, const Tensor& opacity_logits, double p,
+                                             int64_t seed, const OptT& seed_at, int64_t stream) {
+    check_same_device({log_scales, opacity_logits});
+    all_contiguous({log_scales, opacity_logits});
+    check_f32(log_scales, "log_scales");
+    check_f32(opacity_logits, "opacity_logits");
+    const int64_t n = opacity_logits.numel();
+    TORCH_CHECK(log_scales.numel() == 3 * n, "log_scales must hold three values per opacity logit");
+    const xsg_stream_t s = stream_of(log_scales);
+    const auto d = drop_desc(p, seed, seed_at, stream, log_scales.device());
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(log_scales.device());
+    Tensor scales = at::empty_like(log_scales), opacities = at::empty_like(opacity_logits);
+    check_rc(xsg_activate_drop_fwd(&d, n, fptr(log_scales), fptr(opacity_logits), scales.data_ptr<float>(),
+                                   opacities.data_ptr<float>(), s));
+    return {scales, opacities};
+}
+
+std::tuple<Tensor, Tensor> activate_drop_bwd(const Tensor& scales, const Tensor& opacity_logits, const OptT& v_scales,
+                                             const OptT& v_opacities, double p, int64_t seed, const OptT& seed_at,
+                                             int64_t stream) {
+    std::vector<Tensor> ts{scales, opacity_logits};
+    for (const OptT* o : {&v_scales, &v_opacities})
+        if (o->has_value()) ts.push_back(**o);
+    check_same_device(ts);
+    all_contiguous(ts);
+    for (const auto& t : ts) check_f32(t, "activation tensors");
+    const int64_t n = opacity_logits.numel();
+    TORCH_CHECK(scales.numel() == 3 * n, "scales must hold three values per opacity logit");
+    TORCH_CHECK(!v_scales.has_value() || v_scales->numel() == 3 * n, "v_scales must match scales");
+    TORCH_CHECK(!v_opacities.has_value() || v_opacities->numel() == n, "v_opacities must match opacities");
+    const xsg_stream_t s = stream_of(scales);
+    const auto d = drop_desc(p, seed, seed_at, stream, scales.device());
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scales.device());
+    Tensor v_log_scales, v_logits;
+    if (v_scales.has_value()) v_log_scales = at::empty_like(scales);
+    if (v_opacities.has_value()) v_logits = at::empty_like(opacity_logits);
+    check_rc(xsg_activate_drop_bwd(&d, n, fptr(scales), fptr(opacity_logits), fptr(v_scales), fptr(v_opacities),
+                                   v_scales.has_value() ? v_log_scales.data_ptr<float>() : nullptr,
+                                   v_opacities.has_value() ? v_logits.data_ptr<float>() : nullptr, s));
+    return {v_log_scales, v_logits};
+}
+
+// The description of a call and what it points to (a strided x whose pixels do not follow each other at one
+// distance, and a strided mask or parameter, are copied).
+struct NormCall {
+    Tensor x, weight, bias, mask;
+    xsg_norm_desc d{};
+
+    NormCall(const Tensor& input, int64_t groups, const OptT& w, const OptT& b, int64_t act, double eps, const OptT& m,
+             double p, int64_t seed, const OptT& seed_at, int64_t stream) {
+        TORCH_CHECK(input.is_cuda(), "xsimgs_amd ops take GPU tensors (got a tensor on ", input.device(), ")");
+        TORCH_CHECK(input.dim() >= 2, "x must be [batch, ..., channels]");
+        d.dtype = dtype_code(input, "x");
+        const int64_t channels = input.size(-1);
+        TORCH_CHECK(channels >= 1 && channels <= XSG_NORM_MAX_CHANNELS, "x must have 1 to ", XSG_NORM_MAX_CHANNELS,
+                    " channels, not ", channels);
+        TORCH_CHECK(groups >= 1 && channels % groups == 0, groups, " groups do not divide ", channels, " channels");
+        const auto param = [&](const OptT& t, const char* name, Tensor& keep, int& code) -> const void* {
+            if (!t.has_value()) return nullptr;
+            TORCH_CHECK(t->dim() == 1 && t->size(0) == channels, name, " must hold one value per channel");
+            TORCH_CHECK(t->device() == input.device(), "All tensors must be on the same device");
+            TORCH_CHECK(t->scalar_type() == at::kFloat || t->scalar_type() == input.scalar_type(), name,
+                        " must be float32 or of x's type");
+            code = dtype_code(*t, name);
+            keep = t->contiguous();
+            return keep.data_ptr();
+        };
+        const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(input.device());
+        d.weight = param(w, "weight", weight, d.weight_dtype);
+        d.bias = param(b, "bias", bias, d.bias_dtype);
+        if (m.has_value()) {
+            TORCH_CHECK(m->scalar_type() == at::kBool || m->scalar_type() == at::kByte, "mask must be a bool / uint8 tensor");
+            TORCH_CHECK(m->sizes() == input.sizes().slice(0, input.dim() - 1), "mask must have x's sizes without the channels");
+            TORCH_CHECK(m->device() == input.device(), "All tensors must be on the same device");
+            mask = m->contiguous();
+            d.mask = (const uint8_t*)mask.data_ptr();
+        }
+        x = input.dim() == 2 ? input.unsqueeze(1) : input.dim() == 3 ? input : input.flatten(1, -2);
+        if (channels > 1 && x.stride(2) != 1) x = x.contiguous();
+        d.batch = x.size(0); d.pixels = x.size(1);
+        d.channels = (int)channels; d.groups = (int)groups;
+        d.x = x.data_ptr();
+        d.batch_stride = d.batch > 1 ? x.stride(0) : 0;
+        d.pixel_stride = d.pixels > 1 ? x.stride(1) : 0;
+        d.act = (int)act;
+        d.eps = eps;
+        d.drop = drop_desc(p, seed, seed_at, stream, input.device());
+    }
+};
+
+std::tuple<Tensor, Tensor> group_norm_act_fwd(const Tensor& x, int64_t groups, const OptT& weight, const OptT& bias,
+                                              int64_t act, double eps, const OptT& mask, double p, int64_t seed,
+                                              const OptT& seed_at, int64_t stream) {
+    const NormCall c(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    Tensor y = at::empty(x.sizes(), x.options());
+    Tensor stats = at::empty({c.d.batch, groups, 4}, x.options().dtype(at::kFloat));
+    const Tensor ws = workspace(x, xsg_group_norm_act_workspace_bytes(&c.d, 0));
+    check_rc(xsg_group_norm_act_fwd(&c.d, y.data_ptr(), stats.data_ptr<float>(), ws.data_ptr(), stream_of(x)));
+    return {y, stats};
+}
+
+std::tuple<OptT, OptT, OptT> group_norm_act_bwd(const Tensor& v_y, const Tensor& stats, const Tensor& x, int64_t groups,
+                                                const OptT& weight, const OptT& bias, int64_t act, double eps,
+                                                const OptT& mask, double p, int64_t seed, const OptT& seed_at,
+                                                int64_t stream, bool need_x, bool need_weight, bool need_bias) {
+    const NormCall c(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream);
+    check_same_device({x, v_y, stats});
+    all_contiguous({v_y, stats});
+    TORCH_CHECK(v_y.sizes() == x.sizes() && v_y.scalar_type() == x.scalar_type(), "v_y must have x's sizes and type");
+    check_f32(stats, "stats");
+    TORCH_CHECK(stats.numel() == c.d.batch * groups * 4, "stats must be the forward's");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    OptT v_x, v_weight, v_bias;
+    if (need_x) v_x = at::empty(x.sizes(), x.options());
+    if (need_weight) v_weight = at::empty({x.size(-1)}, x.options().dtype(at::kFloat));
+    if (need_bias) v_bias = at::empty({x.size(-1)}, x.options().dtype(at::kFloat));
+    const Tensor ws = workspace(x, xsg_group_norm_act_workspace_bytes(&c.d, 1));
+    check_rc(xsg_group_norm_act_bwd(&c.d, stats.data_ptr<float>(), v_y.data_ptr(), v_x ? v_x->data_ptr() : nullptr,
+                                    v_weight ? v_weight->data_ptr<float>() : nullptr,
+                                    v_bias ? v_bias->data_ptr<float>() : nullptr, ws.data_ptr(), stream_of(x)));
+    return {v_x, v_weight, v_bias};
+}
+
 Tensor packed_mask_from_instances(const Tensor& instance_ids, const Tensor& instance_mask) {
     check_same_device({instance_ids, instance_mask});
     all_contiguous({instance_ids, instance_mask});
@@ -1680,6 +1846,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adam_step_", &adam_step_, py::arg("params"), py::arg("grads"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"),
           py::arg("step"), py::arg("lr"), py::arg("weight_decay"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
           py::arg("max_norm"), py::arg("norm_type"), py::arg("skip_nonfinite"), py::arg("masks"));
+    const auto none = py::none();
+    m.def("dropout", &dropout, py::arg("x"), py::arg("p"), py::arg("seed"), py::arg("seed_at") = none, py::arg("stream") = 0,
+          py::arg("shared") = 1);
+    m.def("drop_mask", &drop_mask, py::arg("n"), py::arg("p"), py::arg("seed"), py::arg("seed_at"), py::arg("stream"),
+          py::arg("device"));
+    m.def("activate_drop_fwd", &activate_drop_fwd, py::arg("log_scales"), py::arg("opacity_logits"), py::arg("p"),
+          py::arg("seed"), py::arg("seed_at") = none, py::arg("stream") = 0);
+    m.def("activate_drop_bwd", &activate_drop_bwd, py::arg("scales"), py::arg("opacity_logits"), py::arg("v_scales"),
+          py::arg("v_opacities"), py::arg("p"), py::arg("seed"), py::arg("seed_at") = none, py::arg("stream") = 0);
+    m.def("group_norm_act_fwd", &group_norm_act_fwd, py::arg("x"), py::arg("groups"), py::arg("weight"), py::arg("bias"),
+          py::arg("act"), py::arg("eps"), py::arg("mask"), py::arg("p"), py::arg("seed"), py::arg("seed_at"),
+          py::arg("stream"));
+    m.def("group_norm_act_bwd", &group_norm_act_bwd, py::arg("v_y"), py::arg("stats"), py::arg("x"), py::arg("groups"),
+          py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("eps"), py::arg("mask"), py::arg("p"),
+          py::arg("seed"), py::arg("seed_at"), py::arg("stream"), py::arg("need_x"), py::arg("need_weight"),
+          py::arg("need_bias"));
     m.def("activate_fwd", &activate_fwd, py::arg("log_scales"), py::arg("opacity_logits"));
     m.def("activate_bwd", &activate_bwd, py::arg("scales"), py::arg("opacities"), py::arg("v_scales"),
           py::arg("v_opacities"));

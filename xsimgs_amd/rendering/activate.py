@@ -6,6 +6,7 @@ torch's, bit for bit (the same float expressions), in one launch forward and one
 import torch
 
 from .. import _C
+from .drop import seed_arguments
 
 
 class _Activate(torch.autograd.Function):
@@ -29,7 +30,35 @@ class _Activate(torch.autograd.Function):
                             None if v_opacities is None else v_opacities.contiguous())
 
 
-def activate_gaussians(log_scales: torch.Tensor, opacity_logits: torch.Tensor):
+class _ActivateDrop(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, log_scales, opacity_logits, seed_at, p, seed, stream):
+        ctx.set_materialize_grads(False)
+        ctx.args = p, seed, stream
+        opacity_logits = opacity_logits.contiguous()
+        scales, opacities = _C.activate_drop_fwd(log_scales.contiguous(), opacity_logits, p, seed, seed_at, stream)
+        ctx.save_for_backward(scales, opacity_logits, seed_at)
+        return scales, opacities
+
+    @staticmethod
+    def backward(ctx, v_scales, v_opacities):
+        scales, opacity_logits, seed_at = ctx.saved_tensors
+        p, seed, stream = ctx.args
+        v_scales = v_scales.contiguous() if v_scales is not None and ctx.needs_input_grad[0] else None
+        v_opacities = v_opacities.contiguous() if v_opacities is not None and ctx.needs_input_grad[1] else None
+        grads = (None, None)
+        if v_scales is not None or v_opacities is not None:
+            grads = _C.activate_drop_bwd(scales, opacity_logits, v_scales, v_opacities, p, seed, seed_at, stream)
+        return (*grads, None, None, None, None)
+
+
+def activate_gaussians(log_scales: torch.Tensor, opacity_logits: torch.Tensor, *, drop: float = 0.0, seed=0,
+                       stream: int = 0):
     """(exp(log_scales), sigmoid(opacity_logits)); log_scales holds three values per opacity logit
-    ([N, 3] and [N] or [N, 1]), float32 on the GPU."""
-    return _Activate.apply(log_scales, opacity_logits)
+    ([N, 3] and [N] or [N, 1]), float32 on the GPU. With ``drop`` each Gaussian's opacity is 0 with that
+    probability and the others' are divided by the share kept (they may pass 1, where the compositor's alpha is
+    clamped all the same); ``drop_mask`` of the same drop, seed and stream tells which are kept."""
+    seed, seed_at = seed_arguments(seed)
+    if drop == 0:
+        return _Activate.apply(log_scales, opacity_logits)
+    return _ActivateDrop.apply(log_scales, opacity_logits, seed_at, float(drop), seed, stream)

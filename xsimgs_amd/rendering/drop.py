@@ -1,0 +1,64 @@
+"""Dropout whose draws come from a counter-based generator: a draw is a function of its number, the seed and the
+stream, so the backward draws again and no mask is stored. An extension of this build.
+
+``seed``: an int in [0, 2^63), another for each step; or an int64 tensor of one value on the GPU, which the kernels
+read (a captured graph then draws anew on each replay if the value is changed in between; not between a forward
+and its backward, which autograd refuses). ``stream``: a number in [0, 2^31), another for each place that
+draws under one seed. Probabilities count in steps of 2^-32; what is kept is divided by the share that is kept."""
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _C
+
+
+def seed_arguments(seed):
+    """(the number, the tensor or None)"""
+    if isinstance(seed, torch.Tensor):
+        return 0, seed
+    if isinstance(seed, bool) or not isinstance(seed, int) or not 0 <= seed < 1 << 63:
+        raise ValueError(f"seed must be an int in [0, 2^63) or an int64 tensor of one value, not {seed!r}")
+    return seed, None
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, seed_at, p, seed, stream, shared):
+        ctx.args = p, seed, stream, shared
+        ctx.save_for_backward(seed_at)
+        return _C.dropout(x.contiguous(), p, seed, seed_at, stream, shared)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, v_y):
+        p, seed, stream, shared = ctx.args
+        return _C.dropout(v_y.contiguous(), p, seed, ctx.saved_tensors[0], stream, shared), None, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed, *, stream: int = 0, shared: int = 0) -> torch.Tensor:
+    """``x`` (float32, bfloat16 or float16 on the GPU) with elements zeroed with probability ``p`` and the others
+    divided by the share kept; zeros whatever ``x`` holds there. ``shared``: so many trailing dimensions share one
+    draw (1 drops whole rows of the last dimension; 2 a Gaussian's SH coefficients of ``[N, K, 3]``). A ``p`` of 0
+    gives ``x`` itself."""
+    if not 0 <= shared <= x.dim():
+        raise ValueError(f"shared must lie in [0, {x.dim()}] for a tensor of {x.dim()} dimensions, not {shared}")
+    row = 1
+    for n in x.shape[x.dim() - shared:]:
+        row *= n
+    seed, seed_at = seed_arguments(seed)
+    if p == 0:
+        return x
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Dropout.apply(x, seed_at, float(p), seed, stream, max(row, 1))
+    return _C.dropout(x.contiguous(), float(p), seed, seed_at, stream, max(row, 1))
+
+
+def drop_mask(n: int, drop: float, seed, *, stream: int = 0, device=None) -> torch.Tensor:
+    """Which of ``n`` Gaussians ``activate_gaussians(..., drop, seed, stream)`` keeps, as a packed mask (bit i % 32 of
+    word i // 32), as ``ut_gs_tiling``'s ``packed_particle_mask`` and the optimizer's ``masks`` take it."""
+    seed, seed_at = seed_arguments(seed)
+    if device is None:
+        device = seed_at.device if seed_at is not None else "cuda"
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return _C.drop_mask(n, float(drop), seed, seed_at, stream, device)

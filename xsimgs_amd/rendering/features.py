@@ -1,0 +1,75 @@
+"""Group norm with an activation and dropout over rendered feature images, channels last as the compositor writes
+them: what a network that decodes them starts each of its blocks with. An extension of this build."""
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _C
+from .drop import seed_arguments
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, mask, seed_at, groups, act, eps, p, seed, stream):
+        y, stats = _C.group_norm_act_fwd(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream)
+        ctx.args = groups, act, eps, p, seed, stream
+        ctx.save_for_backward(x, weight, bias, mask, seed_at, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, v_y):
+        x, weight, bias, mask, seed_at, stats = ctx.saved_tensors
+        groups, act, eps, p, seed, stream = ctx.args
+        v_x, v_weight, v_bias = _C.group_norm_act_bwd(
+            v_y.contiguous(), stats, x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream,
+            *ctx.needs_input_grad[:3])
+        return (v_x, None if v_weight is None else v_weight.to(weight.dtype),
+                None if v_bias is None else v_bias.to(bias.dtype)) + (None,) * 8
+
+
+def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, *, act: str = "silu", eps: float = 1e-5,
+                   mask=None, drop: float = 0.0, seed=0, stream: int = 0) -> torch.Tensor:
+    """``drop(act((x - mean) / sqrt(variance + eps) * weight + bias))`` over each sample and each group of
+    consecutive channels of ``x`` ``[batch, ..., channels]`` (float32, bfloat16 or float16 on the GPU; up to 4096
+    channels, which ``groups`` divides; one camera's ``[H, W, ch]`` goes in as ``x[None]``). Sums are held in 32 and 64
+    bits, the result is rounded once.
+
+    ``weight``, ``bias``: one value per channel, float32 or of x's type, or None. ``act``: none, relu, silu or gelu (by
+    the error function). ``mask``: ``[batch, ...]``, bool; pixels out of it are not read, do not count, and give 0 and
+    no gradient (a sample without any gives zeros). ``drop``, ``seed``, ``stream``: the draws of ``dropout`` on the result."""
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act must be one of {', '.join(ACTIVATIONS)}, not {act!r}")
+    seed, seed_at = seed_arguments(seed)
+    args = int(groups), ACTIVATIONS[act], float(eps), float(drop), seed, stream
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _GroupNormAct.apply(x, weight, bias, mask, seed_at, *args)
+    groups, act, eps, p, seed, stream = args
+    return _C.group_norm_act_fwd(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream)[0]
+
+
+class FeatureNorm(torch.nn.Module):
+    """``group_norm_act`` with its weight and bias, for ``frame.prepare(..., head=)`` and networks behind the
+    compositor. Dropout acts in training mode only and takes the call's ``seed``; ``stream`` tells modules apart
+    that share one."""
+
+    def __init__(self, groups: int, channels: int, act: str = "silu", eps: float = 1e-5, drop: float = 0.0, *,
+                 stream: int = 0, device=None, dtype=None):
+        super().__init__()
+        if act not in ACTIVATIONS or groups < 1 or channels % groups or not 0.0 <= drop <= 1.0:
+            raise ValueError(f"FeatureNorm takes an activation ({', '.join(ACTIVATIONS)}), groups that divide the channels "
+                             "and a drop probability in [0, 1]")
+        self.groups, self.act, self.eps, self.drop, self.stream = groups, act, eps, drop, stream
+        self.weight = torch.nn.Parameter(torch.ones(channels, device=device, dtype=dtype))
+        self.bias = torch.nn.Parameter(torch.zeros(channels, device=device, dtype=dtype))
+
+    def forward(self, x, mask=None, seed=None):
+        drop = self.drop if self.training else 0.0
+        if drop > 0.0 and seed is None:
+            raise ValueError("a FeatureNorm that drops takes another seed in each training step")
+        return group_norm_act(x, self.groups, self.weight, self.bias, act=self.act, eps=self.eps, mask=mask, drop=drop,
+                              seed=0 if seed is None else seed, stream=self.stream)
+
+    def extra_repr(self):
+        return f"{self.groups}, {self.weight.numel()}, act={self.act}, eps={self.eps}, drop={self.drop}"
