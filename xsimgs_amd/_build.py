@@ -27,7 +27,7 @@ ARCH = os.environ.get("XSG_OFFLOAD_ARCH", "gfx950")
 HIP_SOURCES = ["eval3d_bwd_g7.hip", "eval3d_bwd_g6.hip", "eval3d_bwd_g5.hip", "eval3d_bwd_g4.hip",
                "eval3d_bwd_g3.hip", "eval3d_bwd_g2.hip", "eval3d_bwd_g1.hip", "eval3d_bwd_g0.hip",
                "eval3d_fwd.hip", "tiling.hip", "camera.hip", "sh.hip", "capi.hip", "eval3d_bwd.hip",
-               "eval3d_capi.hip", "nodes.hip", "optim.hip", "calibrate.hip", "norm_bwd.hip",
+               "eval3d_capi.hip", "nodes.hip", "optim.hip", "calibrate.hip", "norm_bwd.hip", "norm_small.hip",
                "norm_fwd.hip", "dropout.hip"]
 HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -23,7 +23,7 @@ template <int DT> XSG_DEV void drop_store(void* out, int64_t i0, const Raw<8 * E
     float v[8];
     unpack<DT, 8>(raw, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = keep >> j & 1 ? v[j] * factor : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = keep_bit(v[j] * factor, keep, j);
     store_raw<DT, 8>(out, i0, pack<DT, 8>(v));
 }
 

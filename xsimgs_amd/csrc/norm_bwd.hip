@@ -2,8 +2,9 @@
 // z = xh weight + bias and dz = v_y act'(z) times the draw's factor, over a sample's pixels
 //   v_bias = sum dz,  v_weight = sum dz xh,
 //   v_x = rstd (weight dz - mean_group(weight dz) - xh mean_group(weight dz xh)).
-// A first pass leaves each workgroup's sums of dz and dz xh for each channel, a second joins them, a third
-// writes v_x; sums are added in a fixed order. No reference counterpart.
+// A first pass leaves each workgroup's sums of dz and dz xh for each channel, and of their products with the weight
+// for each group; a second joins the groups' (its own workgroups do, where they are few) and writes v_x, while
+// some more of its workgroups join the channels'. Sums are added in a fixed order. No reference counterpart.
 #include <algorithm>
 #include <limits.h>
 
@@ -11,200 +12,248 @@
 
 namespace {
 
-constexpr int64_t kSumsGroups = 1024;
+
+// A batch of U pixels of x and of v_y.
+template <int DT, int V, int U, bool MASK> struct GradBatch {
+    typedef Raw<V * ElementSize<DT>::value> Vec;
+    Vec x[U], g[U];
+    uint32_t in;
+    XSG_DEV void fetch(const NormArgs& a, const NormPlace<V>& at, const NormPath<DT>& x_at, const NormPath<DT>& g_at, int64_t p) {
+        in = norm_pixels<U, MASK>(a, at, p);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (in >> (16 + u) & 1) {
+                x[u] = load_raw<DT, V>(x_at(p + u * a.ty));
+                g[u] = load_raw<DT, V>(g_at(p + u * a.ty));
+            }
+    }
+};
 
 template <int DT, int V, int ACT, bool DROP, bool MASK>
 __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a, const float4* __restrict__ stats,
-                                                                 const void* __restrict__ v_y, float2* __restrict__ part) {
-    constexpr int U = 2;
+                                                                 const void* __restrict__ v_y, float2* __restrict__ groups,
+                                                                 float2* __restrict__ channels) {
+    constexpr int U = norm_grad_unroll(V * ElementSize<DT>::value);
+    constexpr bool AHEAD = norm_ahead(V * ElementSize<DT>::value);
     constexpr bool EXACT = DT == XSG_DTYPE_F32;
-    extern __shared__ float2 s_sums[];   // [rows][tx][V]
-    const int t = threadIdx.x, v = t % a.tx, r = t / a.tx;
-    const int64_t b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const int64_t p0 = chunk * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
-    const int c0 = a.first_channel<V>(v);
-    float s1[V], s2[V];
+    extern __shared__ float2 s_sums[];   // [threads][V], then [channels]
+    float2* const s_channel = s_sums + V * blockDim.x;
+    const int t = threadIdx.x;
+    const NormPlace<V> at(a, blockIdx.x, U * a.ty);
+    const bool mine = at.r < a.ty;
+    const NormPath<DT> x_at(a.x, at.b * a.batch_stride, a.pixel_stride, at.r, at.c0);
+    const NormPath<DT> g_at(v_y, at.b * a.pixels * a.channels, a.channels, at.r, at.c0);
+    const int64_t first = (at.b * a.pixels + at.r) * a.channels + at.c0;   // element, for the draws
+    GradBatch<DT, V, U, MASK> now, next;
+    now.fetch(a, at, x_at, g_at, at.p0);
+    float mean[V], scale[V], bias[V], s1[V], s2[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
-    if (r < a.ty) {
-        float mean[V], scale[V], bias[V];
+    for (int j = 0; j < V; ++j) {
+        const int c = mine ? at.c0 + j : 0;
+        const float4 s = stats[at.b * a.groups + a.by_cg(c)];
+        mean[j] = s.x;
+        scale[j] = s.y * norm_param(a.weight, a.weight_dtype, c, 1.0f);
+        bias[j] = norm_param(a.bias, a.bias_dtype, c, 0.0f);
+        s1[j] = s2[j] = 0.0f;
+    }
+    const Draws draws(a.drop);
+    for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
+        const bool more = p + at.jump < a.pixels;
+        if (AHEAD && more) next.fetch(a, at, x_at, g_at, p + at.jump);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float4 s = stats[b * a.groups + (c0 + j) / a.cg];
-            mean[j] = s.x;
-            scale[j] = s.y * norm_param(a.weight, a.weight_dtype, c0 + j, 1.0f);
-            bias[j] = norm_param(a.bias, a.bias_dtype, c0 + j, 0.0f);
-        }
-        const Draws draws(a.drop);
-        const uint8_t* const mask = MASK ? a.mask + b * a.pixels : nullptr;
-        const int64_t x0 = b * a.batch_stride + c0, y0 = b * a.pixels * a.channels + c0;
-        for (int64_t p = p0 + r; p < p1; p += U * a.ty) {
-            Raw<V * ElementSize<DT>::value> rx[U], rg[U];
-            bool kept[U];
+        for (int u = 0; u < U; ++u) {
+            const uint32_t keep = DROP ? norm_keep<V>(draws, a.channels, first + (p + u * a.ty) * a.channels) : 0;
+            if (!(now.in >> (16 + u) & 1)) continue;
+            float x[V], g[V];
+            unpack<DT, V>(now.x[u], x);
+            unpack<DT, V>(now.g[u], g);
 #pragma unroll
-            for (int u = 0; u < U; ++u) kept[u] = p + u * a.ty < p1;
-            if (MASK) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) kept[u] = kept[u] && mask[p + u * a.ty] != 0;
+            for (int j = 0; j < V; ++j) {
+                const float e = x[j] - mean[j];
+                float dz = g[j] * norm_act_slope<ACT, EXACT>(e * scale[j] + bias[j]);
+                if (DROP) dz = keep_bit(dz * a.drop.factor, keep, j);
+                s1[j] += dz;
+                s2[j] += dz * e;
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (kept[u]) {
-                    rx[u] = load_raw<DT, V>(a.x, x0 + (p + u * a.ty) * a.pixel_stride);
-                    rg[u] = load_raw<DT, V>(v_y, y0 + (p + u * a.ty) * a.channels);
-                }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (kept[u]) {
-                    float x[V], g[V];
-                    unpack<DT, V>(rx[u], x);
-                    unpack<DT, V>(rg[u], g);
-                    const uint32_t keep = DROP ? draws.keep((uint64_t)(y0 + (p + u * a.ty) * a.channels), V) : 0;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float e = x[j] - mean[j];
-                        float dz = g[j] * norm_act_slope<ACT, EXACT>(e * scale[j] + bias[j]);
-                        if (DROP) dz = keep >> j & 1 ? dz * a.drop.factor : 0.0f;
-                        s1[j] += dz;
-                        s2[j] += dz * e;
-                    }
-                }
+            if (DROP) __builtin_amdgcn_sched_barrier(0);
         }
+        if (!more) break;
+        if (AHEAD) now = next;
+        else now.fetch(a, at, x_at, g_at, p + at.jump);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) s_sums[t * V + j] = make_float2(s1[j], s2[j]);
     __syncthreads();
-    const int l = norm_segment(blockDim.x, a.channels), lane = t & (l - 1);
-    for (int c = t / l; c < a.channels; c += blockDim.x / l) {
-        const int vec = c / V, at = vec * V + c - a.first_channel<V>(vec);
+    {
+        const int l = norm_segment(blockDim.x, a.channels), lane = t & (l - 1);
+        for (int c = t / l; c < a.channels; c += blockDim.x / l) {
+            const int vec = c / V, first = vec * V + c - a.first_channel<V>(vec);
+            float2 sum = make_float2(0.0f, 0.0f);
+            for (int row = lane; row < a.ty; row += l) {
+                const float2 e = s_sums[row * a.tx * V + first];
+                sum.x += e.x;
+                sum.y += e.y;
+            }
+            sum.x = segment_sum(sum.x, l);
+            sum.y = segment_sum(sum.y, l) * stats[at.b * a.groups + a.by_cg(c)].y;
+            if (lane == 0) {
+                if (channels) channels[(int64_t)blockIdx.x * a.channels + c] = sum;
+                const float w = norm_param(a.weight, a.weight_dtype, c, 1.0f);
+                s_channel[c] = make_float2(w * sum.x, w * sum.y);
+            }
+        }
+    }
+    if (!groups) return;
+    __syncthreads();
+    const int l = norm_segment(blockDim.x, a.groups), lane = t & (l - 1);
+    for (int g = t / l; g < a.groups; g += blockDim.x / l) {
         float2 sum = make_float2(0.0f, 0.0f);
-        for (int row = lane; row < a.ty; row += l) {
-            const float2 e = s_sums[row * a.tx * V + at];
-            sum.x += e.x;
-            sum.y += e.y;
+        for (int c = g * a.cg + lane; c < (g + 1) * a.cg; c += l) {
+            sum.x += s_channel[c].x;
+            sum.y += s_channel[c].y;
         }
         sum.x = segment_sum(sum.x, l);
         sum.y = segment_sum(sum.y, l);
-        if (lane == 0)
-            part[(int64_t)blockIdx.x * a.channels + c] = make_float2(sum.x, sum.y * stats[b * a.groups + c / a.cg].y);
+        if (lane == 0) groups[(int64_t)blockIdx.x * a.groups + g] = sum;
     }
 }
 
-// Sums over `rows` rows of [rows, channels] pairs, for the eight channels from c0 on, in 64 bits: out(channel, pair).
-template <typename F>
-XSG_DEV void column_sums(const float2* __restrict__ rows, int64_t n, int channels, int c0, F out) {
-    __shared__ double s_x[256], s_y[256];
+// Adds the entries first, first + step, ... of a column, eight on their way at a time.
+XSG_DEV void add_parts(const float2* __restrict__ part, int columns, int64_t parts, int first, int step, double& x, double& y) {
+    for (int64_t k0 = first; k0 < parts; k0 += 8 * step) {
+        float2 m[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[i] = part[(k0 + i * step < parts ? k0 + i * step : first) * columns];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (k0 + i * step < parts) {
+                x += m[i].x;
+                y += m[i].y;
+            }
+    }
+}
+
+// One workgroup to a group of a sample: the means of weight dz and weight dz xh, sums in 64 bits.
+__global__ __launch_bounds__(256) void norm_means_kernel(int groups, int chunks, const float4* __restrict__ stats,
+                                                         const float2* __restrict__ part, float2* __restrict__ means) {
+    __shared__ double s_x[4], s_y[4];
+    const float2* const p = part + blockIdx.x / groups * (int64_t)chunks * groups + blockIdx.x % groups;
+    double x = 0.0, y = 0.0;
+    add_parts(p, groups, chunks, threadIdx.x, 256, x, y);
+    x = segment_sum(x, 64);
+    y = segment_sum(y, 64);
+    if ((threadIdx.x & 63) == 0) { s_x[threadIdx.x >> 6] = x; s_y[threadIdx.x >> 6] = y; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double inv = stats[blockIdx.x].z;
+        means[blockIdx.x] = make_float2((float)((s_x[0] + s_x[1] + s_x[2] + s_x[3]) * inv),
+                                        (float)((s_y[0] + s_y[1] + s_y[2] + s_y[3]) * inv));
+    }
+}
+
+// The parameters' gradients of eight channels: sums over the rows of [rows, channels] pairs, in 64 bits. A workgroup
+// of a multiple of 64 threads.
+XSG_DEV void norm_columns(int64_t rows, int channels, int c0, const float2* __restrict__ part, float* __restrict__ v_weight,
+                          float* __restrict__ v_bias) {
+    __shared__ double s_x[kNormThreads], s_y[kNormThreads];
     const int t = threadIdx.x, c = c0 + (t & 7);
     double x = 0.0, y = 0.0;
-    if (t < 256 && c < channels)
-        for (int64_t i = t >> 3; i < n; i += 32) {
-            const float2 e = rows[i * channels + c];
-            x += e.x;
-            y += e.y;
-        }
-    if (t < 256) { s_x[t] = x; s_y[t] = y; }
+    if (c < channels && t >> 3 < rows) add_parts(part + c, channels, rows, t >> 3, blockDim.x >> 3, x, y);
+    s_x[t] = x;
+    s_y[t] = y;
     __syncthreads();
     if (t < 8 && c < channels) {
-        for (int k = t + 8; k < 256; k += 8) { x += s_x[k]; y += s_y[k]; }
-        out(c, make_float2((float)x, (float)y));
+        for (int k = t + 8; k < (int)blockDim.x; k += 8) { x += s_x[k]; y += s_y[k]; }
+        if (v_bias) v_bias[c] = (float)x;
+        if (v_weight) v_weight[c] = (float)y;
     }
 }
-
-__global__ __launch_bounds__(256) void norm_columns_kernel(int64_t rows, int channels, const float2* __restrict__ part,
-                                                           float2* __restrict__ total) {
-    const int tiles = (channels + 7) / 8;
-    const int64_t b = blockIdx.x / tiles;
-    column_sums(part + b * rows * channels, rows, channels, 8 * (int)(blockIdx.x % tiles),
-                [&](int c, float2 e) { total[b * channels + c] = e; });
-}
-
-// total over the samples as the parameters' gradients, eight channels a workgroup
-__global__ __launch_bounds__(256) void norm_params_kernel(int64_t batch, int channels, const float2* __restrict__ total,
+__global__ __launch_bounds__(256) void norm_params_kernel(int64_t rows, int channels, const float2* __restrict__ part,
                                                           float* __restrict__ v_weight, float* __restrict__ v_bias) {
-    column_sums(total, batch, channels, 8 * (int)blockIdx.x, [&](int c, float2 e) {
-        if (v_bias) v_bias[c] = e.x;
-        if (v_weight) v_weight[c] = e.y;
-    });
+    norm_columns(rows, channels, 8 * (int)blockIdx.x, part, v_weight, v_bias);
 }
 
-template <int DT, int V, int ACT, bool DROP, bool MASK>
-__global__ __launch_bounds__(kNormThreads) void norm_grad_kernel(NormArgs a, const float4* __restrict__ stats,
-                                                                 const void* __restrict__ v_y,
-                                                                 const float2* __restrict__ total, void* __restrict__ v_x) {
-    constexpr int U = 2;
+// The first `param_blocks` workgroups add up the parameters' gradients, the others write v_x.
+template <int DT, int V, int ACT, bool DROP, bool MASK, bool STREAM>
+__global__ __launch_bounds__(kNormThreads) void norm_grad_kernel(NormArgs a, int param_blocks, const float4* __restrict__ stats,
+                                                                 const void* __restrict__ v_y, const float2* __restrict__ groups,
+                                                                 const float2* __restrict__ means,
+                                                                 const float2* __restrict__ channels, void* __restrict__ v_x,
+                                                                 float* __restrict__ v_weight, float* __restrict__ v_bias) {
+    constexpr int U = norm_grad_unroll(V * ElementSize<DT>::value);
+    constexpr bool AHEAD = norm_ahead(V * ElementSize<DT>::value);
     constexpr bool EXACT = DT == XSG_DTYPE_F32;
+    if ((int)blockIdx.x < param_blocks)
+        return norm_columns(a.batch * a.chunks, a.channels, 8 * (int)blockIdx.x, channels, v_weight, v_bias);
     extern __shared__ float2 s_group[];   // each group's means of weight dz and weight dz xh
-    const int t = threadIdx.x, v = t % a.tx, r = t / a.tx;
-    const int64_t b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const int64_t p0 = chunk * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
-    {
-        const int l = norm_segment(blockDim.x, a.groups), lane = t & (l - 1);
-        for (int g = t / l; g < a.groups; g += blockDim.x / l) {
-            float2 sum = make_float2(0.0f, 0.0f);
-            for (int c = g * a.cg + lane; c < (g + 1) * a.cg; c += l) {
-                const float w = norm_param(a.weight, a.weight_dtype, c, 1.0f);
-                const float2 e = total[b * a.channels + c];
-                sum.x += w * e.x;
-                sum.y += w * e.y;
-            }
-            sum.x = segment_sum(sum.x, l);
-            sum.y = segment_sum(sum.y, l);
-            const float inv = stats[b * a.groups + g].z;
-            if (lane == 0) s_group[g] = make_float2(sum.x * inv, sum.y * inv);
-        }
-    }
-    __syncthreads();
-    if (r >= a.ty) return;
-    const int c0 = a.first_channel<V>(v);
-    // v_x = scale dz - shift - (x - mean) slope
+    const NormPlace<V> at(a, gridDim.x - 1 - blockIdx.x, U * a.ty);   // from the end, which was read last
+    const bool mine = at.r < a.ty;
+    const NormPath<DT> x_at(a.x, at.b * a.batch_stride, a.pixel_stride, at.r, at.c0);
+    const NormPath<DT> g_at(v_y, at.b * a.pixels * a.channels, a.channels, at.r, at.c0);
+    const int64_t first = (at.b * a.pixels + at.r) * a.channels + at.c0;   // element, for the draws
+    const NormPath<DT> to_at(v_x, at.b * a.pixels * a.channels, a.channels, at.r, at.c0);
+    GradBatch<DT, V, U, MASK> now, next;
+    now.fetch(a, at, x_at, g_at, at.p0);
     float mean[V], scale[V], bias[V], shift[V], slope[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int g = (c0 + j) / a.cg;
-        const float4 s = stats[b * a.groups + g];
+        scale[j] = norm_param(a.weight, a.weight_dtype, mine ? at.c0 + j : 0, 1.0f);
+        bias[j] = norm_param(a.bias, a.bias_dtype, mine ? at.c0 + j : 0, 0.0f);
+    }
+    const float2* mean_of = means + at.b * a.groups;
+    if (a.join) {
+        const int l = norm_segment(blockDim.x, a.groups), lane = threadIdx.x & (l - 1);
+        const float2* const p = groups + at.b * a.chunks * a.groups;
+        for (int g = threadIdx.x / l; g < a.groups; g += blockDim.x / l) {
+            double x = 0.0, y = 0.0;
+            add_parts(p + g, a.groups, a.chunks, lane, l, x, y);
+            x = segment_sum(x, l);
+            y = segment_sum(y, l);
+            const double inv = stats[at.b * a.groups + g].z;
+            if (lane == 0) s_group[g] = make_float2((float)(x * inv), (float)(y * inv));
+        }
+        __syncthreads();
+        mean_of = s_group;
+    }
+    // v_x = scale dz - shift - (x - mean) slope
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int g = a.by_cg(mine ? at.c0 + j : 0);
+        const float4 s = stats[at.b * a.groups + g];
+        const float2 m = mean_of[g];
         mean[j] = s.x;
-        scale[j] = s.y * norm_param(a.weight, a.weight_dtype, c0 + j, 1.0f);
-        bias[j] = norm_param(a.bias, a.bias_dtype, c0 + j, 0.0f);
-        shift[j] = s.y * s_group[g].x;
-        slope[j] = s.y * s.y * s_group[g].y;
+        scale[j] *= s.y;
+        shift[j] = s.y * m.x;
+        slope[j] = s.y * s.y * m.y;
     }
     const Draws draws(a.drop);
-    const uint8_t* const mask = MASK ? a.mask + b * a.pixels : nullptr;
-    const int64_t x0 = b * a.batch_stride + c0, y0 = b * a.pixels * a.channels + c0;
-    for (int64_t p = p0 + r; p < p1; p += U * a.ty) {
-        Raw<V * ElementSize<DT>::value> rx[U], rg[U];
-        bool in[U], kept[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) in[u] = p + u * a.ty < p1;
-#pragma unroll
-        for (int u = 0; u < U; ++u) kept[u] = in[u] && (!MASK || mask[p + u * a.ty] != 0);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (kept[u]) {
-                rx[u] = load_raw<DT, V>(a.x, x0 + (p + u * a.ty) * a.pixel_stride);
-                rg[u] = load_raw<DT, V>(v_y, y0 + (p + u * a.ty) * a.channels);
-            }
+    for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
+        const bool more = p + at.jump < a.pixels;
+        if (AHEAD && more) next.fetch(a, at, x_at, g_at, p + at.jump);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (!in[u]) break;
-            const int64_t at = y0 + (p + u * a.ty) * a.channels;
+            const uint32_t keep = DROP ? norm_keep<V>(draws, a.channels, first + (p + u * a.ty) * a.channels) : 0;
+            if (!(now.in >> u & 1)) continue;
             Raw<V * ElementSize<DT>::value> out = {};
-            if (kept[u]) {
+            if (!MASK || (now.in >> (16 + u) & 1)) {
                 float x[V], g[V];
-                unpack<DT, V>(rx[u], x);
-                unpack<DT, V>(rg[u], g);
-                const uint32_t keep = DROP ? draws.keep((uint64_t)at, V) : 0;
+                unpack<DT, V>(now.x[u], x);
+                unpack<DT, V>(now.g[u], g);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float e = x[j] - mean[j];
                     float dz = g[j] * norm_act_slope<ACT, EXACT>(e * scale[j] + bias[j]);
-                    if (DROP) dz = keep >> j & 1 ? dz * a.drop.factor : 0.0f;
+                    if (DROP) dz = keep_bit(dz * a.drop.factor, keep, j);
                     x[j] = scale[j] * dz - shift[j] - e * slope[j];
                 }
                 out = pack<DT, V>(x);
             }
-            store_raw<DT, V>(v_x, at, out);
+            store_raw<DT, V, STREAM>(to_at(p + u * a.ty), 0, out);
+            if (DROP) __builtin_amdgcn_sched_barrier(0);
         }
+        if (!more) break;
+        if (AHEAD) now = next;
+        else now.fetch(a, at, x_at, g_at, p + at.jump);
     }
 }
 
@@ -231,25 +280,38 @@ extern "C" int xsg_group_norm_act_bwd(const xsg_norm_desc* d, const float* stats
     if (!stats || !v_y || !workspace) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: null tensor");
     if (const int rc = xsg_check_workspace(workspace, "group_norm_act_bwd")) return rc;
     if ((uintptr_t)stats % 16) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: stats must be 16-byte aligned");
-    const int vector = norm_vector(d);
-    norm_layout(a, vector, 2, kSumsGroups);
-    if (a.batch * a.chunks > INT_MAX / 2 || a.batch * ((a.channels + 7) / 8) > INT_MAX / 2)
-        return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: too large");
-    const unsigned grid = (unsigned)(a.batch * a.chunks), threads = (unsigned)((a.tx * a.ty + 63) / 64 * 64);
-    float2* const part = (float2*)workspace;
-    float2* const total = part + a.batch * a.chunks * a.channels;
+    const int vector = norm_vector(d, true), size = d->dtype == XSG_DTYPE_F32 ? 4 : 2;
+    norm_layout(a, vector, norm_grad_unroll(vector * size), size, 3, 256);
+    if (a.batch * std::max(a.chunks, a.groups) > INT_MAX / 2) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: too large");
+    const int64_t parts = a.batch * a.chunks;
+    float2* const groups = (float2*)workspace;
+    float2* const channels = groups + parts * a.groups;
+    float2* const means = channels + parts * a.channels;
+    const bool params = v_weight || v_bias;
+    const int tiles = (a.channels + 7) / 8;
     const float4* const st = (const float4*)stats;
     with_dtype(d->dtype, [&](auto dt) {
         with_vector(vector, [&](auto vec) {
             with_norm_flags(d, a, [&](auto act, auto drop, auto mask) {
                 constexpr int DT = decltype(dt)::value, V = decltype(vec)::value, ACT = decltype(act)::value;
                 constexpr bool DROP = decltype(drop)::value, MASK = decltype(mask)::value;
-                norm_sums_kernel<DT, V, ACT, DROP, MASK><<<grid, threads, sizeof(float2) * V * threads, s>>>(a, st, v_y, part);
-                norm_columns_kernel<<<(unsigned)(a.batch * ((a.channels + 7) / 8)), 256, 0, s>>>(a.chunks, a.channels, part, total);
-                if (v_weight || v_bias)
-                    norm_params_kernel<<<(unsigned)((a.channels + 7) / 8), 256, 0, s>>>(a.batch, a.channels, total, v_weight, v_bias);
-                if (v_x)
-                    norm_grad_kernel<DT, V, ACT, DROP, MASK><<<grid, threads, sizeof(float2) * a.groups, s>>>(a, st, v_y, total, v_x);
+                const unsigned threads = norm_threads(a);
+                norm_sums_kernel<DT, V, ACT, DROP, MASK><<<(unsigned)parts, threads, sizeof(float2) * (V * threads + a.channels), s>>>(
+                    a, st, v_y, v_x ? groups : nullptr, params ? channels : nullptr);
+                if (!v_x) {
+                    norm_params_kernel<<<(unsigned)tiles, 256, 0, s>>>(parts, a.channels, channels, v_weight, v_bias);
+                    return;
+                }
+                if (!a.join) norm_means_kernel<<<(unsigned)(a.batch * a.groups), 256, 0, s>>>(a.groups, a.chunks, st, groups, means);
+                const int param_blocks = params ? tiles : 0;
+                const unsigned grid = (unsigned)parts + param_blocks;
+                const size_t lds = a.join ? sizeof(float2) * a.groups : 0;
+                if (norm_may_stream<DT, V>() && a.stream)
+                    norm_grad_kernel<DT, V, ACT, DROP, MASK, norm_may_stream<DT, V>()><<<grid, threads, lds, s>>>(
+                        a, param_blocks, st, v_y, groups, means, channels, v_x, v_weight, v_bias);
+                else
+                    norm_grad_kernel<DT, V, ACT, DROP, MASK, false><<<grid, threads, lds, s>>>(
+                        a, param_blocks, st, v_y, groups, means, channels, v_x, v_weight, v_bias);
             });
         });
     });

@@ -8,68 +8,81 @@
 
 namespace {
 
-// Mean and sum of squared deviations of a run of pixels, per group. Nothing is subtracted from a sum of squares:
-// each thread takes its pixels a batch at a time, whose mean and deviations come from registers, and joins
-// them to what it has by the rule of Chan, Golub and LeVeque ("Algorithms for computing the sample variance", 1983);
-// so an offset that is large against the spread costs no digits. ONE: a vector lies in one group.
+constexpr int kStatsUnroll = 4;      // pixels in flight in a thread
+
+// Mean and sum of squared deviations of a workgroup's pixels, per group. A thread takes its pixels a batch at a time:
+// with m the mean and D the squared deviations of the n values so far, and s1, s2 the sums of x - m and of its square over
+// a batch, the joint mean is m + s1 / (n + nb) and the joint D is D + s2 - s1^2 / (n + nb) (the earlier values' deviations
+// add up to 0). s1^2 is at most nb s2, so no more than the bits of n / (n + nb) cancel, however large the mean is
+// against the spread; the first batch takes its own mean for m. ONE: a vector lies in one group.
 template <int DT, int V, bool ONE, bool MASK>
-__global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a, float4* __restrict__ part) {
-    constexpr int NS = ONE ? 1 : V, U = V == 8 ? 4 : 8;
+__global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a, float2* __restrict__ part,
+                                                                  float* __restrict__ counts) {
+    constexpr int NS = ONE ? 1 : V, U = kStatsUnroll;
+    typedef Raw<V * ElementSize<DT>::value> Vec;
     extern __shared__ float s_stats[];   // (mean, deviations) of each thread and slot, then counts of each thread
     float2* const s_pair = (float2*)s_stats;
     float* const s_count = s_stats + 2 * NS * blockDim.x;
-    const int t = threadIdx.x, v = t % a.tx, r = t / a.tx;
-    const int64_t b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const int64_t p0 = chunk * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
+    const NormPlace<V> at(a, blockIdx.x, U * a.ty);
+    const int t = threadIdx.x;
     float n = 0.0f, mean[NS], dev[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) mean[s] = dev[s] = 0.0f;
 
-    const auto join = [&](const Raw<V * ElementSize<DT>::value>* raw, uint32_t in, int count, auto most) {
+    const auto add = [&](const Vec* raw, uint32_t in, int count, auto most) {
         constexpr int M = decltype(most)::value;
         if (MASK && count == 0) return;
-        const float nb = (float)count, inv = 1.0f / nb;
-        const float total = n + nb, share = nb / total;
-        float sum[NS];
+        const float nb = (float)count;
+        if (n == 0.0f) {
+            float sum[NS];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) sum[s] = 0.0f;
+            for (int s = 0; s < NS; ++s) sum[s] = 0.0f;
 #pragma unroll
-        for (int u = 0; u < M; ++u) {
-            float x[V];
-            unpack<DT, V>(raw[u], x);
+            for (int u = 0; u < M; ++u) {
+                float x[V];
+                unpack<DT, V>(raw[u], x);
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum[ONE ? 0 : j] += x[j];   // zeros of pixels out of the mask
+                for (int j = 0; j < V; ++j) sum[ONE ? 0 : j] += x[j];   // zeros of pixels out of the mask
+            }
+#pragma unroll
+            for (int s = 0; s < NS; ++s) mean[s] = sum[s] / (nb * (ONE ? V : 1));
         }
-        float mb[NS], db[NS];
+        float s1[V], s2[V];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) { mb[s] = sum[s] * (ONE ? inv * (1.0f / V) : inv); db[s] = 0.0f; }
+        for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
 #pragma unroll
         for (int u = 0; u < M; ++u) {
-            if (MASK && !(in >> u & 1)) continue;
             float x[V];
             unpack<DT, V>(raw[u], x);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float e = x[j] - mb[ONE ? 0 : j];
-                db[ONE ? 0 : j] += e * e;
+                float e = x[j] - mean[ONE ? 0 : j];
+                if (MASK) e = in >> u & 1 ? e : 0.0f;
+                s1[j] += e;
+                s2[j] += e * e;
             }
+        }
+        n += nb;
+        const float inv = 1.0f / (n * (ONE ? V : 1));
+        if (ONE) {
+#pragma unroll
+            for (int j = 1; j < V; ++j) { s1[0] += s1[j]; s2[0] += s2[j]; }
         }
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const float e = mb[s] - mean[s];
-            mean[s] += e * share;
-            dev[s] += db[s] + e * e * (n * share * (ONE ? V : 1));
+            const float e = s1[s] * inv;
+            mean[s] += e;
+            dev[s] += s2[s] - s1[s] * e;
         }
-        n = total;
     };
 
-    if (r < a.ty) {
-        const int c0 = a.first_channel<V>(v);
-        const uint8_t* const mask = MASK ? a.mask + b * a.pixels : nullptr;
-        const int64_t x0 = b * a.batch_stride + c0;
-        int64_t p = p0 + r;
-        for (; p + (U - 1) * a.ty < p1; p += U * a.ty) {
-            Raw<V * ElementSize<DT>::value> raw[U];
+    if (at.r < a.ty) {
+        const NormPath<DT> x(a.x, at.b * a.batch_stride, a.pixel_stride, at.r, at.c0);
+        const uint8_t* const mask = MASK ? a.mask + at.b * a.pixels + at.r : nullptr;
+        const int step = U * a.ty;
+        int64_t p = at.p0;
+        for (; p + step <= a.pixels; p += at.jump) {
+            Vec raw[U];
             uint32_t in = (1u << U) - 1;
             if (MASK) {
                 in = 0;
@@ -79,14 +92,15 @@ __global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a, fl
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 raw[u] = {};
-                if (!MASK || (in >> u & 1)) raw[u] = load_raw<DT, V>(a.x, x0 + (p + u * a.ty) * a.pixel_stride);
+                if (!MASK || (in >> u & 1)) raw[u] = load_raw<DT, V>(x(p + u * a.ty));
             }
-            join(raw, in, MASK ? __popc(in) : U, std::integral_constant<int, U>{});
+            add(raw, in, MASK ? __popc(in) : U, std::integral_constant<int, U>{});
         }
-        for (; p < p1; p += a.ty) {
-            if (MASK && !mask[p]) continue;
-            const auto raw = load_raw<DT, V>(a.x, x0 + p * a.pixel_stride);
-            join(&raw, 1, 1, std::integral_constant<int, 1>{});
+        // a last batch of fewer pixels
+        for (int u = 0; u < U && p + u * a.ty + at.r < a.pixels; ++u) {
+            if (MASK && !mask[p + u * a.ty]) continue;
+            const Vec raw = load_raw<DT, V>(x(p + u * a.ty));
+            add(&raw, 1, 1, std::integral_constant<int, 1>{});
         }
     }
 #pragma unroll
@@ -97,129 +111,211 @@ __global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a, fl
     // a segment of lanes joins a group's entries: ty rows of its vectors (ONE) or channels
     const int l = norm_segment(blockDim.x, a.groups), lane = t & (l - 1);
     const int width = ONE ? a.cg / V : a.cg, entries = width * a.ty;
+    const float inv_width = ONE ? a.inv_cg * V : a.inv_cg;
+    const int row0 = (int)((lane + 0.5f) * inv_width), col0 = lane - row0 * width;
+    const int rows = (int)((l + 0.5f) * inv_width), cols = l - rows * width;
     for (int g = t / l; g < a.groups; g += blockDim.x / l) {
-        const auto at = [&](int e, int& thread) {
-            const int row = e / width, c = g * width + e % width;
-            if (ONE) {
-                thread = row * a.tx + c;
-                return s_pair[thread];
+        // (row, col) of entry lane, lane + l, ...
+        const auto each = [&](auto f) {
+            int row = row0, col = col0;
+            for (int e = lane; e < entries; e += l) {
+                const int c = g * width + col, vec = ONE ? c : c / V, thread = row * a.tx + vec;
+                f(s_pair[ONE ? thread : thread * NS + c - a.first_channel<V>(vec)], s_count[thread]);
+                row += rows;
+                col += cols;
+                if (col >= width) { col -= width; ++row; }
             }
-            const int vec = c / V;
-            thread = row * a.tx + vec;
-            return s_pair[thread * NS + c - a.first_channel<V>(vec)];
         };
         float count = 0.0f, sum = 0.0f;
-        for (int e = lane; e < entries; e += l) {
-            int thread;
-            const float2 m = at(e, thread);
-            count += s_count[thread];
-            sum += s_count[thread] * m.x;
-        }
+        each([&](float2 m, float k) { count += k; sum += k * m.x; });
         count = segment_sum(count, l);
         sum = segment_sum(sum, l);
         const float mu = count > 0.0f ? sum / count : 0.0f;
         float d = 0.0f;
-        for (int e = lane; e < entries; e += l) {
-            int thread;
-            const float2 m = at(e, thread);
-            d += m.y + s_count[thread] * (m.x - mu) * (m.x - mu);
-        }
+        each([&](float2 m, float k) { d += m.y + k * (m.x - mu) * (m.x - mu); });
         d = segment_sum(d, l);
-        if (lane == 0) part[(int64_t)blockIdx.x * a.groups + g] = make_float4(count, mu, d, 0.0f);
+        if (lane == 0) part[(int64_t)blockIdx.x * a.groups + g] = make_float2(mu, d);
+        if (lane == 0 && g == 0) counts[blockIdx.x] = count;
     }
 }
 
-// The parts of a sample's group joined, in 64 bits: one wavefront to a group.
-__global__ __launch_bounds__(256) void norm_join_kernel(int64_t n_groups, int groups, int chunks, double eps,
-                                                        const float4* __restrict__ part, float4* __restrict__ stats) {
-    const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    if (i >= n_groups) return;
-    const int lane = threadIdx.x & 63;
-    const float4* const p = part + i / groups * chunks * groups + i % groups;
-    double n = 0.0, sum = 0.0;
-    for (int k = lane; k < chunks; k += 64) {
-        const float4 e = p[(int64_t)k * groups];
-        n += e.x;
-        sum += (double)e.x * e.y;
+// A group's chunks joined in 64 bits, about the first chunk's mean (squares of differences of means, in digits to spare).
+struct NormSums {
+    double n, s1, s2, d;
+    XSG_DEV NormSums() : n(0.0), s1(0.0), s2(0.0), d(0.0) {}
+    XSG_DEV void add(float2 m, float count, float about) {
+        const double e = (double)m.x - about;
+        n += count;
+        s1 += count * e;
+        s2 += count * e * e;
+        d += m.y;
     }
-    n = segment_sum(n, 64);
-    sum = segment_sum(sum, 64);
-    const double mean = n > 0.0 ? sum / n : 0.0;
-    double d = 0.0;
-    for (int k = lane; k < chunks; k += 64) {
-        const float4 e = p[(int64_t)k * groups];
-        if (e.x > 0.0f) d += e.z + e.x * (e.y - mean) * (e.y - mean);
+    // the last steps in 32 bits: they are relative to the spread
+    XSG_DEV float4 stats(float about, float eps) const {
+        const float inv = n > 0.0 ? 1.0f / (float)n : 0.0f;
+        float var = (float)(d + s2 - s1 * s1 * (double)inv) * inv;
+        if (var < 0.0f) var = 0.0f;   // a NaN stays
+        return make_float4(about + (float)s1 * inv, 1.0f / sqrtf(var + eps), inv, 0.0f);
     }
-    d = segment_sum(d, 64);
-    if (lane == 0) {
-        const double inv = n > 0.0 ? 1.0 / n : 0.0;
-        stats[i] = make_float4((float)mean, (float)(1.0 / sqrt(d * inv + eps)), (float)inv, 0.0f);
+    // entries first, first + step, ... of a group's parts, eight on their way at a time
+    XSG_DEV void add_parts(const float2* __restrict__ part, const float* __restrict__ counts, int groups, int parts,
+                           int first, int step, float about) {
+        for (int k0 = first; k0 < parts; k0 += 8 * step) {
+            float2 m[8];
+            float c[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int k = k0 + i * step < parts ? k0 + i * step : first;
+                m[i] = part[(int64_t)k * groups];
+                c[i] = counts[k];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (k0 + i * step < parts) add(m[i], c[i], about);
+        }
+    }
+};
+
+// One workgroup to a group of a sample.
+__global__ __launch_bounds__(256) void norm_join_kernel(int groups, int chunks, float eps, const float2* __restrict__ part,
+                                                        const float* __restrict__ counts, float4* __restrict__ stats) {
+    __shared__ double s_sum[4][4];
+    const int64_t b = blockIdx.x / groups;
+    const float2* const p = part + b * chunks * groups + blockIdx.x % groups;
+    const float* const c = counts + b * chunks;
+    const float about = p[0].x;
+    NormSums sum;
+    sum.add_parts(p, c, groups, chunks, threadIdx.x, 256, about);
+    double* const mine = s_sum[threadIdx.x >> 6];
+    const double n = segment_sum(sum.n, 64), s1 = segment_sum(sum.s1, 64), s2 = segment_sum(sum.s2, 64), d = segment_sum(sum.d, 64);
+    if ((threadIdx.x & 63) == 0) { mine[0] = n; mine[1] = s1; mine[2] = s2; mine[3] = d; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        NormSums all;
+        for (int w = 0; w < 4; ++w) {
+            all.n += s_sum[w][0];
+            all.s1 += s_sum[w][1];
+            all.s2 += s_sum[w][2];
+            all.d += s_sum[w][3];
+        }
+        stats[blockIdx.x] = all.stats(about, eps);
     }
 }
 
-template <int DT, int V, int ACT, bool DROP, bool MASK>
-__global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, const float4* __restrict__ stats,
-                                                                  void* __restrict__ y) {
-    constexpr int U = 4;
+template <int DT, int V, int ACT, bool DROP, bool MASK, bool STREAM>
+__global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, int parts, const float2* __restrict__ part,
+                                                                  const float* __restrict__ counts,
+                                                                  float4* __restrict__ stats, void* __restrict__ y) {
+    constexpr int U = norm_apply_unroll(V * ElementSize<DT>::value);
+    constexpr bool AHEAD = norm_ahead(V * ElementSize<DT>::value);
     constexpr bool EXACT = DT == XSG_DTYPE_F32;
-    const int t = threadIdx.x, v = t % a.tx, r = t / a.tx;
-    if (r >= a.ty) return;
-    const int64_t b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const int64_t p0 = chunk * a.chunk, p1 = min(p0 + a.chunk, a.pixels);
-    const int c0 = a.first_channel<V>(v);
-    float mean[V], scale[V], bias[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float4 s = stats[b * a.groups + (c0 + j) / a.cg];
-        mean[j] = s.x;
-        scale[j] = s.y * norm_param(a.weight, a.weight_dtype, c0 + j, 1.0f);
-        bias[j] = norm_param(a.bias, a.bias_dtype, c0 + j, 0.0f);
-    }
-    const Draws draws(a.drop);
-    const uint8_t* const mask = MASK ? a.mask + b * a.pixels : nullptr;
-    const int64_t x0 = b * a.batch_stride + c0, y0 = b * a.pixels * a.channels + c0;
-    for (int64_t p = p0 + r; p < p1; p += U * a.ty) {
-        Raw<V * ElementSize<DT>::value> raw[U];
-        bool in[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) in[u] = p + u * a.ty < p1;
-        bool kept[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) kept[u] = in[u] && (!MASK || mask[p + u * a.ty] != 0);
+    typedef Raw<V * ElementSize<DT>::value> Vec;
+    extern __shared__ float4 s_group[];
+    const NormPlace<V> at(a, gridDim.x - 1 - blockIdx.x, U * a.ty);   // from the end, which was read last
+    const bool mine = at.r < a.ty;
+    const NormPath<DT> x_at(a.x, at.b * a.batch_stride, a.pixel_stride, at.r, at.c0);
+    const NormPath<DT> y_at(y, at.b * a.pixels * a.channels, a.channels, at.r, at.c0);
+    const int64_t first = (at.b * a.pixels + at.r) * a.channels + at.c0;   // element, for the draws
+    const auto fetch = [&](int64_t p, Vec* raw) {
+        const uint32_t in = norm_pixels<U, MASK>(a, at, p);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             raw[u] = {};
-            if (kept[u]) raw[u] = load_raw<DT, V>(a.x, x0 + (p + u * a.ty) * a.pixel_stride);
+            if (in >> (16 + u) & 1) raw[u] = load_raw<DT, V>(x_at(p + u * a.ty));
         }
+        return in;
+    };
+    Vec raw[U], next[U];
+    uint32_t in = fetch(at.p0, raw), in_next = 0;
+
+    float mean[V], scale[V], bias[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        scale[j] = norm_param(a.weight, a.weight_dtype, mine ? at.c0 + j : 0, 1.0f);
+        bias[j] = norm_param(a.bias, a.bias_dtype, mine ? at.c0 + j : 0, 0.0f);
+    }
+    const float4* group = stats + at.b * a.groups;
+    if (a.join) {
+        const int l = norm_segment(blockDim.x, a.groups), lane = threadIdx.x & (l - 1);
+        const float2* const p = part + at.b * parts * a.groups;
+        for (int g = threadIdx.x / l; g < a.groups; g += blockDim.x / l) {
+            NormSums sum;
+            const float about = p[g].x;
+            sum.add_parts(p + g, counts + at.b * parts, a.groups, parts, lane, l, about);
+            sum.n = segment_sum(sum.n, l);
+            sum.s1 = segment_sum(sum.s1, l);
+            sum.s2 = segment_sum(sum.s2, l);
+            sum.d = segment_sum(sum.d, l);
+            if (lane == 0) {
+                s_group[g] = sum.stats(about, a.eps);
+                if (at.chunk == 0) stats[at.b * a.groups + g] = s_group[g];
+            }
+        }
+        __syncthreads();
+        group = s_group;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float4 s = group[a.by_cg(mine ? at.c0 + j : 0)];
+        mean[j] = s.x;
+        scale[j] *= s.y;
+    }
+    const Draws draws(a.drop);
+    const float kept = 1.0f / a.drop.factor;
+    // (x - mean) scale + bias; in 16 bits x scale + (bias - mean scale), whose cancellation is below x's own digits
+    if (!EXACT) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) bias[j] = fmaf(-mean[j], scale[j], bias[j]);
+    }
+    // every lane goes through every batch: draws are shared between them
+    for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
+        const bool more = p + at.jump < a.pixels;
+        if (AHEAD && more) in_next = fetch(p + at.jump, next);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (!in[u]) break;
-            const int64_t at = y0 + (p + u * a.ty) * a.channels;
-            Raw<V * ElementSize<DT>::value> out = {};
-            if (!MASK || kept[u]) {
+            const uint32_t keep = DROP ? norm_keep<V>(draws, a.channels, first + (p + u * a.ty) * a.channels) : 0;
+            if (!(in >> u & 1)) continue;
+            Vec out = {};
+            if (!MASK || (in >> (16 + u) & 1)) {
                 float x[V];
                 unpack<DT, V>(raw[u], x);
-                const uint32_t keep = DROP ? draws.keep((uint64_t)at, V) : 0;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    x[j] = norm_act<ACT, EXACT>((x[j] - mean[j]) * scale[j] + bias[j]);
-                    if (DROP) x[j] = keep >> j & 1 ? x[j] * a.drop.factor : 0.0f;
+                    const float z = EXACT ? fmaf(x[j] - mean[j], scale[j], bias[j]) : fmaf(x[j], scale[j], bias[j]);
+                    x[j] = norm_act<ACT, EXACT, DROP>(z, a.drop.factor, kept);
+                    if (DROP) x[j] = keep_bit(x[j], keep, j);
                 }
                 out = pack<DT, V>(x);
             }
-            store_raw<DT, V>(y, at, out);
+            store_raw<DT, V, STREAM>(y_at(p + u * a.ty), 0, out);
+            if (DROP) __builtin_amdgcn_sched_barrier(0);   // draws of several pixels at once take too many registers
+        }
+        if (!more) break;
+        if (AHEAD) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = next[u];
+            in = in_next;
+        } else {
+            in = fetch(p + at.jump, raw);
         }
     }
 }
 
-constexpr int64_t kStatsGroups = 1024;   // workgroups of a pass
+// Workgroups of a pass: as many as 64 KB of x to each 256 threads make, eight of those to a CU at most (265 MB: 2048
+// 373 us a training pass, 1024 385) and two at least (31 MB: 512 77 us, 1024 87, whose results take longer to join).
+constexpr int64_t kThreadBytes = 256, kMostThreads = 2048 * 256, kFewThreads = 512 * 256;
+// Results go around the caches from here on.
+#ifndef CB
+#define CB 256
+#endif
+constexpr int64_t kCacheBytes = (int64_t)CB << 20;
 
 }  // namespace
 
-int norm_vector(const xsg_norm_desc* d) {
-    // vectors of 16 bytes; eight float32 where a vector then holds a whole block of draws, or a workgroup the channels
+int norm_vector(const xsg_norm_desc* d, bool draws) {
+    // vectors of 16 bytes; eight float32 where there are draws, which come eight at a time, or too many channels
     if (d->dtype != XSG_DTYPE_F32) return d->channels >= 8 ? 8 : d->channels >= 4 ? 4 : 1;
-    if (d->channels > 4 * kNormThreads || (d->drop.p > 0.0 && d->channels % 8 == 0)) return 8;
+    if (d->channels > 4 * kNormThreads || (draws && d->drop.p > 0.0 && d->channels >= 8)) return 8;
     return d->channels >= 4 ? 4 : 1;
 }
 
@@ -249,6 +345,7 @@ int norm_args(const xsg_norm_desc* d, NormArgs& a, const char* who) {
     a.batch_stride = d->batch_stride; a.pixel_stride = d->pixel_stride;
     a.batch = d->batch; a.pixels = d->pixels;
     a.channels = d->channels; a.groups = d->groups; a.cg = d->channels / d->groups;
+    a.inv_cg = 1.0f / a.cg;
     a.mask = d->mask;
     a.weight = d->weight; a.bias = d->bias;
     a.weight_dtype = d->weight_dtype; a.bias_dtype = d->bias_dtype;
@@ -256,32 +353,30 @@ int norm_args(const xsg_norm_desc* d, NormArgs& a, const char* who) {
     return drop_args(&d->drop, a.drop, who);
 }
 
-void norm_layout(NormArgs& a, int vector, int in_flight, int64_t workgroups) {
-    a.nv = (a.channels + vector - 1) / vector;
-    a.tx = a.nv;
-    // about 256 threads, of which as few as possible idle in the last wavefront
+void norm_layout(NormArgs& a, int vector, int in_flight, int element_size, int tensors, int threads) {
+    a.tx = (a.channels + vector - 1) / vector;
+    a.inv_tx = 1.0f / a.tx;
+    // about so many threads, of which as few as possible idle in the last wavefront
     double best = 0.0;
-    for (int ty = std::max(1, 256 / a.tx); ty * a.tx <= kNormThreads; ++ty) {
+    for (int ty = std::max(1, threads / a.tx); ty * a.tx <= kNormThreads; ++ty) {
         const double used = (double)(ty * a.tx) / ((ty * a.tx + 63) / 64 * 64);
         if (used > best) { best = used; a.ty = ty; }
     }
-    const int64_t step = (int64_t)a.ty * in_flight;
-    const int64_t wanted = std::max<int64_t>(1, std::min((a.pixels + step - 1) / step, (workgroups + a.batch - 1) / a.batch));
-    a.chunk = ((a.pixels + wanted - 1) / wanted + step - 1) / step * step;
-    a.chunks = (int)((a.pixels + a.chunk - 1) / a.chunk);
+    const int64_t bytes = a.batch * a.pixels * a.channels * element_size, step = (int64_t)a.ty * in_flight;
+    const int64_t workgroups = std::min(kMostThreads, std::max(kFewThreads, bytes / kThreadBytes)) / threads;
+    a.chunks = (int)std::max<int64_t>(1, std::min((a.pixels + step - 1) / step, (workgroups + a.batch - 1) / a.batch));
+    a.join = (int64_t)a.chunks * a.groups <= kNormJoin;
+    a.stream = bytes * tensors > kCacheBytes;
 }
-
-static unsigned norm_threads(const NormArgs& a) { return (unsigned)((a.tx * a.ty + 63) / 64 * 64); }
 
 extern "C" size_t xsg_group_norm_act_workspace_bytes(const xsg_norm_desc* d, int backward) {
     NormArgs a;
     if (norm_args(d, a, "group_norm_act") != XSG_OK || d->batch == 0 || d->pixels == 0) return 0;
-    if (backward) {
-        norm_layout(a, norm_vector(d), 2, kStatsGroups);
-        return sizeof(float2) * (size_t)a.channels * (size_t)(a.batch * a.chunks + a.batch);
-    }
-    norm_layout(a, norm_vector(d), 4, kStatsGroups);
-    return sizeof(float4) * (size_t)a.groups * (size_t)(a.batch * a.chunks);
+    const int vector = norm_vector(d, backward != 0), size = d->dtype == XSG_DTYPE_F32 ? 4 : 2;
+    norm_layout(a, vector, backward ? norm_grad_unroll(vector * size) : kStatsUnroll, size, 0, backward ? 256 : 512);
+    const size_t parts = (size_t)(a.batch * a.chunks);
+    if (backward) return sizeof(float2) * (parts * (size_t)(a.channels + a.groups) + (size_t)(a.batch * a.groups));
+    return sizeof(float2) * parts * (size_t)a.groups + sizeof(float) * parts;
 }
 
 extern "C" int xsg_group_norm_act_fwd(const xsg_norm_desc* d, void* y, float* stats, void* workspace, xsg_stream_t stream) {
@@ -291,26 +386,49 @@ extern "C" int xsg_group_norm_act_fwd(const xsg_norm_desc* d, void* y, float* st
     if (!y || !stats || !workspace) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_fwd: null tensor");
     if (const int rc = xsg_check_workspace(workspace, "group_norm_act_fwd")) return rc;
     if ((uintptr_t)stats % 16) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_fwd: stats must be 16-byte aligned");
-    const int vector = norm_vector(d);
-    norm_layout(a, vector, 4, kStatsGroups);
-    if (a.batch * a.chunks > INT_MAX / 2) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_fwd: too large");
+    if (norm_small(d, a, y, stats, (hipStream_t)stream)) {
+        XSG_TRY_LAUNCH("group_norm_act_fwd");
+        return XSG_OK;
+    }
+    const int size = d->dtype == XSG_DTYPE_F32 ? 4 : 2, vector = norm_vector(d, false), draw_vector = norm_vector(d, true);
+    norm_layout(a, vector, kStatsUnroll, size, 2, 512);
+    if (a.batch * std::max(a.chunks, a.groups) > INT_MAX / 2) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_fwd: too large");
     const hipStream_t s = (hipStream_t)stream;
-    const unsigned grid = (unsigned)(a.batch * a.chunks), threads = norm_threads(a);
-    const bool one = a.cg % vector == 0;
+    float2* const part = (float2*)workspace;
+    float* const counts = (float*)(part + a.batch * a.chunks * a.groups);
+    const int chunks = a.chunks;
     with_dtype(d->dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
         with_vector(vector, [&](auto vec) {
-            constexpr int DT = decltype(dt)::value, V = decltype(vec)::value;
-            const size_t lds = sizeof(float) * threads * (2 * (one ? 1 : V) + 1);
-            float4* const part = (float4*)workspace;
-            if (one && a.mask) norm_stats_kernel<DT, V, true, true><<<grid, threads, lds, s>>>(a, part);
-            else if (one) norm_stats_kernel<DT, V, true, false><<<grid, threads, lds, s>>>(a, part);
-            else if (a.mask) norm_stats_kernel<DT, V, false, true><<<grid, threads, lds, s>>>(a, part);
-            else norm_stats_kernel<DT, V, false, false><<<grid, threads, lds, s>>>(a, part);
-            const int64_t n_groups = a.batch * a.groups;
-            norm_join_kernel<<<xsg_blocks(n_groups, 4), 256, 0, s>>>(n_groups, a.groups, a.chunks, d->eps, part, (float4*)stats);
+            constexpr int V = decltype(vec)::value;
+            const auto stats_pass = [&](auto one_group) {
+                constexpr bool ONE = decltype(one_group)::value;
+                const unsigned grid = (unsigned)(a.batch * chunks), threads = norm_threads(a);
+                const size_t lds = sizeof(float) * threads * (2 * (ONE ? 1 : V) + 1);
+                if (a.mask) norm_stats_kernel<DT, V, ONE, true><<<grid, threads, lds, s>>>(a, part, counts);
+                else norm_stats_kernel<DT, V, ONE, false><<<grid, threads, lds, s>>>(a, part, counts);
+            };
+            if constexpr (V == 1) stats_pass(std::true_type{});
+            else if (a.cg % V == 0) stats_pass(std::true_type{});
+            else stats_pass(std::false_type{});
+        });
+        if (!a.join)
+            norm_join_kernel<<<(unsigned)(a.batch * a.groups), 256, 0, s>>>(a.groups, chunks, a.eps, part, counts, (float4*)stats);
+        const int join = a.join;
+        norm_layout(a, draw_vector, norm_apply_unroll(draw_vector * size), size, 2, 256);
+        a.join = join;
+        with_vector(draw_vector, [&](auto vec) {
             with_norm_flags(d, a, [&](auto act, auto drop, auto mask) {
-                norm_apply_kernel<DT, V, decltype(act)::value, decltype(drop)::value, decltype(mask)::value>
-                    <<<grid, threads, 0, s>>>(a, (const float4*)stats, y);
+                constexpr int V = decltype(vec)::value, ACT = decltype(act)::value;
+                constexpr bool DROP = decltype(drop)::value, MASK = decltype(mask)::value;
+                const unsigned grid = (unsigned)(a.batch * a.chunks), threads = norm_threads(a);
+                const size_t lds = join ? sizeof(float4) * a.groups : 0;
+                if (norm_may_stream<DT, V>() && a.stream)
+                    norm_apply_kernel<DT, V, ACT, DROP, MASK, norm_may_stream<DT, V>()>
+                        <<<grid, threads, lds, s>>>(a, chunks, part, counts, (float4*)stats, y);
+                else
+                    norm_apply_kernel<DT, V, ACT, DROP, MASK, false>
+                        <<<grid, threads, lds, s>>>(a, chunks, part, counts, (float4*)stats, y);
             });
         });
     });

@@ -24,7 +24,7 @@ template <int ALIGN, bool STREAM, typename T> XSG_DEV void raw_put(void* p, T x)
 }
 
 template <int DT, int V, bool STREAM = false>
-XSG_DEV Raw<V * ElementSize<DT>::value> load_raw(const void* base, int64_t at) {
+XSG_DEV Raw<V * ElementSize<DT>::value> load_raw(const void* base, int64_t at = 0) {
     constexpr int E = ElementSize<DT>::value, BYTES = V * E;
     const char* p = (const char*)base + at * E;
     Raw<BYTES> r;

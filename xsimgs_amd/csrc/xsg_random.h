@@ -8,11 +8,13 @@
 
 struct Words4 { uint32_t w[4]; };
 
-XSG_HD Words4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
+XSG_DEV uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
+
+XSG_DEV Words4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-        const uint32_t n0 = (uint32_t)(b >> 32) ^ c1 ^ k0, n2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        const uint32_t n0 = xor3((uint32_t)(b >> 32), c1, k0), n2 = xor3((uint32_t)(a >> 32), c3, k1);
         c0 = n0; c1 = (uint32_t)b; c2 = n2; c3 = (uint32_t)a;
         k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
     }
@@ -44,6 +46,7 @@ inline int drop_args(const xsg_drop_desc* d, DropArgs& out, const char* who) {
 
 // The draws of one call in the kernel.
 struct Draws {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     uint32_t k0, k1, stream, upper, lower;   // upper: the threshold's upper 16 bits (up to 2^16)
 
     XSG_DEV explicit Draws(const DropArgs& d) {
@@ -58,22 +61,29 @@ struct Draws {
     // Bit j: value 8 block + j is kept. Sixteen bits a value, so one call serves eight; only a value whose sixteen
     // equal the threshold's (1 in 65536) needs the lower sixteen, from a second call. So the comparison is of 32
     // bits at the price of 16: the generator's integer products issue at a quarter of the rate, and with 32 bits
-    // a value they would take as long as moving it.
+    // a value they would take as long as moving it. The halves are compared two at a time.
     XSG_DEV uint32_t keep8(uint64_t block) const {
         const Words4 r = words(block, 0);
-        uint32_t keep = 0, tie = 0;
+        const uint32_t below = (upper ? upper - 1 : 0) * 0x10001u, at = upper * 0x10001u;
+        uint32_t m = upper ? 0 : 0x550055u, apart = ~0u;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t h = j & 1 ? r.w[j >> 1] >> 16 : r.w[j >> 1] & 0xffffu;
-            keep |= (uint32_t)(h >= upper) << j;
-            tie |= (uint32_t)(h == upper) << j;
+        for (int k = 0; k < 4; ++k) {
+            // 1 in each half that is above `below`: the saturated difference, or 1 (by name: the compiler takes this
+            // apart into comparisons and selections of single halves)
+            uint32_t over;
+            asm("v_pk_sub_u16 %0, %1, %2 clamp\n\tv_pk_min_u16 %0, %0, %3" : "=&v"(over) : "v"(r.w[k]), "v"(below), "v"(0x10001u));
+            m |= over << (2 * k);
+            // a half of 0 where one equals the threshold's
+            apart = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, apart),
+                                                                           __builtin_bit_cast(u16x2, r.w[k] ^ at)));
         }
-        if (lower != 0 && tie != 0) {
+        uint32_t keep = (m | m >> 15) & 0xffu;
+        if (lower != 0 && ((apart & 0xffffu) == 0 || apart < 0x10000u)) {
             const Words4 s = words(block, 1);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t h = j & 1 ? s.w[j >> 1] >> 16 : s.w[j >> 1] & 0xffffu;
-                if ((tie >> j & 1) && h < lower) keep &= ~(1u << j);
+                const uint32_t h = r.w[j >> 1] >> 16 * (j & 1) & 0xffffu, l = s.w[j >> 1] >> 16 * (j & 1) & 0xffffu;
+                if (h == upper && l < lower) keep &= ~(1u << j);
             }
         }
         return keep;
@@ -85,4 +95,27 @@ struct Draws {
         if (at + n > 8) bits |= keep8((first >> 3) + 1) << 8;
         return bits >> at;
     }
+    // keep(first, 8) where the lanes of a wavefront, all of them here, hold runs in order that together lie in about 64
+    // blocks: lane i draws the i-th of them, and each takes its two from the lanes that have them.
+    XSG_DEV uint32_t keep_in_order(uint64_t first) const {
+        const uint64_t mine = first >> 3;
+        const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)mine) |
+                              (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(mine >> 32)) << 32;
+        const uint32_t drawn = keep8(base + __lane_id());
+        const uint64_t from = mine - base;
+        uint32_t bits = __shfl(drawn, (int)(from & 63)) | __shfl(drawn, (int)((from + 1) & 63)) << 8;
+        // lanes at the end of a wavefront may reach past what it drew
+        if (from > 62) {
+            if (from > 63) bits = keep8(mine) | (bits & 0xff00u);
+            if (first & 7u) bits = (bits & 0xffu) | keep8(mine + 1) << 8;
+        }
+        return bits >> ((uint32_t)first & 7u);
+    }
 };
+
+// x where bit j of keep is set, else 0, whatever x holds
+XSG_DEV float keep_bit(float x, uint32_t keep, int j) {
+    uint32_t all = (uint32_t)__builtin_amdgcn_sbfe((int)keep, j, 1);
+    asm("" : "+v"(all));   // one AND: the compiler would make a comparison and a selection of it
+    return __uint_as_float(__float_as_uint(x) & all);
+}
