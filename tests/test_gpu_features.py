@@ -370,9 +370,13 @@ def test_refusals(dev):
                        (lambda: f(x, 2, drop=0.5, seed=torch.zeros(2, dtype=torch.int64, device=dev)), "one int64")):
         with pytest.raises(RuntimeError, match=says):
             call()
-    y = f(x.requires_grad_(), 2)
-    with pytest.raises(RuntimeError, match="once_differentiable|twice|does not require grad"):
-        torch.autograd.grad(torch.autograd.grad(y.sum(), x, create_graph=True)[0].sum(), x)
+    # a gradient's gradient: the first comes, the second is refused, also beside other terms
+    x.requires_grad_()
+    for y in (f(x, 2, w, b), rendering.dropout(x, 0.5, 1)):
+        g, = torch.autograd.grad((y * x).sum(), x, create_graph=True)
+        for total in (g.sum(), (g * x).sum()):
+            with pytest.raises(RuntimeError, match="differentiated once"):
+                torch.autograd.grad(total, x, retain_graph=True)
 
 
 def test_graphs_and_streams(dev):

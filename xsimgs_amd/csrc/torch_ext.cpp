@@ -2,6 +2,8 @@
 // xsimgs_amd C-ABI. This file validates and allocates exactly as the reference ops do, then calls
 // the HIP kernels through include/xsimgs_amd.h on the current stream of the input's device.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <c10/util/SmallVector.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -1080,16 +1082,79 @@ xsg_drop_desc drop_desc(double p, int64_t seed, const OptT& seed_at, int64_t str
                          seed_at.has_value() ? (const uint64_t*)seed_at->data_ptr<int64_t>() : nullptr, (uint32_t)stream};
 }
 
-Tensor dropout(const Tensor& x, double p, int64_t seed, const OptT& seed_at, int64_t stream, int64_t shared) {
-    TORCH_CHECK(x.is_contiguous(), "x must be contiguous");
-    const int dt = dtype_code(x, "x");
-    const xsg_stream_t s = stream_of(x);
-    const auto d = drop_desc(p, seed, seed_at, stream, x.device());
-    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+// Autograd in C++ for these operators: on small tensors the calls through Python would cost more than the kernels.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(std::initializer_list<const OptT*> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const OptT* t : ts)
+        if (t->has_value() && (*t)->defined() && (*t)->requires_grad()) return true;
+    return false;
+}
+
+OptT optional(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+Tensor defined_or_not(const OptT& t) { return t.value_or(Tensor()); }
+
+// Gradients that are asked for with a graph of their own (create_graph) raise when that is followed to what they were
+// made of.
+template <typename... Ts> variable_list differentiated_once(variable_list grads, const char* who, const Ts&... made_of) {
+    if (!at::GradMode::is_enabled()) return grads;
+    const auto error = std::make_shared<torch::autograd::Error>(std::string(who) + " is differentiated once",
+                                                                torch::autograd::collect_next_edges(made_of...));
+    for (auto& g : grads)
+        if (g.defined()) {
+            g = g.detach();
+            torch::autograd::set_history(g, error);
+        }
+    return grads;
+}
+
+// The draws' arguments, kept from a forward for its backward.
+void keep_draws(AutogradContext* ctx, double p, int64_t seed, int64_t stream) {
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["stream"] = stream;
+}
+struct KeptDraws {
+    double p;
+    int64_t seed, stream;
+    explicit KeptDraws(AutogradContext* ctx)
+        : p(ctx->saved_data["p"].toDouble()), seed(ctx->saved_data["seed"].toInt()), stream(ctx->saved_data["stream"].toInt()) {}
+};
+
+Tensor dropout_values(const Tensor& input, double p, int64_t seed, const OptT& seed_at, int64_t stream, int64_t shared) {
+    const xsg_stream_t s = stream_of(input);
+    const int dt = dtype_code(input, "x");
+    const auto d = drop_desc(p, seed, seed_at, stream, input.device());
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(input.device());
+    const Tensor x = input.contiguous();
     Tensor out = at::empty(x.sizes(), x.options());
     if (x.numel() == 0) return out;
     check_rc(xsg_dropout(&d, dt, x.numel(), shared, x.data_ptr(), out.data_ptr(), s));
     return out;
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptT& seed_at, double p, int64_t seed,
+                          int64_t stream, int64_t shared) {
+        keep_draws(ctx, p, seed, stream);
+        ctx->saved_data["shared"] = shared;
+        ctx->save_for_backward({defined_or_not(seed_at)});
+        return dropout_values(x, p, seed, seed_at, stream, shared);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const KeptDraws k(ctx);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor v_x = dropout_values(grads[0], k.p, k.seed, optional(saved[0]), k.stream, ctx->saved_data["shared"].toInt());
+        return differentiated_once({v_x, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, "dropout", grads[0]);
+    }
+};
+
+Tensor dropout(const Tensor& x, double p, int64_t seed, const OptT& seed_at, int64_t stream, int64_t shared) {
+    const OptT ox(x);
+    if (wants_grad({&ox})) return Dropout::apply(x, seed_at, p, seed, stream, shared);
+    return dropout_values(x, p, seed, seed_at, stream, shared);
 }
 
 Tensor drop_mask(int64_t n, double p, int64_t seed, const OptT& seed_at, int64_t stream, const c10::Device& device) {
@@ -1102,46 +1167,49 @@ Tensor drop_mask(int64_t n, double p, int64_t seed, const OptT& seed_at, int64_t
     return out;
 }
 
-std::tuple<Tensor, Tensor> activate_drop_fwd(const Tensor& log_scales, const Tensor& opacity_logits, double p,
-                                             int64_t seed, const OptT& seed_at, int64_t stream) {
-    check_same_device({log_scales, opacity_logits});
-    all_contiguous({log_scales, opacity_logits});
-    check_f32(log_scales, "log_scales");
-    check_f32(opacity_logits, "opacity_logits");
-    const int64_t n = opacity_logits.numel();
-    TORCH_CHECK(log_scales.numel() == 3 * n, "log_scales must hold three values per opacity logit");
-    const xsg_stream_t s = stream_of(log_scales);
-    const auto d = drop_desc(p, seed, seed_at, stream, log_scales.device());
-    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(log_scales.device());
-    Tensor scales = at::empty_like(log_scales), opacities = at::empty_like(opacity_logits);
-    check_rc(xsg_activate_drop_fwd(&d, n, fptr(log_scales), fptr(opacity_logits), scales.data_ptr<float>(),
-                                   opacities.data_ptr<float>(), s));
-    return {scales, opacities};
-}
+struct ActivateDrop : torch::autograd::Function<ActivateDrop> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& log_scales, const Tensor& opacity_logits,
+                                 const OptT& seed_at, double p, int64_t seed, int64_t stream) {
+        check_same_device({log_scales, opacity_logits});
+        check_f32(log_scales, "log_scales");
+        check_f32(opacity_logits, "opacity_logits");
+        const int64_t n = opacity_logits.numel();
+        TORCH_CHECK(log_scales.numel() == 3 * n, "log_scales must hold three values per opacity logit");
+        const xsg_stream_t s = stream_of(log_scales);
+        const auto d = drop_desc(p, seed, seed_at, stream, log_scales.device());
+        const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(log_scales.device());
+        const Tensor a = log_scales.contiguous(), o = opacity_logits.contiguous();
+        Tensor scales = at::empty(a.sizes(), a.options()), opacities = at::empty(o.sizes(), o.options());
+        check_rc(xsg_activate_drop_fwd(&d, n, fptr(a), fptr(o), scales.data_ptr<float>(), opacities.data_ptr<float>(), s));
+        keep_draws(ctx, p, seed, stream);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({scales, opacity_logits, defined_or_not(seed_at)});
+        return {scales, opacities};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const KeptDraws k(ctx);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &scales = saved[0], o = saved[1].contiguous();
+        Tensor v_scales, v_opacities, v_log_scales, v_logits;
+        if (grads[0].defined() && ctx->needs_input_grad(0)) v_scales = grads[0].contiguous();
+        if (grads[1].defined() && ctx->needs_input_grad(1)) v_opacities = grads[1].contiguous();
+        const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scales.device());
+        if (v_scales.defined()) v_log_scales = at::empty(scales.sizes(), scales.options());
+        if (v_opacities.defined()) v_logits = at::empty(o.sizes(), o.options());
+        const auto d = drop_desc(k.p, k.seed, optional(saved[2]), k.stream, scales.device());
+        check_rc(xsg_activate_drop_bwd(&d, o.numel(), fptr(scales), fptr(o), v_scales.defined() ? fptr(v_scales) : nullptr,
+                                       v_opacities.defined() ? fptr(v_opacities) : nullptr,
+                                       v_log_scales.defined() ? v_log_scales.data_ptr<float>() : nullptr,
+                                       v_logits.defined() ? v_logits.data_ptr<float>() : nullptr, stream_of(scales)));
+        return differentiated_once({v_log_scales, v_logits, Tensor(), Tensor(), Tensor(), Tensor()}, "activate_gaussians", scales,
+                                   saved[1], grads[0], grads[1]);
+    }
+};
 
-std::tuple<Tensor, Tensor> activate_drop_bwd(const Tensor& scales, const Tensor& opacity_logits, const OptT& v_scales,
-                                             const OptT& v_opacities, double p, int64_t seed, const OptT& seed_at,
-                                             int64_t stream) {
-    std::vector<Tensor> ts{scales, opacity_logits};
-    for (const OptT* o : {&v_scales, &v_opacities})
-        if (o->has_value()) ts.push_back(**o);
-    check_same_device(ts);
-    all_contiguous(ts);
-    for (const auto& t : ts) check_f32(t, "activation tensors");
-    const int64_t n = opacity_logits.numel();
-    TORCH_CHECK(scales.numel() == 3 * n, "scales must hold three values per opacity logit");
-    TORCH_CHECK(!v_scales.has_value() || v_scales->numel() == 3 * n, "v_scales must match scales");
-    TORCH_CHECK(!v_opacities.has_value() || v_opacities->numel() == n, "v_opacities must match opacities");
-    const xsg_stream_t s = stream_of(scales);
-    const auto d = drop_desc(p, seed, seed_at, stream, scales.device());
-    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(scales.device());
-    Tensor v_log_scales, v_logits;
-    if (v_scales.has_value()) v_log_scales = at::empty_like(scales);
-    if (v_opacities.has_value()) v_logits = at::empty_like(opacity_logits);
-    check_rc(xsg_activate_drop_bwd(&d, n, fptr(scales), fptr(opacity_logits), fptr(v_scales), fptr(v_opacities),
-                                   v_scales.has_value() ? v_log_scales.data_ptr<float>() : nullptr,
-                                   v_opacities.has_value() ? v_logits.data_ptr<float>() : nullptr, s));
-    return {v_log_scales, v_logits};
+std::tuple<Tensor, Tensor> activate_drop(const Tensor& log_scales, const Tensor& opacity_logits, double p, int64_t seed,
+                                         const OptT& seed_at, int64_t stream) {
+    const auto out = ActivateDrop::apply(log_scales, opacity_logits, seed_at, p, seed, stream);
+    return {out[0], out[1]};
 }
 
 // The description of a call and what it points to (a strided x whose pixels do not follow each other at one
@@ -1192,38 +1260,63 @@ struct NormCall {
     }
 };
 
-std::tuple<Tensor, Tensor> group_norm_act_fwd(const Tensor& x, int64_t groups, const OptT& weight, const OptT& bias,
-                                              int64_t act, double eps, const OptT& mask, double p, int64_t seed,
-                                              const OptT& seed_at, int64_t stream) {
-    const NormCall c(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream);
+std::tuple<Tensor, Tensor> group_norm_values(const NormCall& c, const Tensor& x) {
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
     Tensor y = at::empty(x.sizes(), x.options());
-    Tensor stats = at::empty({c.d.batch, groups, 4}, x.options().dtype(at::kFloat));
+    Tensor stats = at::empty({c.d.batch, c.d.groups, 4}, x.options().dtype(at::kFloat));
     const Tensor ws = workspace(x, xsg_group_norm_act_workspace_bytes(&c.d, 0));
     check_rc(xsg_group_norm_act_fwd(&c.d, y.data_ptr(), stats.data_ptr<float>(), ws.data_ptr(), stream_of(x)));
     return {y, stats};
 }
 
-std::tuple<OptT, OptT, OptT> group_norm_act_bwd(const Tensor& v_y, const Tensor& stats, const Tensor& x, int64_t groups,
-                                                const OptT& weight, const OptT& bias, int64_t act, double eps,
-                                                const OptT& mask, double p, int64_t seed, const OptT& seed_at,
-                                                int64_t stream, bool need_x, bool need_weight, bool need_bias) {
-    const NormCall c(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream);
-    check_same_device({x, v_y, stats});
-    all_contiguous({v_y, stats});
-    TORCH_CHECK(v_y.sizes() == x.sizes() && v_y.scalar_type() == x.scalar_type(), "v_y must have x's sizes and type");
-    check_f32(stats, "stats");
-    TORCH_CHECK(stats.numel() == c.d.batch * groups * 4, "stats must be the forward's");
-    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
-    OptT v_x, v_weight, v_bias;
-    if (need_x) v_x = at::empty(x.sizes(), x.options());
-    if (need_weight) v_weight = at::empty({x.size(-1)}, x.options().dtype(at::kFloat));
-    if (need_bias) v_bias = at::empty({x.size(-1)}, x.options().dtype(at::kFloat));
-    const Tensor ws = workspace(x, xsg_group_norm_act_workspace_bytes(&c.d, 1));
-    check_rc(xsg_group_norm_act_bwd(&c.d, stats.data_ptr<float>(), v_y.data_ptr(), v_x ? v_x->data_ptr() : nullptr,
-                                    v_weight ? v_weight->data_ptr<float>() : nullptr,
-                                    v_bias ? v_bias->data_ptr<float>() : nullptr, ws.data_ptr(), stream_of(x)));
-    return {v_x, v_weight, v_bias};
+struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptT& weight, const OptT& bias,
+                          const OptT& mask, const OptT& seed_at, int64_t groups, int64_t act, double eps, double p,
+                          int64_t seed, int64_t stream) {
+        const NormCall c(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream);
+        const auto [y, stats] = group_norm_values(c, x);
+        keep_draws(ctx, p, seed, stream);
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["eps"] = eps;
+        ctx->save_for_backward({x, defined_or_not(weight), defined_or_not(bias), defined_or_not(mask), defined_or_not(seed_at), stats});
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const KeptDraws k(ctx);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[5];
+        const NormCall c(x, ctx->saved_data["groups"].toInt(), optional(weight), optional(bias), ctx->saved_data["act"].toInt(),
+                         ctx->saved_data["eps"].toDouble(), optional(saved[3]), k.p, k.seed, optional(saved[4]), k.stream);
+        const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+        const Tensor v_y = grads[0].contiguous();
+        TORCH_CHECK(v_y.scalar_type() == x.scalar_type(), "the gradient must be of x's type");
+        Tensor v_x, v_weight, v_bias;
+        const auto floats = x.options().dtype(at::kFloat);
+        if (ctx->needs_input_grad(0)) v_x = at::empty(x.sizes(), x.options());
+        // inputs that are not there have no number
+        if (weight.defined() && ctx->needs_input_grad(1)) v_weight = at::empty({x.size(-1)}, floats);
+        if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1)) v_bias = at::empty({x.size(-1)}, floats);
+        const Tensor ws = workspace(x, xsg_group_norm_act_workspace_bytes(&c.d, 1));
+        check_rc(xsg_group_norm_act_bwd(&c.d, stats.data_ptr<float>(), v_y.data_ptr(), v_x.defined() ? v_x.data_ptr() : nullptr,
+                                        v_weight.defined() ? v_weight.data_ptr<float>() : nullptr,
+                                        v_bias.defined() ? v_bias.data_ptr<float>() : nullptr, ws.data_ptr(), stream_of(x)));
+        if (v_weight.defined()) v_weight = v_weight.to(weight.scalar_type());
+        if (v_bias.defined()) v_bias = v_bias.to(bias.scalar_type());
+        variable_list out(11);
+        out[0] = v_x;
+        out[1] = v_weight;
+        out[2] = v_bias;
+        return differentiated_once(std::move(out), "group_norm_act", x, weight, bias, grads[0]);
+    }
+};
+
+Tensor group_norm_act(const Tensor& x, int64_t groups, const OptT& weight, const OptT& bias, int64_t act, double eps,
+                      const OptT& mask, double p, int64_t seed, const OptT& seed_at, int64_t stream) {
+    const OptT ox(x);
+    if (wants_grad({&ox, &weight, &bias}))
+        return GroupNormAct::apply(x, weight, bias, mask, seed_at, groups, act, eps, p, seed, stream);
+    return std::get<0>(group_norm_values(NormCall(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream), x));
 }
 
 Tensor packed_mask_from_instances(const Tensor& instance_ids, const Tensor& instance_mask) {
@@ -1846,22 +1939,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adam_step_", &adam_step_, py::arg("params"), py::arg("grads"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"),
           py::arg("step"), py::arg("lr"), py::arg("weight_decay"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
           py::arg("max_norm"), py::arg("norm_type"), py::arg("skip_nonfinite"), py::arg("masks"));
-    const auto none = py::none();
-    m.def("dropout", &dropout, py::arg("x"), py::arg("p"), py::arg("seed"), py::arg("seed_at") = none, py::arg("stream") = 0,
-          py::arg("shared") = 1);
+    m.def("dropout", &dropout, py::arg("x"), py::arg("p"), py::arg("seed"), py::arg("seed_at"), py::arg("stream"),
+          py::arg("shared"));
     m.def("drop_mask", &drop_mask, py::arg("n"), py::arg("p"), py::arg("seed"), py::arg("seed_at"), py::arg("stream"),
           py::arg("device"));
-    m.def("activate_drop_fwd", &activate_drop_fwd, py::arg("log_scales"), py::arg("opacity_logits"), py::arg("p"),
-          py::arg("seed"), py::arg("seed_at") = none, py::arg("stream") = 0);
-    m.def("activate_drop_bwd", &activate_drop_bwd, py::arg("scales"), py::arg("opacity_logits"), py::arg("v_scales"),
-          py::arg("v_opacities"), py::arg("p"), py::arg("seed"), py::arg("seed_at") = none, py::arg("stream") = 0);
-    m.def("group_norm_act_fwd", &group_norm_act_fwd, py::arg("x"), py::arg("groups"), py::arg("weight"), py::arg("bias"),
+    m.def("activate_drop", &activate_drop, py::arg("log_scales"), py::arg("opacity_logits"), py::arg("p"), py::arg("seed"),
+          py::arg("seed_at"), py::arg("stream"));
+    m.def("group_norm_act", &group_norm_act, py::arg("x"), py::arg("groups"), py::arg("weight"), py::arg("bias"),
           py::arg("act"), py::arg("eps"), py::arg("mask"), py::arg("p"), py::arg("seed"), py::arg("seed_at"),
           py::arg("stream"));
-    m.def("group_norm_act_bwd", &group_norm_act_bwd, py::arg("v_y"), py::arg("stats"), py::arg("x"), py::arg("groups"),
-          py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("eps"), py::arg("mask"), py::arg("p"),
-          py::arg("seed"), py::arg("seed_at"), py::arg("stream"), py::arg("need_x"), py::arg("need_weight"),
-          py::arg("need_bias"));
     m.def("activate_fwd", &activate_fwd, py::arg("log_scales"), py::arg("opacity_logits"));
     m.def("activate_bwd", &activate_bwd, py::arg("scales"), py::arg("opacities"), py::arg("v_scales"),
           py::arg("v_opacities"));

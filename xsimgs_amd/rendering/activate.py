@@ -30,28 +30,6 @@ class _Activate(torch.autograd.Function):
                             None if v_opacities is None else v_opacities.contiguous())
 
 
-class _ActivateDrop(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, log_scales, opacity_logits, seed_at, p, seed, stream):
-        ctx.set_materialize_grads(False)
-        ctx.args = p, seed, stream
-        opacity_logits = opacity_logits.contiguous()
-        scales, opacities = _C.activate_drop_fwd(log_scales.contiguous(), opacity_logits, p, seed, seed_at, stream)
-        ctx.save_for_backward(scales, opacity_logits, seed_at)
-        return scales, opacities
-
-    @staticmethod
-    def backward(ctx, v_scales, v_opacities):
-        scales, opacity_logits, seed_at = ctx.saved_tensors
-        p, seed, stream = ctx.args
-        v_scales = v_scales.contiguous() if v_scales is not None and ctx.needs_input_grad[0] else None
-        v_opacities = v_opacities.contiguous() if v_opacities is not None and ctx.needs_input_grad[1] else None
-        grads = (None, None)
-        if v_scales is not None or v_opacities is not None:
-            grads = _C.activate_drop_bwd(scales, opacity_logits, v_scales, v_opacities, p, seed, seed_at, stream)
-        return (*grads, None, None, None, None)
-
-
 def activate_gaussians(log_scales: torch.Tensor, opacity_logits: torch.Tensor, *, drop: float = 0.0, seed=0,
                        stream: int = 0):
     """(exp(log_scales), sigmoid(opacity_logits)); log_scales holds three values per opacity logit
@@ -61,4 +39,4 @@ def activate_gaussians(log_scales: torch.Tensor, opacity_logits: torch.Tensor, *
     seed, seed_at = seed_arguments(seed)
     if drop == 0:
         return _Activate.apply(log_scales, opacity_logits)
-    return _ActivateDrop.apply(log_scales, opacity_logits, seed_at, float(drop), seed, stream)
+    return _C.activate_drop(log_scales, opacity_logits, float(drop), seed, seed_at, stream)

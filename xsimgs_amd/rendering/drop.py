@@ -6,7 +6,6 @@ read (a captured graph then draws anew on each replay if the value is changed in
 and its backward, which autograd refuses). ``stream``: a number in [0, 2^31), another for each place that
 draws under one seed. Probabilities count in steps of 2^-32; what is kept is divided by the share that is kept."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _C
 
@@ -18,20 +17,6 @@ def seed_arguments(seed):
     if isinstance(seed, bool) or not isinstance(seed, int) or not 0 <= seed < 1 << 63:
         raise ValueError(f"seed must be an int in [0, 2^63) or an int64 tensor of one value, not {seed!r}")
     return seed, None
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, seed_at, p, seed, stream, shared):
-        ctx.args = p, seed, stream, shared
-        ctx.save_for_backward(seed_at)
-        return _C.dropout(x.contiguous(), p, seed, seed_at, stream, shared)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, v_y):
-        p, seed, stream, shared = ctx.args
-        return _C.dropout(v_y.contiguous(), p, seed, ctx.saved_tensors[0], stream, shared), None, None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed, *, stream: int = 0, shared: int = 0) -> torch.Tensor:
@@ -47,9 +32,7 @@ def dropout(x: torch.Tensor, p: float, seed, *, stream: int = 0, shared: int = 0
     seed, seed_at = seed_arguments(seed)
     if p == 0:
         return x
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Dropout.apply(x, seed_at, float(p), seed, stream, max(row, 1))
-    return _C.dropout(x.contiguous(), float(p), seed, seed_at, stream, max(row, 1))
+    return _C.dropout(x, float(p), seed, seed_at, stream, max(row, 1))
 
 
 def drop_mask(n: int, drop: float, seed, *, stream: int = 0, device=None) -> torch.Tensor:

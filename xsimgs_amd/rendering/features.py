@@ -1,32 +1,11 @@
 """Group norm with an activation and dropout over rendered feature images, channels last as the compositor writes
 them: what a network that decodes them starts each of its blocks with. An extension of this build."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _C
 from .drop import seed_arguments
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, mask, seed_at, groups, act, eps, p, seed, stream):
-        y, stats = _C.group_norm_act_fwd(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream)
-        ctx.args = groups, act, eps, p, seed, stream
-        ctx.save_for_backward(x, weight, bias, mask, seed_at, stats)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, v_y):
-        x, weight, bias, mask, seed_at, stats = ctx.saved_tensors
-        groups, act, eps, p, seed, stream = ctx.args
-        v_x, v_weight, v_bias = _C.group_norm_act_bwd(
-            v_y.contiguous(), stats, x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream,
-            *ctx.needs_input_grad[:3])
-        return (v_x, None if v_weight is None else v_weight.to(weight.dtype),
-                None if v_bias is None else v_bias.to(bias.dtype)) + (None,) * 8
 
 
 def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, *, act: str = "silu", eps: float = 1e-5,
@@ -42,11 +21,7 @@ def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, *, act:
     if act not in ACTIVATIONS:
         raise ValueError(f"act must be one of {', '.join(ACTIVATIONS)}, not {act!r}")
     seed, seed_at = seed_arguments(seed)
-    args = int(groups), ACTIVATIONS[act], float(eps), float(drop), seed, stream
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _GroupNormAct.apply(x, weight, bias, mask, seed_at, *args)
-    groups, act, eps, p, seed, stream = args
-    return _C.group_norm_act_fwd(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream)[0]
+    return _C.group_norm_act(x, groups, weight, bias, ACTIVATIONS[act], eps, mask, drop, seed, seed_at, stream)
 
 
 class FeatureNorm(torch.nn.Module):
