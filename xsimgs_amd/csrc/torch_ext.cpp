@@ -1160,8 +1160,8 @@ Tensor dropout(const Tensor& x, double p, int64_t seed, const OptT& seed_at, int
 Tensor drop_mask(int64_t n, double p, int64_t seed, const OptT& seed_at, int64_t stream, const c10::Device& device) {
     TORCH_CHECK(n >= 0, "n must not be negative");
     TORCH_CHECK(device.is_cuda(), "xsimgs_amd ops take GPU tensors (got the device ", device, ")");
-    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(device);
     Tensor out = at::empty({(n + 31) / 32}, at::TensorOptions().device(device).dtype(at::kUInt32));
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(out.device());
     const auto d = drop_desc(p, seed, seed_at, stream, out.device());
     check_rc(xsg_drop_mask(&d, n, (uint32_t*)out.data_ptr(), stream_of(out)));
     return out;

@@ -17,9 +17,10 @@ from dataclasses import dataclass, field
 import torch
 
 from . import cameras as C
-from ._C import isect_regular_tiles_batched, packed_visibility_mask
+from ._C import isect_regular_tiles_batched, mask_radii_packed, packed_visibility_mask
 from .optim import Adam
 from .rendering.activate import activate_gaussians
+from .rendering.drop import drop_mask
 from .rendering.rasterize import ut_gs_rasterize, ut_gs_rasterize_batched
 from .rendering.render import ut_gs_tiling
 from .rendering.sh import spherical_harmonics_fused
@@ -36,6 +37,7 @@ class FrameState:
     sh: torch.Tensor | None
     colors: torch.Tensor | None
     cams: list = field(default_factory=list)
+    head: torch.nn.Module | None = None   # a rendering.FeatureNorm over the composited features
 
 
 def make_camera(spec, device) -> C.FusedRSCamera:
@@ -55,7 +57,8 @@ def make_camera(spec, device) -> C.FusedRSCamera:
     return C.LidarCamera(pose, torch.tensor(spec.impl), spec.beam_v)
 
 
-def prepare(scene, device, requires_grad: bool = True) -> FrameState:
+def prepare(scene, device, requires_grad: bool = True, head=None) -> FrameState:
+    """``head``: a ``rendering.FeatureNorm`` over the scene's channels, through which each frame's features go."""
     def leaf(t):
         if t is None:
             return None
@@ -64,29 +67,52 @@ def prepare(scene, device, requires_grad: bool = True) -> FrameState:
     st = FrameState(scene, torch.device(device), leaf(scene.means), leaf(scene.log_scales), leaf(scene.quats),
                     leaf(scene.opacity_logits), leaf(scene.sh_coeffs), leaf(scene.colors))
     st.cams = [make_camera(spec, device) for spec in scene.cameras]
+    st.head = head.to(device) if head is not None else None
     return st
 
 
-def render_frame(st: FrameState, backward: bool = False, grads=None, cam_index: int = 0) -> dict:
+def _drawn(st: FrameState, drop: float, seed):
+    """Activated scales and opacities with a share of the Gaussians dropped, and the packed mask of those kept
+    (None where nothing is dropped)."""
+    scales, opac = activate_gaussians(st.log_scales, st.opacity_logits, drop=drop, seed=seed)
+    return scales, opac, drop_mask(st.means.shape[0], drop, seed, device=st.device) if drop > 0 else None
+
+
+def _headed(st: FrameState, rgb, out: dict, seed):
+    """The image that a frame's gradient goes to: the head's features where there is one, [C, H, W, ch] as rgb."""
+    if st.head is None:
+        return rgb
+    batched = rgb if rgb.dim() == 4 else rgb.unsqueeze(0)
+    out["features"] = st.head(batched, seed=seed).view(rgb.shape)
+    return out["features"]
+
+
+def render_frame(st: FrameState, backward: bool = False, grads=None, cam_index: int = 0, *, drop: float = 0.0,
+                 seed=0) -> dict:
+    """``drop``: each Gaussian is left out of the frame with this probability and the others' opacities are divided by the
+    share kept (``rendering.activate_gaussians``); ``out["kept"]`` is the packed mask of those kept. ``seed``: another
+    one for each step, as for ``rendering.dropout``; a head in training mode draws under it too. With a head the colour
+    gradient is that of ``out["features"]``."""
     sc = st.scene
     spec = sc.cameras[cam_index]
     cam = st.cams[cam_index]
-    scales, opac = activate_gaussians(st.log_scales, st.opacity_logits)
+    scales, opac, kept = _drawn(st, drop, seed)
     tsx, tsy = sc.tile_size
     with cam._freeze_ctx():
         ray_o, ray_d = cam.camera_rays(spec.width, spec.height, normalized_rays=True, return_origins=True,
                                        world_space=True)
         tiles = ut_gs_tiling(cam, st.means, scales, st.quats, spec.width, spec.height, opacity=opac,
-                             tile_size_x=tsx, tile_size_y=tsy, use_phm=sc.use_phm)
+                             packed_particle_mask=kept, tile_size_x=tsx, tile_size_y=tsy, use_phm=sc.use_phm)
         colors = _colors(st, cam.pose.t, tiles["radii"] if spec.kind in REGULAR_TILING else None)
         rgb, depth, alpha = ut_gs_rasterize(st.means, st.quats, scales, opac, colors, ray_o, ray_d,
                                             tiles["isect_offsets"], tiles["flatten_ids"], tsx, tsy)
     out = dict(rgb=rgb, depth=depth, alpha=alpha, colors=colors, ray_o=ray_o, ray_d=ray_d,
                offsets=tiles["isect_offsets"], flatten_ids=tiles["flatten_ids"], radii=tiles["radii"],
-               means2d=tiles["means2d"], depths=tiles["depth"])
+               means2d=tiles["means2d"], depths=tiles["depth"], kept=kept)
+    image = _headed(st, rgb, out, seed)
     if backward:
         g_rgb, g_depth, g_alpha = [g.to(st.device) for g in grads]
-        torch.autograd.backward([rgb, depth, alpha], [g_rgb, g_depth, g_alpha])
+        torch.autograd.backward([image, depth, alpha], [g_rgb, g_depth, g_alpha])
         out["grads"] = dict(means=st.means.grad, quats=st.quats.grad, log_scales=st.log_scales.grad,
                             opacity_logits=st.opacity_logits.grad,
                             sh=st.sh.grad if st.sh is not None else None,
@@ -110,19 +136,20 @@ def rig_shares_origin(st: FrameState) -> bool:
     return len({tuple(float(x) for x in s.t) for s in st.scene.cameras}) == 1
 
 
-def render_rig(st: FrameState, backward: bool = False, grads=None) -> dict:
+def render_rig(st: FrameState, backward: bool = False, grads=None, *, drop: float = 0.0, seed=0) -> dict:
     """Every camera of a rig in one batched pass (an extension of this build; the reference's caller
     renders one camera per call, render.py:85-187). Per camera the UT projection and the rays, as
     in render_frame; then one batched binning (keys carry the camera above the tile bits), one
     compositor launch per pass over all cameras' tiles and, when the cameras share their origin,
     one SH evaluation whose colours every camera uses (its gradient sums over the cameras).
-    grads: ([C, H, W, ch], [C, H, W], [C, H, W]) image gradients."""
+    grads: ([C, H, W, ch], [C, H, W], [C, H, W]) image gradients. drop, seed and a head as in render_frame; the
+    same Gaussians are dropped for every camera."""
     sc = st.scene
     specs = sc.cameras
     if not rig_batchable(st):
         raise ValueError("render_rig takes a static rig of regular-tiling cameras of one image size")
     W, H = specs[0].width, specs[0].height
-    scales, opac = activate_gaussians(st.log_scales, st.opacity_logits)
+    scales, opac, kept = _drawn(st, drop, seed)
     if st.sh is None:
         colors = st.colors
     elif rig_shares_origin(st):
@@ -160,16 +187,20 @@ def render_rig(st: FrameState, backward: bool = False, grads=None) -> dict:
             for c, cam in enumerate(st.cams):
                 cam.ut_gs_projection(st.means, scales, st.quats, W, H, opacity=opac, use_phm=sc.use_phm,
                                      out=(flags[c], radii[c], means2d[c], depths[c]))
+        if kept is not None:
+            for c in range(C):
+                mask_radii_packed(kept, radii[c])
         offsets = torch.empty((len(specs), nty, ntx), dtype=torch.int32, device=st.device)
         _, _, flatten_ids = isect_regular_tiles_batched(means2d, radii, depths, W, H, tsx, tsy, sort=True,
                                                         tile_offsets=offsets, keys=False)
     rgb, depth, alpha = ut_gs_rasterize_batched(st.means, st.quats, scales, opac, colors, ray_o, ray_d, offsets,
                                                 flatten_ids, tsx, tsy)
     out = dict(rgb=rgb, depth=depth, alpha=alpha, colors=colors, ray_o=ray_o, ray_d=ray_d, offsets=offsets,
-               flatten_ids=flatten_ids, radii=radii, means2d=means2d, depths=depths)
+               flatten_ids=flatten_ids, radii=radii, means2d=means2d, depths=depths, kept=kept)
+    image = _headed(st, rgb, out, seed)
     if backward:
         g_rgb, g_depth, g_alpha = [g.to(st.device) for g in grads]
-        torch.autograd.backward([rgb, depth, alpha], [g_rgb, g_depth, g_alpha])
+        torch.autograd.backward([image, depth, alpha], [g_rgb, g_depth, g_alpha])
         out["grads"] = dict(means=st.means.grad, quats=st.quats.grad, log_scales=st.log_scales.grad,
                             opacity_logits=st.opacity_logits.grad,
                             sh=st.sh.grad if st.sh is not None else None,
@@ -191,29 +222,35 @@ def _colors(st: FrameState, origin, radii=None):
 
 # learning rates of a scene's parameters (the SH rate serves fixed colours too)
 RATES = dict(means=1.6e-4, quats=1e-3, log_scales=5e-3, opacity_logits=5e-2, sh=2.5e-3, colors=2.5e-3)
+HEAD_RATE = 1e-3
 
 
 def make_optimizer(st: FrameState, rates=None, **kw) -> Adam:
-    """An Adam over the scene's parameters, one group for each with its own rate; ``kw``: max_norm,
-    skip_nonfinite and the other arguments of ``optim.Adam``."""
+    """An Adam over the scene's parameters, one group for each with its own rate, and the head's (``head``); ``kw``:
+    max_norm, skip_nonfinite and the other arguments of ``optim.Adam``."""
     rates = dict(RATES, **(rates or {}))
-    return Adam([dict(params=[getattr(st, k)], lr=r, name=k) for k, r in rates.items() if getattr(st, k) is not None],
-                **kw)
+    head_rate = rates.pop("head", HEAD_RATE)
+    groups = [dict(params=[getattr(st, k)], lr=r, name=k) for k, r in rates.items() if getattr(st, k) is not None]
+    if st.head is not None:
+        groups.append(dict(params=list(st.head.parameters()), lr=head_rate, name="head"))
+    return Adam(groups, **kw)
 
 
-def train_frame(st: FrameState, optimizer: Adam, grads, cam_index: int = 0, rig: bool = False) -> dict:
+def train_frame(st: FrameState, optimizer: Adam, grads, cam_index: int = 0, rig: bool = False, *, drop: float = 0.0,
+                seed=0) -> dict:
     """One training step: the frame (of one camera, or of the whole rig) forward and backward, then the
     optimizer's update with whatever clipping it carries. In a regular tiling only the Gaussians that some
     tile can hold are updated (their packed mask from the projection's radii; the others' gradients are
     zeros, their momentum rests). Parameters beside the scene's (a pose, an exposure) are updated whole, from
     what the frame's backward and the caller's own before this call gave them; these gradients count for one
-    step and are cleared behind it. Returns the frame's outputs and ``grad_norm`` before clipping."""
+    step and are cleared behind it. ``drop`` and ``seed`` as in ``render_frame``; dropped Gaussians keep their parameters
+    and momentum, in every tiling. Returns the frame's outputs and ``grad_norm`` before clipping."""
     zero_grads(st)
     if rig:
-        out = render_rig(st, backward=True, grads=grads)
+        out = render_rig(st, backward=True, grads=grads, drop=drop, seed=seed)
     else:
-        out = render_frame(st, backward=True, grads=grads, cam_index=cam_index)
-    masks = None
+        out = render_frame(st, backward=True, grads=grads, cam_index=cam_index, drop=drop, seed=seed)
+    masks = None if out["kept"] is None else {t: out["kept"] for t in _leaves(st)}
     if rig or st.scene.cameras[cam_index].kind in REGULAR_TILING:
         mask = packed_visibility_mask(out["radii"].detach().contiguous())
         masks = {t: mask for t in _leaves(st)}

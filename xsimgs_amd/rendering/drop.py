@@ -41,7 +41,4 @@ def drop_mask(n: int, drop: float, seed, *, stream: int = 0, device=None) -> tor
     seed, seed_at = seed_arguments(seed)
     if device is None:
         device = seed_at.device if seed_at is not None else "cuda"
-    device = torch.device(device)
-    if device.type == "cuda" and device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    return _C.drop_mask(n, float(drop), seed, seed_at, stream, device)
+    return _C.drop_mask(n, float(drop), seed, seed_at, stream, torch.device(device))

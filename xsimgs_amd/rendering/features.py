@@ -27,10 +27,10 @@ def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, *, act:
 class FeatureNorm(torch.nn.Module):
     """``group_norm_act`` with its weight and bias, for ``frame.prepare(..., head=)`` and networks behind the
     compositor. Dropout acts in training mode only and takes the call's ``seed``; ``stream`` tells modules apart
-    that share one."""
+    that share one (0 is the frame's Gaussians')."""
 
     def __init__(self, groups: int, channels: int, act: str = "silu", eps: float = 1e-5, drop: float = 0.0, *,
-                 stream: int = 0, device=None, dtype=None):
+                 stream: int = 1, device=None, dtype=None):
         super().__init__()
         if act not in ACTIVATIONS or groups < 1 or channels % groups or not 0.0 <= drop <= 1.0:
             raise ValueError(f"FeatureNorm takes an activation ({', '.join(ACTIVATIONS)}), groups that divide the channels "

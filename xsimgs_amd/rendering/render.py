@@ -6,7 +6,7 @@ compositor, in the reference's order.
 """
 import torch
 
-from .._C import mask_radii, eval3d_supported_ndims
+from .._C import mask_radii, mask_radii_packed, eval3d_supported_ndims
 from .rasterize import ut_gs_rasterize
 from .rasterize_dynamic import ut_gs_dynamic_rasterize
 
@@ -19,7 +19,9 @@ def ut_gs_tiling(camera, points, scale, rotation, width: int, height: int, point
             points=points, points_velocity=points_velocity, scale=scale, rotation=rotation, opacity=opacity,
             width=width, height=height, ut_alpha=ut_alpha, ut_beta=ut_beta, ut_kappa=ut_kappa, use_phm=use_phm)
         if packed_particle_mask is not None:
-            mask_radii(packed_particle_mask, radii)
+            # the reference's call takes one byte per Gaussian; words (uint32) are packed_visibility_mask's layout
+            by_words = packed_particle_mask.dtype == torch.uint32
+            (mask_radii_packed if by_words else mask_radii)(packed_particle_mask, radii)
         n_tiles_width = (width + tile_size_x - 1) // tile_size_x
         n_tiles_height = (height + tile_size_y - 1) // tile_size_y
         # the sorted fill writes the tile offsets that isect_offset_encode would compute from its keys, so
