@@ -60,9 +60,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a, con
     for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
         const bool more = p + at.jump < a.pixels;
         if (AHEAD && more) next.fetch(a, at, x_at, g_at, p + at.jump);
+        NormDraws<V> drawn{draws, a.channels, first + p * a.channels, (int64_t)a.ty * a.channels, 0};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t keep = DROP ? norm_keep<V>(draws, a.channels, first + (p + u * a.ty) * a.channels) : 0;
+            const uint32_t keep = DROP ? drawn(u) : 0;
             if (!(now.in >> (16 + u) & 1)) continue;
             float x[V], g[V];
             unpack<DT, V>(now.x[u], x);
@@ -71,11 +72,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a, con
             for (int j = 0; j < V; ++j) {
                 const float e = x[j] - mean[j];
                 float dz = g[j] * norm_act_slope<ACT, EXACT>(e * scale[j] + bias[j]);
-                if (DROP) dz = keep_bit(dz * a.drop.factor, keep, j);
+                if (DROP) dz = keep_bit(dz, keep, j);   // the factor comes at the end
                 s1[j] += dz;
                 s2[j] += dz * e;
             }
-            if (DROP) __builtin_amdgcn_sched_barrier(0);
+            if (DROP) __builtin_amdgcn_sched_barrier(0);   // several pixels' draws at once take too many registers
         }
         if (!more) break;
         if (AHEAD) now = next;
@@ -94,8 +95,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a, con
                 sum.x += e.x;
                 sum.y += e.y;
             }
-            sum.x = segment_sum(sum.x, l);
-            sum.y = segment_sum(sum.y, l) * stats[at.b * a.groups + a.by_cg(c)].y;
+            sum.x = segment_sum(sum.x, l) * a.drop.factor;
+            sum.y = segment_sum(sum.y, l) * stats[at.b * a.groups + a.by_cg(c)].y * a.drop.factor;
             if (lane == 0) {
                 if (channels) channels[(int64_t)blockIdx.x * a.channels + c] = sum;
                 const float w = norm_param(a.weight, a.weight_dtype, c, 1.0f);
@@ -230,9 +231,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_kernel(NormArgs a, int
     for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
         const bool more = p + at.jump < a.pixels;
         if (AHEAD && more) next.fetch(a, at, x_at, g_at, p + at.jump);
+        NormDraws<V> drawn{draws, a.channels, first + p * a.channels, (int64_t)a.ty * a.channels, 0};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t keep = DROP ? norm_keep<V>(draws, a.channels, first + (p + u * a.ty) * a.channels) : 0;
+            const uint32_t keep = DROP ? drawn(u) : 0;
             if (!(now.in >> u & 1)) continue;
             Raw<V * ElementSize<DT>::value> out = {};
             if (!MASK || (now.in >> (16 + u) & 1)) {

@@ -271,9 +271,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, in
     for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
         const bool more = p + at.jump < a.pixels;
         if (AHEAD && more) in_next = fetch(p + at.jump, next);
+        NormDraws<V> drawn{draws, a.channels, first + p * a.channels, (int64_t)a.ty * a.channels, 0};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t keep = DROP ? norm_keep<V>(draws, a.channels, first + (p + u * a.ty) * a.channels) : 0;
+            const uint32_t keep = DROP ? drawn(u) : 0;
             if (!(in >> u & 1)) continue;
             Vec out = {};
             if (!MASK || (in >> (16 + u) & 1)) {
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, in
                 out = pack<DT, V>(x);
             }
             store_raw<DT, V, STREAM>(y_at(p + u * a.ty), 0, out);
-            if (DROP) __builtin_amdgcn_sched_barrier(0);   // draws of several pixels at once take too many registers
+            if (DROP) __builtin_amdgcn_sched_barrier(0);   // several pixels' draws at once take too many registers
         }
         if (!more) break;
         if (AHEAD) {
@@ -312,10 +313,15 @@ constexpr int64_t kCacheBytes = (int64_t)128 << 20;
 }  // namespace
 
 int norm_vector(const xsg_norm_desc* d, bool draws) {
-    // vectors of 16 bytes; eight float32 where there are draws, which come eight at a time, or too many channels
-    if (d->dtype != XSG_DTYPE_F32) return d->channels >= 8 ? 8 : d->channels >= 4 ? 4 : 1;
-    if (d->channels > 4 * kNormThreads || (draws && d->drop.p > 0.0 && d->channels >= 8)) return 8;
-    return d->channels >= 4 ? 4 : 1;
+    const int c = d->channels;
+    if (d->dtype != XSG_DTYPE_F32) return c >= 8 ? 8 : c >= 4 ? 4 : 1;
+    if (c > 4 * kNormThreads) return 8;   // a workgroup would not have the threads
+    // With draws: a wavefront's vectors of four lie in 32 blocks of draws where the channels are a multiple of eight, or
+    // where the vectors overlap by enough (65 channels, 17 M values: 125 us the three passes, 132 with vectors of eight);
+    // else some lane needs a 33rd, and eight are better (513 channels, 246 M values: 1390 and 1800 us)
+    const int vectors = (c + 3) / 4;
+    if (draws && d->drop.p > 0.0 && c >= 8 && c % 8 != 0 && 64 * (4 * vectors - c) < 8 * vectors) return 8;
+    return c >= 4 ? 4 : 1;
 }
 
 int norm_args(const xsg_norm_desc* d, NormArgs& a, const char* who) {

@@ -140,11 +140,27 @@ template <int U, bool MASK, int V> XSG_DEV uint32_t norm_pixels(const NormArgs& 
     return in;
 }
 
-// A vector's draws: bit j for element first + j. Every lane of the wavefront comes here, in the order of their elements.
-template <int V> XSG_DEV uint32_t norm_keep(const Draws& draws, int channels, int64_t first) {
-    if (V < 8) return draws.keep((uint64_t)first, V);
-    return channels % 8 == 0 ? draws.keep8((uint64_t)first >> 3) : draws.keep_in_order((uint64_t)first);
-}
+// A thread's draws: bit j for element first + j of pixel u of a batch. Every lane of the wavefront comes here for every
+// pixel, in the order of their elements. With vectors of four, two pixels' draws come at once.
+template <int V> struct NormDraws {
+    const Draws& draws;
+    int channels;
+    int64_t first, step;   // element of the batch's first pixel, and from pixel to pixel
+    uint32_t next;
+    XSG_DEV uint32_t operator()(int u) {
+        const int64_t e = first + u * step;
+        uint32_t keep;
+        if (V == 8) {
+            keep = channels % 8 == 0 ? draws.keep8((uint64_t)e >> 3) : draws.keep_in_order((uint64_t)e);
+        } else if (V == 4) {
+            if (u % 2) return next;
+            draws.keep_in_order((uint64_t)e, (uint64_t)(e + step), keep, next);
+        } else {
+            keep = draws.keep((uint64_t)e, V);
+        }
+        return keep;
+    }
+};
 
 // Statistics of a sample's groups lie in `part` (mean and squared deviations of each chunk) and `counts` (elements of
 // a group in each); up to this many pairs the next launch's workgroups each join them themselves (8 bytes each, from

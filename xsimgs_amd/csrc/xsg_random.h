@@ -95,21 +95,33 @@ struct Draws {
         if (at + n > 8) bits |= keep8((first >> 3) + 1) << 8;
         return bits >> at;
     }
-    // keep(first, 8) where the lanes of a wavefront, all of them here, hold runs in order that together lie in about 64
-    // blocks: lane i draws the i-th of them, and each takes its two from the lanes that have them.
-    XSG_DEV uint32_t keep_in_order(uint64_t first) const {
-        const uint64_t mine = first >> 3;
-        const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)mine) |
-                              (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(mine >> 32)) << 32;
-        const uint32_t drawn = keep8(base + __lane_id());
-        const uint64_t from = mine - base;
-        uint32_t bits = __shfl(drawn, (int)(from & 63)) | __shfl(drawn, (int)((from + 1) & 63)) << 8;
+    // Bits from value first on (eight, or four where they need not reach further) for two sets of runs, in each of which the
+    // lanes of a wavefront, all of them here, hold runs of eight (four) in order, next to each other or overlapping: they
+    // lie in about 64 (32) blocks, so a lane draws one block of the set (half the lanes for each of two sets) and takes its
+    // own two from the lanes that have them.
+    XSG_DEV uint32_t shared_keep(uint64_t first, uint64_t base, uint32_t drawn, int lane0, int lanes, int values) const {
+        const uint64_t mine = first >> 3, from = mine - base;
+        uint32_t bits = __shfl(drawn, lane0 + (int)(from & (lanes - 1))) | __shfl(drawn, lane0 + (int)((from + 1) & (lanes - 1))) << 8;
         // lanes at the end of a wavefront may reach past what it drew
-        if (from > 62) {
-            if (from > 63) bits = keep8(mine) | (bits & 0xff00u);
-            if (first & 7u) bits = (bits & 0xffu) | keep8(mine + 1) << 8;
+        if (from + 2 > (uint64_t)lanes) {
+            if (from >= (uint64_t)lanes) bits = keep8(mine) | (bits & 0xff00u);
+            if ((first & 7u) + values > 8) bits = (bits & 0xffu) | keep8(mine + 1) << 8;
         }
         return bits >> ((uint32_t)first & 7u);
+    }
+    XSG_DEV static uint64_t of_first_lane(uint64_t x) {
+        return (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)x) | (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32;
+    }
+    XSG_DEV uint32_t keep_in_order(uint64_t first) const {
+        const uint64_t base = of_first_lane(first >> 3);
+        return shared_keep(first, base, keep8(base + __lane_id()), 0, 64, 8);
+    }
+    XSG_DEV void keep_in_order(uint64_t first, uint64_t second, uint32_t& a, uint32_t& b) const {
+        const uint64_t base = of_first_lane(first >> 3), base2 = of_first_lane(second >> 3);
+        const uint32_t lane = __lane_id();
+        const uint32_t drawn = keep8((lane < 32 ? base : base2) + (lane & 31));
+        a = shared_keep(first, base, drawn, 0, 32, 4);
+        b = shared_keep(second, base2, drawn, 32, 32, 4);
     }
 };
 
