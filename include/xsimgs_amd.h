@@ -246,7 +246,7 @@ int xsg_activate_bwd(int64_t n, const float* scales, const float* opacities, con
  * T = round(p 2^32); the upper 16 of them are half e % 2 (the lower half first) of word e % 8 / 2 of
  * Philox4x32-10 with the seed's two words (lower first) as key and the counter (lower and upper word of e / 8,
  * stream, 0), the lower 16 the same half and word under the counter (.., .., stream, 1). What is kept is
- * multiplied by 1 / (1 - T / 2^32). XSG_DTYPE_* as below. */
+ * multiplied by 1 / (1 - T / 2^32). XSG_DTYPE_* as in the training step. */
 typedef struct {
     double p;                  /* in [0, 1] */
     uint64_t seed;
@@ -283,7 +283,7 @@ int xsg_activate_drop_bwd(const xsg_drop_desc* drop, int64_t n, const float* sca
 /* Group norm of feature images, channels last, with an activation and dropout behind it: over each sample and
  * each group of channels / groups consecutive channels, with mean and (biased) variance over the pixels in the
  * mask, y = drop(act((x - mean) / sqrt(variance + eps) weight + bias)). Pixels out of the mask are not read; y
- * and v_x are 0 there. */
+ * and v_x are 0 there. Up to 2^23 - 1 workgroups, so no more samples. Results are the same bits on every call. */
 typedef struct {
     int dtype;                        /* of x, y and their gradients */
     int64_t batch, pixels;

@@ -127,6 +127,10 @@ def test_norm_pointers_and_sizes(lib):
         assert lib.xsg_group_norm_act_workspace_bytes(C.byref(e), 0) == 0
         assert lib.xsg_group_norm_act_fwd(C.byref(e), None, None, None, None) == 0
     assert lib.xsg_group_norm_act_bwd(C.byref(d), None, None, None, None, None, None, None) == 0
+    many = _norm(batch=1 << 24, pixels=1, batch_stride=8)
+    for call in (lambda: lib.xsg_group_norm_act_fwd(C.byref(many), P, P, P, None),
+                 lambda: lib.xsg_group_norm_act_bwd(C.byref(many), P, P, P, P, P, P, None)):
+        assert call() == -1 and "too many samples" in lib.xsg_last_error().decode()
     big = _norm(batch=6, pixels=2_073_600, channels=64, groups=8, batch_stride=64 * 2_073_600, pixel_stride=64)
     for backward in (0, 1):
         assert 0 < lib.xsg_group_norm_act_workspace_bytes(C.byref(big), backward) < 4 << 20

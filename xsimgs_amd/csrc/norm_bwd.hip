@@ -6,7 +6,6 @@
 // for each group; a second joins the groups' (its own workgroups do, where they are few) and writes v_x, while
 // some more of its workgroups join the channels'. Sums are added in a fixed order. No reference counterpart.
 #include <algorithm>
-#include <limits.h>
 
 #include "xsg_norm.h"
 
@@ -284,13 +283,14 @@ extern "C" int xsg_group_norm_act_bwd(const xsg_norm_desc* d, const float* stats
     if ((uintptr_t)stats % 16) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: stats must be 16-byte aligned");
     const int vector = norm_vector(d, true), size = d->dtype == XSG_DTYPE_F32 ? 4 : 2;
     norm_layout(a, vector, norm_grad_unroll(vector * size), size, 3, 256);
-    if (a.batch * std::max(a.chunks, a.groups) > INT_MAX / 2) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: too large");
+    const int tiles = (a.channels + 7) / 8;
+    if (a.batch * a.chunks + tiles > kNormBlocks || (!a.join && a.batch * a.groups > kNormBlocks))
+        return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: too many samples (%lld)", (long long)a.batch);
     const int64_t parts = a.batch * a.chunks;
     float2* const groups = (float2*)workspace;
     float2* const channels = groups + parts * a.groups;
     float2* const means = channels + parts * a.channels;
     const bool params = v_weight || v_bias;
-    const int tiles = (a.channels + 7) / 8;
     const float4* const st = (const float4*)stats;
     with_dtype(d->dtype, [&](auto dt) {
         with_vector(vector, [&](auto vec) {

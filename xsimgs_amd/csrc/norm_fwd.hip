@@ -176,7 +176,7 @@ struct NormSums {
     }
 };
 
-// One workgroup to a group of a sample.
+// One workgroup to a group of a sample (1080p x 64: 4.7 us, as long as a launch takes).
 __global__ __launch_bounds__(256) void norm_join_kernel(int groups, int chunks, float eps, const float2* __restrict__ part,
                                                         const float* __restrict__ counts, float4* __restrict__ stats) {
     __shared__ double s_sum[4][4];
@@ -302,8 +302,9 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, in
     }
 }
 
-// Workgroups of a pass: as many as 64 KB of x to each 256 threads make, eight of those to a CU at most (265 MB: 2048
-// 373 us a training pass, 1024 385) and two at least (31 MB: 512 77 us, 1024 87, whose results take longer to join).
+// Workgroups of a pass: as many as 64 KB of x to each 256 threads make, eight of those to a CU at most (six images of 92
+// MB: 2048 863 us forward and backward, 1024 960) and two at least (31 MB: 512 77 us, 1024 87, whose results take
+// longer to join).
 constexpr int64_t kThreadBytes = 256, kMostThreads = 2048 * 256, kFewThreads = 512 * 256;
 // Results go around the last-level cache where a call moves more than half of it: they would push out what the next pass
 // or the next call reads (265 MB of x: statistics 73 -> 46 us; 132 MB: 37 -> 22, also with a kernel that reads the
@@ -317,8 +318,8 @@ int norm_vector(const xsg_norm_desc* d, bool draws) {
     if (d->dtype != XSG_DTYPE_F32) return c >= 8 ? 8 : c >= 4 ? 4 : 1;
     if (c > 4 * kNormThreads) return 8;   // a workgroup would not have the threads
     // With draws: a wavefront's vectors of four lie in 32 blocks of draws where the channels are a multiple of eight, or
-    // where the vectors overlap by enough (65 channels, 17 M values: 125 us the three passes, 132 with vectors of eight);
-    // else some lane needs a 33rd, and eight are better (513 channels, 246 M values: 1390 and 1800 us)
+    // where the vectors overlap by enough (65 channels, 17 M values: 120 us the three passes, 125 with vectors of eight);
+    // else some lane needs a 33rd, and eight are better (513 channels, 246 M values: 1460 us, 1797 with four)
     const int vectors = (c + 3) / 4;
     if (draws && d->drop.p > 0.0 && c >= 8 && c % 8 != 0 && 64 * (4 * vectors - c) < 8 * vectors) return 8;
     return c >= 4 ? 4 : 1;
@@ -397,7 +398,8 @@ extern "C" int xsg_group_norm_act_fwd(const xsg_norm_desc* d, void* y, float* st
     }
     const int size = d->dtype == XSG_DTYPE_F32 ? 4 : 2, vector = norm_vector(d, false), draw_vector = norm_vector(d, true);
     norm_layout(a, vector, kStatsUnroll, size, 2, 512);
-    if (a.batch * std::max(a.chunks, a.groups) > INT_MAX / 2) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_fwd: too large");
+    if (a.batch * a.chunks > kNormBlocks || (!a.join && a.batch * a.groups > kNormBlocks))
+        return xsg_fail(XSG_ERR_INVALID, "group_norm_act_fwd: too many samples (%lld)", (long long)a.batch);
     const hipStream_t s = (hipStream_t)stream;
     float2* const part = (float2*)workspace;
     float* const counts = (float*)(part + a.batch * a.chunks * a.groups);

@@ -3,7 +3,8 @@ stream, so the backward draws again and no mask is stored. An extension of this 
 
 ``seed``: an int in [0, 2^63), another for each step; or an int64 tensor of one value on the GPU, which the kernels
 read (a captured graph then draws anew on each replay if the value is changed in between; not between a forward
-and its backward, which autograd refuses). ``stream``: a number in [0, 2^31), another for each place that
+and its backward, which autograd refuses; as with any operator, a backward is captured while no eager graph of the same leaves
+lives). ``stream``: a number in [0, 2^31), another for each place that
 draws under one seed. Probabilities count in steps of 2^-32; what is kept is divided by the share that is kept."""
 import torch
 
