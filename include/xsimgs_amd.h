@@ -299,7 +299,7 @@ typedef struct {
     xsg_drop_desc drop;               /* value e is element e of the dense y */
 } xsg_norm_desc;
 
-/* stats [batch, groups, 4]: mean, 1 / sqrt(variance + eps), 1 / count (0 of none), 0; the backward takes them, and
+/* stats [batch, groups, 4]: mean, 1 / sqrt(variance + eps), 1 / count (zeros of none), 0; the backward takes them, and
  * the same desc. weight and bias gradients in float32, either may be NULL, as may v_x. */
 size_t xsg_group_norm_act_workspace_bytes(const xsg_norm_desc* d, int backward);
 int xsg_group_norm_act_fwd(const xsg_norm_desc* d, void* y, float* stats, void* workspace, xsg_stream_t stream);

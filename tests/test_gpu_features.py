@@ -55,7 +55,7 @@ def _formula(x, groups, w, b, act, eps, mask, drop, seed, stream, v_y=None):
     n = (keep.sum(1, keepdim=True) * cg).clamp(min=1)
     mean = x.sum((1, 3), keepdim=True) / n
     var = torch.where(keep, (x - mean) ** 2, 0.0).sum((1, 3), keepdim=True) / n
-    rstd = 1 / (var + eps).sqrt()
+    rstd = torch.where(keep.any(1, keepdim=True), 1 / (var + eps).sqrt(), 0.0)
     xh = torch.where(keep, (x - mean) * rstd, 0.0)
     z = xh * w + b
     y, slope = _act(z, act)
@@ -203,6 +203,21 @@ def test_constant_groups(dev):
     x = torch.full((1, 50, 4), 3.25, device=dev)
     w, b = _params(4, 5, dev)
     _run(x, 2, w, b, act="none", v_y=_randn(x.shape, 7, dev))
+    # a flat image far from zero is its bias, in every type
+    from xsimgs_amd import rendering
+
+    for dtype in TYPES:
+        for pixels in (50, 40_000):
+            flat = torch.full((1, pixels, 4), 1000.0, dtype=dtype, device=dev)
+            assert torch.equal(rendering.group_norm_act(flat, 2, w, b, act="none"), b.to(dtype).expand(flat.shape))
+
+
+@pytest.mark.parametrize("pixels", [30, 6000])
+def test_samples_out_of_the_mask_without_eps(dev, pixels):
+    x, (w, b) = _randn((3, pixels, 8), 1, dev), _params(8, 5, dev)
+    mask = torch.ones(3, pixels, dtype=torch.bool, device=dev)
+    mask[1] = False
+    _run(x, 2, w, b, eps=0.0, mask=mask, v_y=_randn(x.shape, 7, dev))
 
 
 @pytest.mark.parametrize("batch", [1, 7, 65, 1500])

@@ -155,7 +155,8 @@ struct NormSums {
         const float inv = n > 0.0 ? 1.0f / (float)n : 0.0f;
         float var = (float)(d + s2 - s1 * s1 * (double)inv) * inv;
         if (var < 0.0f) var = 0.0f;   // a NaN stays
-        return make_float4(about + (float)s1 * inv, 1.0f / sqrtf(var + eps), inv, 0.0f);
+        // nothing in the mask: zeros, also without eps
+        return make_float4(about + (float)s1 * inv, n > 0.0 ? 1.0f / sqrtf(var + eps) : 0.0f, inv, 0.0f);
     }
     // entries first, first + step, ... of a group's parts, eight on their way at a time
     XSG_DEV void add_parts(const float2* __restrict__ part, const float* __restrict__ counts, int groups, int parts,
@@ -262,11 +263,6 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, in
     }
     const Draws draws(a.drop);
     const float kept = 1.0f / a.drop.factor;
-    // (x - mean) scale + bias; in 16 bits x scale + (bias - mean scale), whose cancellation is below x's own digits
-    if (!EXACT) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) bias[j] = fmaf(-mean[j], scale[j], bias[j]);
-    }
     // every lane goes through every batch: draws are shared between them
     for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
         const bool more = p + at.jump < a.pixels;
@@ -282,8 +278,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, in
                 unpack<DT, V>(raw[u], x);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float z = EXACT ? fmaf(x[j] - mean[j], scale[j], bias[j]) : fmaf(x[j], scale[j], bias[j]);
-                    x[j] = norm_act<ACT, EXACT, DROP>(z, a.drop.factor, kept);
+                    x[j] = norm_act<ACT, EXACT, DROP>(fmaf(x[j] - mean[j], scale[j], bias[j]), a.drop.factor, kept);
                     if (DROP) x[j] = keep_bit(x[j], keep, j);
                 }
                 out = pack<DT, V>(x);

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kSmallThreads) void norm_small_kernel(NormArgs a, S
             const float inv = m.z > 0.0f ? 1.0f / m.z : 0.0f, left = sum * inv;
             float var = dev * inv - left * left;
             if (var < 0.0f) var = 0.0f;   // a NaN stays
-            s_group[g] = make_float4(m.x + left, 1.0f / sqrtf(var + a.eps), inv, 0.0f);
+            s_group[g] = make_float4(m.x + left, inv > 0.0f ? 1.0f / sqrtf(var + a.eps) : 0.0f, inv, 0.0f);
             stats[b * a.groups + g0 + g] = s_group[g];
         }
     }
