@@ -295,10 +295,21 @@ def test_dropout_behind_is_dropout(dev):
 
     for c in (64, 32, 11, 3):
         for dtype in TYPES:
-            x = _randn((2, 301, c), 1, dev, dtype)
-            y = rendering.group_norm_act(x, 1, act="silu")
-            dropped = rendering.group_norm_act(x, 1, act="silu", drop=0.3, seed=6, stream=4)
-            assert torch.equal(dropped != 0, rendering.dropout(torch.ones_like(y), 0.3, 6, stream=4).ne(0) & (y != 0))
+            x = _randn((2, 1301, c), 1, dev, dtype).requires_grad_()
+            y = rendering.group_norm_act(x.detach(), 1, act="silu")
+            # the last two: a threshold below 2^16, and one that a value's own 32 bits equal but for one
+            u = _draws.draws(0, y.numel(), 6, 4)
+            for p in (0.3, 0.999, 1e-5, (int(u[9 * c + 1]) + 1) / 2 ** 32):
+                kept = rendering.dropout(torch.ones_like(y), p, 6, stream=4).ne(0)
+                assert torch.equal(kept.cpu().view(-1), torch.as_tensor(_draws.kept(y.numel(), p, 6, 4)[0]))
+                dropped = rendering.group_norm_act(x, 1, act="silu", drop=p, seed=6, stream=4)
+                assert torch.equal(dropped != 0, kept & (y != 0))
+                # with everything else out, v_b is the sum of the kept elements' factors and slopes
+                b = torch.zeros(c, device=dev, requires_grad=True)
+                z = rendering.group_norm_act(x, 1, None, b, act="none", drop=p, seed=6, stream=4)
+                g, = torch.autograd.grad(z, b, torch.ones_like(z))
+                want = kept.view(-1, c).double().sum(0) * _draws.kept(1, p, 6)[1]
+                assert bool(((g.double() - want).abs() <= 128 * U * want).all())
 
 
 def test_the_same_bits_each_time(dev):

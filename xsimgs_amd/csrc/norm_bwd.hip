@@ -59,19 +59,20 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a, con
     for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
         const bool more = p + at.jump < a.pixels;
         if (AHEAD && more) next.fetch(a, at, x_at, g_at, p + at.jump);
-        NormDraws<V> drawn{draws, a.channels, first + p * a.channels, (int64_t)a.ty * a.channels, 0};
+        NormDraws<DT, V> drawn(draws, a.channels, first + p * a.channels, (int64_t)a.ty * a.channels);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t keep = DROP ? drawn(u) : 0;
+            if (DROP) drawn.draw(u);
             if (!(now.in >> (16 + u) & 1)) continue;
             float x[V], g[V];
             unpack<DT, V>(now.x[u], x);
+            if (DROP) drawn.mask(now.g[u]);
             unpack<DT, V>(now.g[u], g);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float e = x[j] - mean[j];
                 float dz = g[j] * norm_act_slope<ACT, EXACT>(e * scale[j] + bias[j]);
-                if (DROP) dz = keep_bit(dz, keep, j);   // the factor comes at the end
+                if (DROP) dz = drawn.one(dz, j);   // the factor comes at the end
                 s1[j] += dz;
                 s2[j] += dz * e;
             }
@@ -230,21 +231,22 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_kernel(NormArgs a, int
     for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
         const bool more = p + at.jump < a.pixels;
         if (AHEAD && more) next.fetch(a, at, x_at, g_at, p + at.jump);
-        NormDraws<V> drawn{draws, a.channels, first + p * a.channels, (int64_t)a.ty * a.channels, 0};
+        NormDraws<DT, V> drawn(draws, a.channels, first + p * a.channels, (int64_t)a.ty * a.channels);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t keep = DROP ? drawn(u) : 0;
+            if (DROP) drawn.draw(u);
             if (!(now.in >> u & 1)) continue;
             Raw<V * ElementSize<DT>::value> out = {};
             if (!MASK || (now.in >> (16 + u) & 1)) {
                 float x[V], g[V];
                 unpack<DT, V>(now.x[u], x);
-                unpack<DT, V>(now.g[u], g);
+                if (DROP) drawn.mask(now.g[u]);
+            unpack<DT, V>(now.g[u], g);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float e = x[j] - mean[j];
                     float dz = g[j] * norm_act_slope<ACT, EXACT>(e * scale[j] + bias[j]);
-                    if (DROP) dz = keep_bit(dz * a.drop.factor, keep, j);
+                    if (DROP) dz = drawn.one(dz * a.drop.factor, j);
                     x[j] = scale[j] * dz - shift[j] - e * slope[j];
                 }
                 out = pack<DT, V>(x);

@@ -267,10 +267,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, in
     for (int64_t p = at.p0; p < a.pixels; p += at.jump) {
         const bool more = p + at.jump < a.pixels;
         if (AHEAD && more) in_next = fetch(p + at.jump, next);
-        NormDraws<V> drawn{draws, a.channels, first + p * a.channels, (int64_t)a.ty * a.channels, 0};
+        NormDraws<DT, V> drawn(draws, a.channels, first + p * a.channels, (int64_t)a.ty * a.channels);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t keep = DROP ? drawn(u) : 0;
+            if (DROP) drawn.draw(u);
             if (!(in >> u & 1)) continue;
             Vec out = {};
             if (!MASK || (in >> (16 + u) & 1)) {
@@ -279,9 +279,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, in
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     x[j] = norm_act<ACT, EXACT, DROP>(fmaf(x[j] - mean[j], scale[j], bias[j]), a.drop.factor, kept);
-                    if (DROP) x[j] = keep_bit(x[j], keep, j);
+                    if (DROP) x[j] = drawn.one(x[j], j);
                 }
                 out = pack<DT, V>(x);
+                if (DROP) drawn.mask(out);
             }
             store_raw<DT, V, STREAM>(y_at(p + u * a.ty), 0, out);
             if (DROP) __builtin_amdgcn_sched_barrier(0);   // several pixels' draws at once take too many registers

@@ -4,7 +4,7 @@
 //
 // All of it is bound by memory where images are large and nothing is drawn: x is read for its statistics and again for the
 // result, x and v_y for their sums and again for v_x, at 5.3 to 6.2 TB/s (1080p x 64 bfloat16, silu: statistics 46 us,
-// result 85, sums 96, v_x 140). With draws the vector units are (225 x 400 x 128 x 6 float16: 57, 72 and 80 us).
+// result 85, sums 96, v_x 140). With draws the vector units are (225 x 400 x 128 x 6 float16: 58, 69 and 78 us).
 #pragma once
 #include "xsg_elements.h"
 #include "xsg_random.h"
@@ -146,26 +146,41 @@ template <int U, bool MASK, int V> XSG_DEV uint32_t norm_pixels(const NormArgs& 
     return in;
 }
 
-// A thread's draws: bit j for element first + j of pixel u of a batch. Every lane of the wavefront comes here for every
-// pixel, in the order of their elements. With vectors of four, two pixels' draws come at once.
-template <int V> struct NormDraws {
+// A thread's draws of pixel u of a batch, from element first + u step on. Every lane of the wavefront comes here for every
+// pixel, in the order of their elements. With vectors of four, two pixels' draws come at once; with eight 16-bit values
+// they are words that the packed values are masked with, two values an operation (69 M float16 values: 214 us the three
+// passes, 227 with bits).
+template <int DT, int V> struct NormDraws {
+    static constexpr bool HALVES = DT != XSG_DTYPE_F32 && V == 8;
     const Draws& draws;
     int channels;
     int64_t first, step;   // element of the batch's first pixel, and from pixel to pixel
-    uint32_t next;
-    XSG_DEV uint32_t operator()(int u) {
+    uint32_t bits, next;
+    Words4 halves;
+    XSG_DEV NormDraws(const Draws& draws_, int channels_, int64_t first_, int64_t step_)
+        : draws(draws_), channels(channels_), first(first_), step(step_), bits(0), next(0), halves{} {}
+    XSG_DEV void draw(int u) {
         const int64_t e = first + u * step;
-        uint32_t keep;
-        if (V == 8) {
-            keep = channels % 8 == 0 ? draws.keep8((uint64_t)e >> 3) : draws.keep_in_order((uint64_t)e);
+        if (HALVES) {
+            halves = channels % 8 == 0 ? draws.halves8((uint64_t)e >> 3) : Draws::halves_of(draws.keep_in_order((uint64_t)e));
+        } else if (V == 8) {
+            bits = channels % 8 == 0 ? draws.keep8((uint64_t)e >> 3) : draws.keep_in_order((uint64_t)e);
         } else if (V == 4) {
-            if (u % 2) return next;
-            draws.keep_in_order((uint64_t)e, (uint64_t)(e + step), keep, next);
+            if (u % 2) bits = next;
+            else draws.keep_in_order((uint64_t)e, (uint64_t)(e + step), bits, next);
         } else {
-            keep = draws.keep((uint64_t)e, V);
+            bits = draws.keep((uint64_t)e, V);
         }
-        return keep;
     }
+    // zeros in packed values that are dropped, whatever they hold
+    XSG_DEV void mask(Raw<V * ElementSize<DT>::value>& r) const {
+        if constexpr (HALVES) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r.w[k] &= halves.w[k];
+        }
+    }
+    // the same of one value, where mask() does nothing
+    XSG_DEV float one(float x, int j) const { return HALVES ? x : keep_bit(x, bits, j); }
 };
 
 // Statistics of a sample's groups lie in `part` (mean and squared deviations of each chunk) and `counts` (elements of

@@ -64,8 +64,8 @@ struct Draws {
     // a value they would take as long as moving it. The halves are compared two at a time.
     XSG_DEV uint32_t keep8(uint64_t block) const {
         const Words4 r = words(block, 0);
-        const uint32_t below = (upper ? upper - 1 : 0) * 0x10001u, at = upper * 0x10001u;
-        uint32_t m = upper ? 0 : 0x550055u, apart = ~0u;
+        const uint32_t below = (upper ? upper - 1 : 0) * 0x10001u;
+        uint32_t m = upper ? 0 : 0x550055u;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             // 1 in each half that is above `below`: the saturated difference, or 1 (by name: the compiler takes this
@@ -73,20 +73,49 @@ struct Draws {
             uint32_t over;
             asm("v_pk_sub_u16 %0, %1, %2 clamp\n\tv_pk_min_u16 %0, %0, %3" : "=&v"(over) : "v"(r.w[k]), "v"(below), "v"(0x10001u));
             m |= over << (2 * k);
-            // a half of 0 where one equals the threshold's
-            apart = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, apart),
-                                                                           __builtin_bit_cast(u16x2, r.w[k] ^ at)));
         }
         uint32_t keep = (m | m >> 15) & 0xffu;
+        ties(r, block, [&](int j) { keep &= ~(1u << j); });
+        return keep;
+    }
+    // The same as words of ones and zeros: half j % 2 of word j / 2 for value 8 block + j.
+    XSG_DEV Words4 halves8(uint64_t block) const {
+        const Words4 r = words(block, 0);
+        const uint32_t below = (upper ? upper - 1 : 0) * 0x10001u;
+        Words4 m;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            asm("v_pk_sub_u16 %0, %1, %2 clamp\n\tv_pk_min_u16 %0, %0, %3\n\tv_pk_sub_u16 %0, 0, %0"
+                : "=&v"(m.w[k]) : "v"(r.w[k]), "v"(below), "v"(0x10001u));
+            if (upper == 0) m.w[k] = ~0u;
+        }
+        ties(r, block, [&](int j) { m.w[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u; });
+        return m;
+    }
+    // drop(j) for each value whose upper bits are the threshold's and whose lower ones are below it
+    template <typename F> XSG_DEV void ties(const Words4& r, uint64_t block, F drop) const {
+        const uint32_t at = upper * 0x10001u;
+        uint32_t apart = ~0u;   // a half of 0 where one equals the threshold's
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            apart = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, apart),
+                                                                           __builtin_bit_cast(u16x2, r.w[k] ^ at)));
         if (lower != 0 && ((apart & 0xffffu) == 0 || apart < 0x10000u)) {
             const Words4 s = words(block, 1);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t h = r.w[j >> 1] >> 16 * (j & 1) & 0xffffu, l = s.w[j >> 1] >> 16 * (j & 1) & 0xffffu;
-                if (h == upper && l < lower) keep &= ~(1u << j);
+                if (h == upper && l < lower) drop(j);
             }
         }
-        return keep;
+    }
+    XSG_DEV static Words4 halves_of(uint32_t keep) {
+        Words4 m;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            m.w[k] = ((uint32_t)__builtin_amdgcn_sbfe((int)keep, 2 * k, 1) & 0xffffu) |
+                     ((uint32_t)__builtin_amdgcn_sbfe((int)keep, 2 * k + 1, 1) & 0xffff0000u);
+        return m;
     }
     // Bit j < n: value first + j is kept, n up to 8; two calls where they lie in two blocks.
     XSG_DEV uint32_t keep(uint64_t first, int n) const {
