@@ -5,7 +5,6 @@
 // A first pass leaves each workgroup's sums of dz and dz xh for each channel, and of their products with the weight
 // for each group; a second joins the groups' (its own workgroups do, where they are few) and writes v_x, while
 // some more of its workgroups join the channels'. Sums are added in a fixed order. No reference counterpart.
-#include <algorithm>
 
 #include "xsg_norm.h"
 
