@@ -1,0 +1,36 @@
+"""The feature norm and dropout at the places where they once went wrong. Tolerances: those of test_gpu_features, whose
+formula in 64 bits is used; what is exact is said where it is asserted."""
+import pytest
+import torch
+
+from tests.test_gpu_features import TYPES, _params, _randn, _run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("channels, groups, pixels", [(16, 4, 3000), (8, 1, 5000), (40, 40, 25_000), (65, 5, 9000)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("where", ["first", "middle", "last", "all but the last"])
+def test_offsets_under_a_mask(dev, dtype, channels, groups, pixels, where):
+    """A mean of many spreads, and parts of the image (first of all its beginning) that the mask empties and that hold no
+    numbers: an empty part has no mean, and the joint variance is no difference of what 32 bits hold. With 40 groups the
+    parts are too many for the kernels that need them to join them."""
+    offset, spread = dict(zip(TYPES, ((1000.0, 1.0), (1000.0, 8.0), (1000.0, 1.0))))[dtype]
+    x = (_randn((2, pixels, channels), 1, dev) * spread + offset).to(dtype)
+    part = min(pixels // 3, 1500)
+    mask = torch.ones(2, pixels, dtype=torch.bool, device=dev)
+    mask[:, {"first": slice(0, part), "middle": slice(part, 2 * part), "last": slice(pixels - part, None),
+             "all but the last": slice(0, pixels - 100)}[where]] = False
+    x[~mask] = float("nan")
+    w, b = _params(channels, 5, dev)
+    _run(x, groups, w, b, mask=mask, v_y=_randn(x.shape, 7, dev, dtype))
+
+
+def test_a_beginning_far_from_the_rest(dev):
+    """The only pixel of the first part that the mask leaves lies hundreds of deviations from the mean."""
+    x = _randn((1, 100_000, 4), 1, dev)
+    x[:, 0] = 1e4
+    mask = torch.ones(1, 100_000, dtype=torch.bool, device=dev)
+    mask[:, 1:2000] = False
+    w, b = _params(4, 5, dev)
+    _run(x, 1, w, b, act="gelu", mask=mask, v_y=_randn(x.shape, 7, dev))

@@ -139,7 +139,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a, fl
     }
 }
 
-// A group's chunks joined in 64 bits, about the first chunk's mean (squares of differences of means, in digits to spare).
+// A group's chunks joined in 64 bits, about the mean of the first chunk that has any pixels: squares of differences of
+// means, in digits to spare (with that chunk of one pixel and n values behind it, they cancel to 1 / n at worst).
 struct NormSums {
     double n, s1, s2, d;
     XSG_DEV NormSums() : n(0.0), s1(0.0), s2(0.0), d(0.0) {}
@@ -150,13 +151,23 @@ struct NormSums {
         s2 += count * e * e;
         d += m.y;
     }
-    // the last steps in 32 bits: they are relative to the spread
+    // what cancels is divided in 64 bits too: a reciprocal of 32 leaves 6e-8 of s2
     XSG_DEV float4 stats(float about, float eps) const {
-        const float inv = n > 0.0 ? 1.0f / (float)n : 0.0f;
-        float var = (float)(d + s2 - s1 * s1 * (double)inv) * inv;
+        if (!(n > 0.0)) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // nothing in the mask: zeros, also without eps
+        const double shift = s1 / n;
+        const float inv = 1.0f / (float)n;
+        float var = (float)(d + s2 - s1 * shift) * inv;
         if (var < 0.0f) var = 0.0f;   // a NaN stays
-        // nothing in the mask: zeros, also without eps
-        return make_float4(about + (float)s1 * inv, n > 0.0 ? 1.0f / sqrtf(var + eps) : 0.0f, inv, 0.0f);
+        return make_float4((float)(about + shift), 1.0f / sqrtf(var + eps), inv, 0.0f);
+    }
+    // the mean of the first chunk that has any pixels (of an empty one it is 0, which may be far away): a segment of l lanes
+    template <bool MASK> XSG_DEV static float about(const float2* __restrict__ part, const float* __restrict__ counts, int groups,
+                                                    int parts, int lane, int l) {
+        if (!MASK || counts[0] > 0.0f) return part[0].x;
+        int k = lane;
+        while (k < parts && !(counts[k] > 0.0f)) k += l;
+        for (int d = l >> 1; d; d >>= 1) k = min(k, __shfl_xor(k, d));
+        return k < parts ? part[(int64_t)k * groups].x : 0.0f;
     }
     // entries first, first + step, ... of a group's parts, eight on their way at a time
     XSG_DEV void add_parts(const float2* __restrict__ part, const float* __restrict__ counts, int groups, int parts,
@@ -178,13 +189,14 @@ struct NormSums {
 };
 
 // One workgroup to a group of a sample (1080p x 64: 4.7 us, as long as a launch takes).
+template <bool MASK>
 __global__ __launch_bounds__(256) void norm_join_kernel(int groups, int chunks, float eps, const float2* __restrict__ part,
                                                         const float* __restrict__ counts, float4* __restrict__ stats) {
     __shared__ double s_sum[4][4];
     const int64_t b = blockIdx.x / groups;
     const float2* const p = part + b * chunks * groups + blockIdx.x % groups;
     const float* const c = counts + b * chunks;
-    const float about = p[0].x;
+    const float about = NormSums::about<MASK>(p, c, groups, chunks, threadIdx.x & 63, 64);   // the same in each wavefront
     NormSums sum;
     sum.add_parts(p, c, groups, chunks, threadIdx.x, 256, about);
     double* const mine = s_sum[threadIdx.x >> 6];
@@ -241,7 +253,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, in
         const float2* const p = part + at.b * parts * a.groups;
         for (int g = threadIdx.x / l; g < a.groups; g += blockDim.x / l) {
             NormSums sum;
-            const float about = p[g].x;
+            const float about = NormSums::about<MASK>(p + g, counts + at.b * parts, a.groups, parts, lane, l);
             sum.add_parts(p + g, counts + at.b * parts, a.groups, parts, lane, l, about);
             sum.n = segment_sum(sum.n, l);
             sum.s1 = segment_sum(sum.s1, l);
@@ -416,7 +428,8 @@ extern "C" int xsg_group_norm_act_fwd(const xsg_norm_desc* d, void* y, float* st
             else stats_pass(std::false_type{});
         });
         if (!a.join)
-            norm_join_kernel<<<(unsigned)(a.batch * a.groups), 256, 0, s>>>(a.groups, chunks, a.eps, part, counts, (float4*)stats);
+            (a.mask ? norm_join_kernel<true> : norm_join_kernel<false>)<<<(unsigned)(a.batch * a.groups), 256, 0, s>>>(
+                a.groups, chunks, a.eps, part, counts, (float4*)stats);
         const int join = a.join;
         norm_layout(a, draw_vector, norm_apply_unroll(draw_vector * size), size, 2, 256);
         a.join = join;
