@@ -34,3 +34,20 @@ def test_a_beginning_far_from_the_rest(dev):
     mask[:, 1:2000] = False
     w, b = _params(4, 5, dev)
     _run(x, 1, w, b, act="gelu", mask=mask, v_y=_randn(x.shape, 7, dev))
+
+@pytest.mark.parametrize("value", [0.1, -77.77, 1000.1, 3e5 + 0.3])
+@pytest.mark.parametrize("channels, groups", [(4, 2), (9, 3), (64, 8), (1, 1), (130, 1)])
+def test_flat_images(dev, value, channels, groups):
+    """Each pixel of a flat image is its bias, whatever the value: its mean is the value itself, and (x - mean) is 0."""
+    from xsimgs_amd import rendering
+
+    w, b = _params(channels, 5, dev)
+    for dtype in TYPES:
+        for pixels in (50, 3001, 40_000):
+            flat = torch.full((1, pixels, channels), value if dtype != torch.float16 else value / 10, dtype=dtype, device=dev)
+            assert torch.equal(rendering.group_norm_act(flat, groups, w, b, act="none"), b.to(dtype).expand(flat.shape))
+            mask = torch.ones(1, pixels, dtype=torch.bool, device=dev)
+            mask[:, :pixels // 4] = False
+            mask[:, ::7] = False
+            y = rendering.group_norm_act(flat, groups, w, b, act="none", mask=mask)
+            assert torch.equal(y, torch.where(mask[..., None], b.to(dtype), 0.0).to(dtype))

@@ -128,13 +128,18 @@ __global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a, fl
         };
         float count = 0.0f, sum = 0.0f;
         each([&](float2 m, float k) { count += k; sum += k * m.x; });
-        count = segment_sum(count, l);
-        sum = segment_sum(sum, l);
+        segment_sums(count, sum, l);
         const float mu = count > 0.0f ? sum / count : 0.0f;
-        float d = 0.0f;
-        each([&](float2 m, float k) { d += m.y + k * (m.x - mu) * (m.x - mu); });
-        d = segment_sum(d, l);
-        if (lane == 0) part[(int64_t)blockIdx.x * a.groups + g] = make_float2(mu, d);
+        // deviations about that mean, and what its own rounding left of their sum
+        float d = 0.0f, left = 0.0f;
+        each([&](float2 m, float k) {
+            const float e = m.x - mu;
+            d += m.y + k * e * e;
+            left += k * e;
+        });
+        segment_sums(d, left, l);
+        const float shift = count > 0.0f ? left / count : 0.0f;
+        if (lane == 0) part[(int64_t)blockIdx.x * a.groups + g] = make_float2(mu + shift, d - left * shift);
         if (lane == 0 && g == 0) counts[blockIdx.x] = count;
     }
 }

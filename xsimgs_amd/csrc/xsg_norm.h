@@ -107,6 +107,14 @@ template <typename T> XSG_DEV T segment_sum(T x, int l) {
     for (int d = l >> 1; d; d >>= 1) x += __shfl_xor(x, d);
     return x;
 }
+// two sums side by side, which wait for each other's lanes once
+XSG_DEV void segment_sums(float& x, float& y, int l) {
+    for (int d = l >> 1; d; d >>= 1) {
+        const float x2 = __shfl_xor(x, d), y2 = __shfl_xor(y, d);
+        x += x2;
+        y += y2;
+    }
+}
 
 // A thread's place: its first channel, its row of the pixels side by side, and its workgroup's batches of pixels: from
 // p0 on in jumps, in turn with the sample's other workgroups, so that all of them together move through one stretch of
