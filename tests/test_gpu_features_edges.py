@@ -51,3 +51,40 @@ def test_flat_images(dev, value, channels, groups):
             mask[:, ::7] = False
             y = rendering.group_norm_act(flat, groups, w, b, act="none", mask=mask)
             assert torch.equal(y, torch.where(mask[..., None], b.to(dtype), 0.0).to(dtype))
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
+@pytest.mark.parametrize("pixels", [30, 2500])
+def test_biases_at_the_ends_of_float32(dev, dtype, act, pixels):
+    """A channel that its bias switches off gives 0 and no gradient; one far on the other side is linear. At z = -88 and
+    below each activation and its slope are less than 1e-36 in size."""
+    from xsimgs_amd import rendering
+
+    low = torch.tensor([torch.finfo(torch.float32).min, -1e30, -1e6, -200.0])
+    high = torch.tensor([torch.finfo(torch.float32).max, 2.5e38, 1e30, 1e4])
+    x, v_y = _randn((2, pixels, 12), 1, dev, dtype).requires_grad_(), _randn((2, pixels, 12), 7, dev, dtype)
+    w = torch.ones(12, device=dev, requires_grad=True)
+    b = torch.cat([low, high, torch.zeros(4)]).to(dev).requires_grad_()
+    y = rendering.group_norm_act(x, 3, w, b, act=act)
+    assert bool((y[..., :4].float().abs() <= 1e-30).all())
+    z = rendering.group_norm_act(x, 3, w, b, act="none")       # the same values without an activation
+    half = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    # the activation is z itself there: each is rounded once, after 8 units of float32
+    far, want = y[..., 4:8].detach().double(), z[..., 4:8].detach().double()
+    assert bool(((far == want) | ((far - want).abs() <= (2 * half + 2.0 ** -20) * want.abs())).all())
+    v_x, v_w, v_b = torch.autograd.grad(y, [x, w, b], v_y)
+    assert bool((v_x[..., :4] == 0).all()) and bool((v_w[:4].abs() <= 1e-30).all()) and bool((v_b[:4].abs() <= 1e-30).all())
+    want = v_y[..., 4:8].double().sum((0, 1))
+    assert bool(((v_b[4:8].double() - want).abs() <= 80 * 2.0 ** -24 * v_y[..., 4:8].double().abs().sum((0, 1))).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
+@pytest.mark.parametrize("pixels", [30, 2500])
+def test_an_infinite_bias(dev, dtype, act, pixels):
+    """Activations of infinity are infinity."""
+    from xsimgs_amd import rendering
+
+    b = torch.full((8,), float("inf"), device=dev)
+    y = rendering.group_norm_act(_randn((2, pixels, 8), 1, dev, dtype), 2, None, b, act=act)
+    assert bool((y == float("inf")).all())

@@ -42,18 +42,19 @@ XSG_DEV float norm_param(const void* p, int dtype, int i, float otherwise) {
 }
 
 // 1 / (1 + exp(-z)) from the hardware's exponential and reciprocal (1 ulp each). EXACT, for float32 results: the
-// exponent's rounding and the reciprocal's last bit are made good; the other types are rounded to 8 or 11 bits next.
+// exponent's rounding and the reciprocal's last bit are made good, within 2^+-126 (beyond, the corrections would be differences
+// of infinities; what lies above the exponent's range is 1, and what lies below is no normal number: 0, so that z times it is
+// small for every z); the other types are rounded to 8 or 11 bits next.
 template <bool EXACT> XSG_DEV float norm_sigmoid(float z) {
-    float p = z * -1.44269504f, e;
+    const float p = z * -1.44269504f;
+    float e = __builtin_amdgcn_exp2f(p);
     if (EXACT) {
-        p = fminf(p, 126.0f);   // so that 1 + e stays finite for the correction
-        e = __builtin_amdgcn_exp2f(p);
         const float low = fmaf(z, -1.44269504f, -p) + z * -1.92596303e-8f;
-        if (p < 126.0f) e = fmaf(e * 0.69314718f, low, e);
+        if (fabsf(p) < 126.0f) e = fmaf(e * 0.69314718f, low, e);
         const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d);
-        return fmaf(r, fmaf(-d, r, 1.0f), r);
+        return p < 126.0f ? fmaf(r, fmaf(-d, r, 1.0f), r) : 0.0f;
     }
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(p));
+    return __builtin_amdgcn_rcpf(1.0f + e);
 }
 // The normal distribution function and exp(-z^2 / 2). With t = 1 / (1 + 0.29 |z|), the tail is exp(-z^2 / 2) times a
 // polynomial in t of degree 8 (a least-squares fit of erfc(x) exp(x^2) / 2, weighted towards the least largest error: 2e-9
