@@ -88,3 +88,24 @@ def test_an_infinite_bias(dev, dtype, act, pixels):
     b = torch.full((8,), float("inf"), device=dev)
     y = rendering.group_norm_act(_randn((2, pixels, 8), 1, dev, dtype), 2, None, b, act=act)
     assert bool((y == float("inf")).all())
+
+def test_a_frames_head_that_drops_needs_a_seed(dev):
+    """Without one the same features would be dropped in every step; a head in evaluation needs none."""
+    from tests.test_gpu_frame_drop import _image_grads, _scene
+    from xsimgs_amd import frame, rendering
+
+    for rig in (False, True):
+        sc = _scene("rig" if rig else "cfg0", 8)
+        st = frame.prepare(sc, dev, head=rendering.FeatureNorm(2, 8, drop=0.25))
+        opt = frame.make_optimizer(st)
+        before = [t.detach().clone() for t in (st.means, st.colors, st.head.weight)]
+        grads = _image_grads(sc, 8, dev, rig)
+        render = frame.render_rig if rig else frame.render_frame
+        for call in (lambda: render(st), lambda: frame.train_frame(st, opt, grads, rig=rig),
+                     lambda: frame.train_frame(st, opt, grads, rig=rig, drop=0.2)):
+            with pytest.raises(ValueError, match="seed"):
+                call()
+        assert all(torch.equal(a, t.detach()) for a, t in zip(before, (st.means, st.colors, st.head.weight)))
+        st.head.eval()
+        frame.train_frame(st, opt, grads, rig=rig)
+        assert not torch.equal(before[2], st.head.weight.detach())

@@ -88,11 +88,11 @@ def _headed(st: FrameState, rgb, out: dict, seed):
 
 
 def render_frame(st: FrameState, backward: bool = False, grads=None, cam_index: int = 0, *, drop: float = 0.0,
-                 seed=0) -> dict:
+                 seed=None) -> dict:
     """``drop``: each Gaussian is left out of the frame with this probability and the others' opacities are divided by the
     share kept (``rendering.activate_gaussians``); ``out["kept"]`` is the packed mask of those kept. ``seed``: another
-    one for each step, as for ``rendering.dropout``; a head in training mode draws under it too. With a head the colour
-    gradient is that of ``out["features"]``."""
+    one for each step, as for ``rendering.dropout``, needed where something is dropped; a head in training mode draws under
+    it too. With a head the colour gradient is that of ``out["features"]``."""
     sc = st.scene
     spec = sc.cameras[cam_index]
     cam = st.cams[cam_index]
@@ -136,7 +136,7 @@ def rig_shares_origin(st: FrameState) -> bool:
     return len({tuple(float(x) for x in s.t) for s in st.scene.cameras}) == 1
 
 
-def render_rig(st: FrameState, backward: bool = False, grads=None, *, drop: float = 0.0, seed=0) -> dict:
+def render_rig(st: FrameState, backward: bool = False, grads=None, *, drop: float = 0.0, seed=None) -> dict:
     """Every camera of a rig in one batched pass (an extension of this build; the reference's caller
     renders one camera per call, render.py:85-187). Per camera the UT projection and the rays, as
     in render_frame; then one batched binning (keys carry the camera above the tile bits), one
@@ -237,7 +237,7 @@ def make_optimizer(st: FrameState, rates=None, **kw) -> Adam:
 
 
 def train_frame(st: FrameState, optimizer: Adam, grads, cam_index: int = 0, rig: bool = False, *, drop: float = 0.0,
-                seed=0) -> dict:
+                seed=None) -> dict:
     """One training step: the frame (of one camera, or of the whole rig) forward and backward, then the
     optimizer's update with whatever clipping it carries. In a regular tiling only the Gaussians that some
     tile can hold are updated (their packed mask from the projection's radii; the others' gradients are

@@ -30,13 +30,14 @@ class _Activate(torch.autograd.Function):
                             None if v_opacities is None else v_opacities.contiguous())
 
 
-def activate_gaussians(log_scales: torch.Tensor, opacity_logits: torch.Tensor, *, drop: float = 0.0, seed=0,
+def activate_gaussians(log_scales: torch.Tensor, opacity_logits: torch.Tensor, *, drop: float = 0.0, seed=None,
                        stream: int = 0):
     """(exp(log_scales), sigmoid(opacity_logits)); log_scales holds three values per opacity logit
     ([N, 3] and [N] or [N, 1]), float32 on the GPU. With ``drop`` each Gaussian's opacity is 0 with that
     probability and the others' are divided by the share kept (they may pass 1, where the compositor's alpha is
-    clamped all the same); ``drop_mask`` of the same drop, seed and stream tells which are kept."""
-    seed, seed_at = seed_arguments(seed)
+    clamped all the same); ``drop_mask`` of the same drop, seed and stream tells which are kept. ``seed``: another for each
+    step, needed where ``drop`` is not 0."""
+    seed, seed_at = seed_arguments(seed, drop, stream)
     if drop == 0:
         return _Activate.apply(log_scales, opacity_logits)
     return _C.activate_drop(log_scales, opacity_logits, float(drop), seed, seed_at, stream)

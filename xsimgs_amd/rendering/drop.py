@@ -11,12 +11,16 @@ import torch
 from .. import _C
 
 
-def seed_arguments(seed):
-    """(the number, the tensor or None)"""
+def seed_arguments(seed, drop: float = 1.0, stream: int = 0):
+    """(the number, the tensor or None). None is refused where something is dropped: a seed that is always the same drops
+    the same places in every step."""
+    if seed is None and not (0 < drop <= 1 and 0 <= stream < 1 << 31):
+        return 0, None         # nothing is drawn, or the probability or the stream is refused behind this
     if isinstance(seed, torch.Tensor):
         return 0, seed
     if isinstance(seed, bool) or not isinstance(seed, int) or not 0 <= seed < 1 << 63:
-        raise ValueError(f"seed must be an int in [0, 2^63) or an int64 tensor of one value, not {seed!r}")
+        raise ValueError("seed must be an int in [0, 2^63) or an int64 tensor of one value, another for each step, "
+                         f"not {seed!r}")
     return seed, None
 
 

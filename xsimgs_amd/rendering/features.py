@@ -9,7 +9,7 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
 def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, *, act: str = "silu", eps: float = 1e-5,
-                   mask=None, drop: float = 0.0, seed=0, stream: int = 0) -> torch.Tensor:
+                   mask=None, drop: float = 0.0, seed=None, stream: int = 0) -> torch.Tensor:
     """``drop(act((x - mean) / sqrt(variance + eps) * weight + bias))`` over each sample and each group of
     consecutive channels of ``x`` ``[batch, ..., channels]`` (float32, bfloat16 or float16 on the GPU; up to 4096
     channels, which ``groups`` divides; one camera's ``[H, W, ch]`` goes in as ``x[None]``). Sums are held in 32 and 64
@@ -17,10 +17,11 @@ def group_norm_act(x: torch.Tensor, groups: int, weight=None, bias=None, *, act:
 
     ``weight``, ``bias``: one value per channel, float32 or of x's type, or None. ``act``: none, relu, silu or gelu (by
     the error function). ``mask``: ``[batch, ...]``, bool; pixels out of it are not read, do not count, and give 0 and
-    no gradient (a sample without any gives zeros). ``drop``, ``seed``, ``stream``: the draws of ``dropout`` on the result."""
+    no gradient (a sample without any gives zeros). ``drop``, ``seed``, ``stream``: the draws of ``dropout`` on the result; a
+    ``seed`` is needed where ``drop`` is not 0, another for each step."""
     if act not in ACTIVATIONS:
         raise ValueError(f"act must be one of {', '.join(ACTIVATIONS)}, not {act!r}")
-    seed, seed_at = seed_arguments(seed)
+    seed, seed_at = seed_arguments(seed, drop, stream)
     return _C.group_norm_act(x, groups, weight, bias, ACTIVATIONS[act], eps, mask, drop, seed, seed_at, stream)
 
 
@@ -44,7 +45,7 @@ class FeatureNorm(torch.nn.Module):
         if drop > 0.0 and seed is None:
             raise ValueError("a FeatureNorm that drops takes another seed in each training step")
         return group_norm_act(x, self.groups, self.weight, self.bias, act=self.act, eps=self.eps, mask=mask, drop=drop,
-                              seed=0 if seed is None else seed, stream=self.stream)
+                              seed=seed, stream=self.stream)
 
     def extra_repr(self):
         return f"{self.groups}, {self.weight.numel()}, act={self.act}, eps={self.eps}, drop={self.drop}"
