@@ -1,9 +1,29 @@
 """What dropout and the feature norm refuse before anything runs: calls that would be answered wrongly in silence."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from xsimgs_amd import rendering
 
+
+CALLS = dict(dropout=lambda x: rendering.dropout(x, 0.5, 1),
+             group_norm_act=lambda x: rendering.group_norm_act(x, 1),
+             weight=lambda x: rendering.group_norm_act(torch.zeros(2, 3, 4), 1, x[0, 0]),
+             bias=lambda x: rendering.group_norm_act(torch.zeros(2, 3, 4), 1, None, x[0, 0]),
+             scales=lambda x: rendering.activate_gaussians(x[0, :, :3], torch.zeros(3), drop=0.5, seed=1)[0],
+             logits=lambda x: rendering.activate_gaussians(torch.zeros(3, 3), x[0, :, 0], drop=0.5, seed=1)[1])
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused(name, requires_grad):
+    """A tangent would be lost: the result would look like a constant."""
+    with fwd.dual_level():
+        x = fwd.make_dual(torch.randn(2, 3, 4), torch.randn(2, 3, 4))
+        if requires_grad:
+            x = x * torch.ones((), requires_grad=True)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            CALLS[name](x)
 
 def test_what_drops_needs_a_seed():
     """Without one the same would be dropped in every step; where nothing is, none is needed."""

@@ -109,3 +109,19 @@ def test_a_frames_head_that_drops_needs_a_seed(dev):
         st.head.eval()
         frame.train_frame(st, opt, grads, rig=rig)
         assert not torch.equal(before[2], st.head.weight.detach())
+
+def test_a_gradients_tangent_is_refused(dev):
+    """A tangent of the incoming gradient alone (a dual parameter behind the operator) would be lost in the backward."""
+    import torch.autograd.forward_ad as fwd
+
+    from xsimgs_amd import rendering
+
+    x = _randn((2, 20, 8), 1, dev).requires_grad_()
+    a, o = _randn((20, 3), 2, dev).requires_grad_(), _randn((20,), 3, dev).requires_grad_()
+    with fwd.dual_level():
+        p = fwd.make_dual(torch.ones((), device=dev), torch.ones((), device=dev))
+        for y, leaf in ((rendering.dropout(x, 0.5, 1), x), (rendering.group_norm_act(x, 2), x),
+                        (rendering.activate_gaussians(a, o, drop=0.5, seed=1)[1], o),
+                        (rendering.activate_gaussians(a, o, drop=0.5, seed=1)[0], a)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y.sum() * p, leaf)

@@ -1082,9 +1082,22 @@ xsg_drop_desc drop_desc(double p, int64_t seed, const OptT& seed_at, int64_t str
                          seed_at.has_value() ? (const uint64_t*)seed_at->data_ptr<int64_t>() : nullptr, (uint32_t)stream};
 }
 
-// Autograd in C++ for these operators: on small tensors the calls through Python would cost more than the kernels.
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
+
+// A tangent would pass these operators by (they are no torch operators, and know no forward mode), and the result would look
+// like a constant. Asked before the autograd function is entered, within which tangents do not show.
+void refuse_tangents(const char* who, std::initializer_list<const OptT*> ts) {
+    for (const OptT* t : ts)
+        TORCH_CHECK(!t->has_value() || !(*t)->defined() || !(*t)->_fw_grad(/*level=*/0).defined(), who,
+                    " has no forward-mode derivative");
+}
+void refuse_tangents(const char* who, const variable_list& grads) {
+    for (const Tensor& g : grads)
+        TORCH_CHECK(!g.defined() || !g._fw_grad(/*level=*/0).defined(), who, "'s gradient has no forward-mode derivative");
+}
+
+// Autograd in C++ for these operators: on small tensors the calls through Python would cost more than the kernels.
 
 bool wants_grad(std::initializer_list<const OptT*> ts) {
     if (!at::GradMode::is_enabled()) return false;
@@ -1144,6 +1157,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
         return dropout_values(x, p, seed, seed_at, stream, shared);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_tangents("dropout", grads);
         const KeptDraws k(ctx);
         const auto saved = ctx->get_saved_variables();
         const Tensor v_x = dropout_values(grads[0], k.p, k.seed, optional(saved[0]), k.stream, ctx->saved_data["shared"].toInt());
@@ -1153,6 +1167,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor& x, double p, int64_t seed, const OptT& seed_at, int64_t stream, int64_t shared) {
     const OptT ox(x);
+    refuse_tangents("dropout", {&ox});
     if (wants_grad({&ox})) return Dropout::apply(x, seed_at, p, seed, stream, shared);
     return dropout_values(x, p, seed, seed_at, stream, shared);
 }
@@ -1187,6 +1202,7 @@ struct ActivateDrop : torch::autograd::Function<ActivateDrop> {
         return {scales, opacities};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_tangents("activate_gaussians", grads);
         const KeptDraws k(ctx);
         const auto saved = ctx->get_saved_variables();
         const Tensor &scales = saved[0], o = saved[1].contiguous();
@@ -1208,6 +1224,8 @@ struct ActivateDrop : torch::autograd::Function<ActivateDrop> {
 
 std::tuple<Tensor, Tensor> activate_drop(const Tensor& log_scales, const Tensor& opacity_logits, double p, int64_t seed,
                                          const OptT& seed_at, int64_t stream) {
+    const OptT scales(log_scales), logits(opacity_logits);
+    refuse_tangents("activate_gaussians", {&scales, &logits});
     const auto out = ActivateDrop::apply(log_scales, opacity_logits, seed_at, p, seed, stream);
     return {out[0], out[1]};
 }
@@ -1283,6 +1301,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_tangents("group_norm_act", grads);
         const KeptDraws k(ctx);
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[5];
@@ -1314,6 +1333,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 Tensor group_norm_act(const Tensor& x, int64_t groups, const OptT& weight, const OptT& bias, int64_t act, double eps,
                       const OptT& mask, double p, int64_t seed, const OptT& seed_at, int64_t stream) {
     const OptT ox(x);
+    refuse_tangents("group_norm_act", {&ox, &weight, &bias});
     if (wants_grad({&ox, &weight, &bias}))
         return GroupNormAct::apply(x, weight, bias, mask, seed_at, groups, act, eps, p, seed, stream);
     return std::get<0>(group_norm_values(NormCall(x, groups, weight, bias, act, eps, mask, p, seed, seed_at, stream), x));
