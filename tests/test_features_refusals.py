@@ -25,6 +25,14 @@ def test_forward_mode_is_refused(name, requires_grad):
         with pytest.raises(RuntimeError, match="forward-mode"):
             CALLS[name](x)
 
+@pytest.mark.parametrize("name", [*CALLS, "drop_mask"])
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_tracing_is_refused(name, requires_grad):
+    """A trace would record the result's allocation alone, and replay memory that nothing has written."""
+    call = CALLS.get(name, lambda x: x.sum() + rendering.drop_mask(8, 0.5, 1, device="cpu").sum())
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(call, (torch.randn(2, 3, 4, requires_grad=requires_grad),), check_trace=False)
+
 def test_what_drops_needs_a_seed():
     """Without one the same would be dropped in every step; where nothing is, none is needed."""
     from xsimgs_amd import frame

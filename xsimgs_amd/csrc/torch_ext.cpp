@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/util/SmallVector.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -1097,6 +1098,9 @@ void refuse_tangents(const char* who, const variable_list& grads) {
         TORCH_CHECK(!g.defined() || !g._fw_grad(/*level=*/0).defined(), who, "'s gradient has no forward-mode derivative");
 }
 
+// A trace would record the allocation of the results alone: its replays would return memory that nothing has written.
+void refuse_tracing(const char* who) { TORCH_CHECK(!torch::jit::tracer::isTracing(), who, " cannot be traced"); }
+
 // Autograd in C++ for these operators: on small tensors the calls through Python would cost more than the kernels.
 
 bool wants_grad(std::initializer_list<const OptT*> ts) {
@@ -1167,12 +1171,14 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor& x, double p, int64_t seed, const OptT& seed_at, int64_t stream, int64_t shared) {
     const OptT ox(x);
+    refuse_tracing("dropout");
     refuse_tangents("dropout", {&ox});
     if (wants_grad({&ox})) return Dropout::apply(x, seed_at, p, seed, stream, shared);
     return dropout_values(x, p, seed, seed_at, stream, shared);
 }
 
 Tensor drop_mask(int64_t n, double p, int64_t seed, const OptT& seed_at, int64_t stream, const c10::Device& device) {
+    refuse_tracing("drop_mask");
     TORCH_CHECK(n >= 0, "n must not be negative");
     TORCH_CHECK(device.is_cuda(), "xsimgs_amd ops take GPU tensors (got the device ", device, ")");
     Tensor out = at::empty({(n + 31) / 32}, at::TensorOptions().device(device).dtype(at::kUInt32));
@@ -1225,6 +1231,7 @@ struct ActivateDrop : torch::autograd::Function<ActivateDrop> {
 std::tuple<Tensor, Tensor> activate_drop(const Tensor& log_scales, const Tensor& opacity_logits, double p, int64_t seed,
                                          const OptT& seed_at, int64_t stream) {
     const OptT scales(log_scales), logits(opacity_logits);
+    refuse_tracing("activate_gaussians");
     refuse_tangents("activate_gaussians", {&scales, &logits});
     const auto out = ActivateDrop::apply(log_scales, opacity_logits, seed_at, p, seed, stream);
     return {out[0], out[1]};
@@ -1333,6 +1340,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 Tensor group_norm_act(const Tensor& x, int64_t groups, const OptT& weight, const OptT& bias, int64_t act, double eps,
                       const OptT& mask, double p, int64_t seed, const OptT& seed_at, int64_t stream) {
     const OptT ox(x);
+    refuse_tracing("group_norm_act");
     refuse_tangents("group_norm_act", {&ox, &weight, &bias});
     if (wants_grad({&ox, &weight, &bias}))
         return GroupNormAct::apply(x, weight, bias, mask, seed_at, groups, act, eps, p, seed, stream);
