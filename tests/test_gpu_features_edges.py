@@ -125,3 +125,14 @@ def test_a_gradients_tangent_is_refused(dev):
                         (rendering.activate_gaussians(a, o, drop=0.5, seed=1)[0], a)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(y.sum() * p, leaf)
+
+def test_gradients_of_a_dropout_that_depend_on_nothing(dev):
+    """Dropout is linear: its gradient depends on the incoming gradient alone, and where that is a constant so is it. A
+    penalty on it beside other terms is differentiated as usual."""
+    from xsimgs_amd import rendering
+
+    x = _randn((50, 8), 1, dev).requires_grad_()
+    g, = torch.autograd.grad(rendering.dropout(x, 0.5, 1).sum(), x, create_graph=True)
+    assert not g.requires_grad
+    again, = torch.autograd.grad((g * x).sum(), x)
+    assert torch.equal(again, g)

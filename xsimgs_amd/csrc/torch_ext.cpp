@@ -1114,9 +1114,9 @@ OptT optional(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 Tensor defined_or_not(const OptT& t) { return t.value_or(Tensor()); }
 
 // Gradients that are asked for with a graph of their own (create_graph) raise when that is followed to what they were
-// made of.
+// made of; made of constants alone (a dropout's gradient of a sum), they are constants.
 template <typename... Ts> variable_list differentiated_once(variable_list grads, const char* who, const Ts&... made_of) {
-    if (!at::GradMode::is_enabled()) return grads;
+    if (!torch::autograd::compute_requires_grad(made_of...)) return grads;
     const auto error = std::make_shared<torch::autograd::Error>(std::string(who) + " is differentiated once",
                                                                 torch::autograd::collect_next_edges(made_of...));
     for (auto& g : grads)
