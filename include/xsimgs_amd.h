@@ -283,7 +283,7 @@ int xsg_activate_drop_bwd(const xsg_drop_desc* drop, int64_t n, const float* sca
 /* Group norm of feature images, channels last, with an activation and dropout behind it: over each sample and
  * each group of channels / groups consecutive channels, with mean and (biased) variance over the pixels in the
  * mask, y = drop(act((x - mean) / sqrt(variance + eps) weight + bias)). Pixels out of the mask are not read; y
- * and v_x are 0 there. Up to 2^23 - 1 workgroups, so no more samples. Results are the same bits on every call. */
+ * and v_x are 0 there. Up to 2^23 - 1 samples. Results are the same bits on every call. */
 typedef struct {
     int dtype;                        /* of x, y and their gradients */
     int64_t batch, pixels;

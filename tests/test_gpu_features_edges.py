@@ -136,3 +136,46 @@ def test_gradients_of_a_dropout_that_depend_on_nothing(dev):
     assert not g.requires_grad
     again, = torch.autograd.grad((g * x).sum(), x)
     assert torch.equal(again, g)
+
+def test_the_most_samples(dev):
+    """2^23 - 1 samples forward and backward; one more is refused in both."""
+    from xsimgs_amd import rendering
+
+    n = 2 ** 23 - 1
+    x, v_y = torch.randn((n, 2), device=dev), torch.randn((n, 2), device=dev)
+    w, b = _params(2, 5, dev)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = rendering.group_norm_act(leaves[0], 1, *leaves[1:])
+    v_x, v_w, v_b = torch.autograd.grad(y, leaves, v_y)
+    for at in (slice(0, 500), slice(n // 2, n // 2 + 500), slice(n - 500, n)):
+        some = _run(x[at], 1, w, b, v_y=v_y[at])
+        assert torch.equal(y[at].detach(), some["y"]) and torch.equal(v_x[at], some["v_x"])
+    xd = x.double()
+    xh = (xd - xd.mean(1, keepdim=True)) / (xd.var(1, correction=0, keepdim=True) + 1e-5).sqrt()
+    z = xh * w.double() + b.double()
+    s = torch.sigmoid(z)
+    dz = v_y.double() * s * (1 + z * (1 - s))
+    # per term 132 U of xh (5e3 U where the spread is smaller than sqrt(eps): |mean| rstd) and 80 U of its own; sums in 64 bits
+    for got, terms in ((v_b, dz), (v_w, dz * xh)):
+        loose = (v_y.double().abs() * (1 + x.double().abs().amax(1, keepdim=True) * 320)).sum(0)
+        assert bool(((got.double() - terms.sum(0)).abs() <= 400 * 2.0 ** -24 * loose).all())
+    with pytest.raises(RuntimeError, match="too many samples"):
+        rendering.group_norm_act(torch.zeros(n + 1, 2, device=dev), 1)
+
+
+def test_more_groups_than_a_launch_has_workgroups(dev):
+    """2049 samples of 4096 groups are more than 2^23: the launches that join their parts take several in turn. The samples
+    repeat, so each gives what it gives in a call of 64."""
+    from xsimgs_amd import rendering
+
+    w, b = (t.to(torch.bfloat16) for t in _params(4096, 5, dev))
+    for pixels in (3, 260):      # a forward in one launch, and in several
+        one, g = _randn((1, pixels, 4096), 1, dev, torch.bfloat16), _randn((1, pixels, 4096), 2, dev, torch.bfloat16)
+        want = _run(one, 4096, w, b, v_y=g)
+        x = one.expand(2049, pixels, 4096).detach().requires_grad_()
+        y = rendering.group_norm_act(x, 4096, w, b)
+        v_x, = torch.autograd.grad(y, x, g.expand(x.shape))
+        for got, name in ((y, "y"), (v_x, "v_x")):
+            off = (got.detach().float() - want[name].float()).abs()
+            assert bool((off <= 2.0 ** -7 * want[name].float().abs() + 1e-6).all())
+            assert bool((got[1:] == got[:1]).all())

@@ -133,21 +133,25 @@ XSG_DEV void add_parts(const float2* __restrict__ part, int columns, int64_t par
     }
 }
 
-// One workgroup to a group of a sample: the means of weight dz and weight dz xh, sums in 64 bits.
-__global__ __launch_bounds__(256) void norm_means_kernel(int groups, int chunks, const float4* __restrict__ stats,
+// One workgroup to a group of a sample, or to several in turn: the means of weight dz and weight dz xh, sums in 64 bits.
+__global__ __launch_bounds__(256) void norm_means_kernel(int64_t all, int groups, int chunks, const float4* __restrict__ stats,
                                                          const float2* __restrict__ part, float2* __restrict__ means) {
     __shared__ double s_x[4], s_y[4];
-    const float2* const p = part + blockIdx.x / groups * (int64_t)chunks * groups + blockIdx.x % groups;
-    double x = 0.0, y = 0.0;
-    add_parts(p, groups, chunks, threadIdx.x, 256, x, y);
-    x = segment_sum(x, 64);
-    y = segment_sum(y, 64);
-    if ((threadIdx.x & 63) == 0) { s_x[threadIdx.x >> 6] = x; s_y[threadIdx.x >> 6] = y; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const double inv = stats[blockIdx.x].z;
-        means[blockIdx.x] = make_float2((float)((s_x[0] + s_x[1] + s_x[2] + s_x[3]) * inv),
-                                        (float)((s_y[0] + s_y[1] + s_y[2] + s_y[3]) * inv));
+    for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
+        const int64_t b = i / groups;
+        const float2* const p = part + b * chunks * groups + (i - b * groups);
+        double x = 0.0, y = 0.0;
+        add_parts(p, groups, chunks, threadIdx.x, 256, x, y);
+        x = segment_sum(x, 64);
+        y = segment_sum(y, 64);
+        if ((threadIdx.x & 63) == 0) { s_x[threadIdx.x >> 6] = x; s_y[threadIdx.x >> 6] = y; }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const double inv = stats[i].z;
+            means[i] = make_float2((float)((s_x[0] + s_x[1] + s_x[2] + s_x[3]) * inv),
+                                   (float)((s_y[0] + s_y[1] + s_y[2] + s_y[3]) * inv));
+        }
+        __syncthreads();
     }
 }
 
@@ -285,7 +289,7 @@ extern "C" int xsg_group_norm_act_bwd(const xsg_norm_desc* d, const float* stats
     const int vector = norm_vector(d, true), size = d->dtype == XSG_DTYPE_F32 ? 4 : 2;
     norm_layout(a, vector, norm_grad_unroll(vector * size), size, 3, 256);
     const int tiles = (a.channels + 7) / 8;
-    if (a.batch * a.chunks + tiles > kNormBlocks || (!a.join && a.batch * a.groups > kNormBlocks))
+    if (a.batch * a.chunks > kNormBlocks)
         return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: too many samples (%lld)", (long long)a.batch);
     const int64_t parts = a.batch * a.chunks;
     float2* const groups = (float2*)workspace;
@@ -301,12 +305,13 @@ extern "C" int xsg_group_norm_act_bwd(const xsg_norm_desc* d, const float* stats
                 const unsigned threads = norm_threads(a);
                 norm_sums_kernel<DT, V, ACT, DROP, MASK><<<(unsigned)parts, threads, sizeof(float2) * (V * threads + a.channels), s>>>(
                     a, st, v_y, v_x ? groups : nullptr, params ? channels : nullptr);
-                if (!v_x) {
-                    norm_params_kernel<<<(unsigned)tiles, 256, 0, s>>>(parts, a.channels, channels, v_weight, v_bias);
-                    return;
-                }
-                if (!a.join) norm_means_kernel<<<(unsigned)(a.batch * a.groups), 256, 0, s>>>(a.groups, a.chunks, st, groups, means);
-                const int param_blocks = params ? tiles : 0;
+                // in a launch of their own where that of v_x has no workgroups left for them
+                const bool apart = params && (!v_x || parts + tiles > kNormBlocks);
+                if (apart) norm_params_kernel<<<(unsigned)tiles, 256, 0, s>>>(parts, a.channels, channels, v_weight, v_bias);
+                if (!v_x) return;
+                if (!a.join)
+                    norm_means_kernel<<<norm_join_blocks(a), 256, 0, s>>>(a.batch * a.groups, a.groups, a.chunks, st, groups, means);
+                const int param_blocks = params && !apart ? tiles : 0;
                 const unsigned grid = (unsigned)parts + param_blocks;
                 const size_t lds = a.join ? sizeof(float2) * a.groups : 0;
                 if (norm_may_stream<DT, V>() && a.stream)

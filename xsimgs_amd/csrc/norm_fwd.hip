@@ -193,30 +193,35 @@ struct NormSums {
     }
 };
 
-// One workgroup to a group of a sample (1080p x 64: 4.7 us, as long as a launch takes).
+// One workgroup to a group of a sample (1080p x 64: 4.7 us, as long as a launch takes), or to several in turn where a launch
+// does not have as many.
 template <bool MASK>
-__global__ __launch_bounds__(256) void norm_join_kernel(int groups, int chunks, float eps, const float2* __restrict__ part,
-                                                        const float* __restrict__ counts, float4* __restrict__ stats) {
+__global__ __launch_bounds__(256) void norm_join_kernel(int64_t all, int groups, int chunks, float eps,
+                                                        const float2* __restrict__ part, const float* __restrict__ counts,
+                                                        float4* __restrict__ stats) {
     __shared__ double s_sum[4][4];
-    const int64_t b = blockIdx.x / groups;
-    const float2* const p = part + b * chunks * groups + blockIdx.x % groups;
-    const float* const c = counts + b * chunks;
-    const float about = NormSums::about<MASK>(p, c, groups, chunks, threadIdx.x & 63, 64);   // the same in each wavefront
-    NormSums sum;
-    sum.add_parts(p, c, groups, chunks, threadIdx.x, 256, about);
-    double* const mine = s_sum[threadIdx.x >> 6];
-    const double n = segment_sum(sum.n, 64), s1 = segment_sum(sum.s1, 64), s2 = segment_sum(sum.s2, 64), d = segment_sum(sum.d, 64);
-    if ((threadIdx.x & 63) == 0) { mine[0] = n; mine[1] = s1; mine[2] = s2; mine[3] = d; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        NormSums all;
-        for (int w = 0; w < 4; ++w) {
-            all.n += s_sum[w][0];
-            all.s1 += s_sum[w][1];
-            all.s2 += s_sum[w][2];
-            all.d += s_sum[w][3];
+    for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
+        const int64_t b = i / groups;
+        const float2* const p = part + b * chunks * groups + (i - b * groups);
+        const float* const c = counts + b * chunks;
+        const float about = NormSums::about<MASK>(p, c, groups, chunks, threadIdx.x & 63, 64);   // the same in each wavefront
+        NormSums sum;
+        sum.add_parts(p, c, groups, chunks, threadIdx.x, 256, about);
+        double* const mine = s_sum[threadIdx.x >> 6];
+        const double n = segment_sum(sum.n, 64), s1 = segment_sum(sum.s1, 64), s2 = segment_sum(sum.s2, 64), d = segment_sum(sum.d, 64);
+        if ((threadIdx.x & 63) == 0) { mine[0] = n; mine[1] = s1; mine[2] = s2; mine[3] = d; }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            NormSums all_sums;
+            for (int w = 0; w < 4; ++w) {
+                all_sums.n += s_sum[w][0];
+                all_sums.s1 += s_sum[w][1];
+                all_sums.s2 += s_sum[w][2];
+                all_sums.d += s_sum[w][3];
+            }
+            stats[i] = all_sums.stats(about, eps);
         }
-        stats[blockIdx.x] = all.stats(about, eps);
+        __syncthreads();
     }
 }
 
@@ -411,7 +416,7 @@ extern "C" int xsg_group_norm_act_fwd(const xsg_norm_desc* d, void* y, float* st
     }
     const int size = d->dtype == XSG_DTYPE_F32 ? 4 : 2, vector = norm_vector(d, false), draw_vector = norm_vector(d, true);
     norm_layout(a, vector, kStatsUnroll, size, 2, 512);
-    if (a.batch * a.chunks > kNormBlocks || (!a.join && a.batch * a.groups > kNormBlocks))
+    if (a.batch * a.chunks > kNormBlocks)
         return xsg_fail(XSG_ERR_INVALID, "group_norm_act_fwd: too many samples (%lld)", (long long)a.batch);
     const hipStream_t s = (hipStream_t)stream;
     float2* const part = (float2*)workspace;
@@ -433,8 +438,8 @@ extern "C" int xsg_group_norm_act_fwd(const xsg_norm_desc* d, void* y, float* st
             else stats_pass(std::false_type{});
         });
         if (!a.join)
-            (a.mask ? norm_join_kernel<true> : norm_join_kernel<false>)<<<(unsigned)(a.batch * a.groups), 256, 0, s>>>(
-                a.groups, chunks, a.eps, part, counts, (float4*)stats);
+            (a.mask ? norm_join_kernel<true> : norm_join_kernel<false>)<<<norm_join_blocks(a), 256, 0, s>>>(
+                a.batch * a.groups, a.groups, chunks, a.eps, part, counts, (float4*)stats);
         const int join = a.join;
         norm_layout(a, draw_vector, norm_apply_unroll(draw_vector * size), size, 2, 256);
         a.join = join;

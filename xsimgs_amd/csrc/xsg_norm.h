@@ -212,6 +212,8 @@ constexpr int norm_grad_unroll(int) { return 2; }
 constexpr bool norm_ahead(int bytes) { return bytes <= 16; }
 // The forward in one launch, where a sample's groups fit workgroups; false where they do not.
 bool norm_small(const xsg_norm_desc* d, const NormArgs& a, void* y, float* stats, hipStream_t s);
+// of the launches that join parts, one to a group of a sample
+inline unsigned norm_join_blocks(const NormArgs& a) { return (unsigned)(a.batch * a.groups < kNormBlocks ? a.batch * a.groups : kNormBlocks); }
 inline unsigned norm_threads(const NormArgs& a) { return (unsigned)((a.tx * a.ty + 63) / 64 * 64); }
 
 template <typename F> void with_norm_flags(const xsg_norm_desc* d, const NormArgs& a, F&& f) {
