@@ -10,7 +10,6 @@
 
 namespace {
 
-
 // A batch of U pixels of x and of v_y.
 template <int DT, int V, int U, bool MASK> struct GradBatch {
     typedef Raw<V * ElementSize<DT>::value> Vec;
@@ -31,7 +30,7 @@ template <int DT, int V, int ACT, bool DROP, bool MASK>
 __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormArgs a, const float4* __restrict__ stats,
                                                                  const void* __restrict__ v_y, float2* __restrict__ groups,
                                                                  float2* __restrict__ channels) {
-    constexpr int U = norm_grad_unroll(V * ElementSize<DT>::value);
+    constexpr int U = kNormGradUnroll;
     constexpr bool AHEAD = norm_ahead(V * ElementSize<DT>::value);
     constexpr bool EXACT = DT == XSG_DTYPE_F32;
     extern __shared__ float2 s_sums[];   // [threads][V], then [channels]
@@ -184,7 +183,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_kernel(NormArgs a, int
                                                                  const float2* __restrict__ means,
                                                                  const float2* __restrict__ channels, void* __restrict__ v_x,
                                                                  float* __restrict__ v_weight, float* __restrict__ v_bias) {
-    constexpr int U = norm_grad_unroll(V * ElementSize<DT>::value);
+    constexpr int U = kNormGradUnroll;
     constexpr bool AHEAD = norm_ahead(V * ElementSize<DT>::value);
     constexpr bool EXACT = DT == XSG_DTYPE_F32;
     if ((int)blockIdx.x < param_blocks)
@@ -244,7 +243,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_kernel(NormArgs a, int
                 float x[V], g[V];
                 unpack<DT, V>(now.x[u], x);
                 if (DROP) drawn.mask(now.g[u]);
-            unpack<DT, V>(now.g[u], g);
+                unpack<DT, V>(now.g[u], g);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float e = x[j] - mean[j];
@@ -287,7 +286,7 @@ extern "C" int xsg_group_norm_act_bwd(const xsg_norm_desc* d, const float* stats
     if (const int rc = xsg_check_workspace(workspace, "group_norm_act_bwd")) return rc;
     if ((uintptr_t)stats % 16) return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: stats must be 16-byte aligned");
     const int vector = norm_vector(d, true), size = d->dtype == XSG_DTYPE_F32 ? 4 : 2;
-    norm_layout(a, vector, norm_grad_unroll(vector * size), size, 3, 256);
+    norm_layout(a, vector, kNormGradUnroll, size, 3, 256);
     const int tiles = (a.channels + 7) / 8;
     if (a.batch * a.chunks > kNormBlocks)
         return xsg_fail(XSG_ERR_INVALID, "group_norm_act_bwd: too many samples (%lld)", (long long)a.batch);

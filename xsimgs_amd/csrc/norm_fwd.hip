@@ -193,7 +193,7 @@ struct NormSums {
     }
 };
 
-// One workgroup to a group of a sample (1080p x 64: 4.7 us, as long as a launch takes), or to several in turn where a launch
+// One workgroup to a group of a sample (1080p x 64: 5 us, as long as a launch takes), or to several in turn where a launch
 // does not have as many.
 template <bool MASK>
 __global__ __launch_bounds__(256) void norm_join_kernel(int64_t all, int groups, int chunks, float eps,
@@ -397,7 +397,7 @@ extern "C" size_t xsg_group_norm_act_workspace_bytes(const xsg_norm_desc* d, int
     NormArgs a;
     if (norm_args(d, a, "group_norm_act") != XSG_OK || d->batch == 0 || d->pixels == 0) return 0;
     const int vector = norm_vector(d, backward != 0), size = d->dtype == XSG_DTYPE_F32 ? 4 : 2;
-    norm_layout(a, vector, backward ? norm_grad_unroll(vector * size) : kStatsUnroll, size, 0, backward ? 256 : 512);
+    norm_layout(a, vector, backward ? kNormGradUnroll : kStatsUnroll, size, 0, backward ? 256 : 512);
     const size_t parts = (size_t)(a.batch * a.chunks);
     if (backward) return sizeof(float2) * (parts * (size_t)(a.channels + a.groups) + (size_t)(a.batch * a.groups));
     return sizeof(float2) * parts * (size_t)a.groups + sizeof(float) * parts;

@@ -3,8 +3,12 @@
 // to a pixel, V consecutive channels each, and ty pixels side by side, so that its accesses are one run of memory.
 //
 // All of it is bound by memory where images are large and nothing is drawn: x is read for its statistics and again for the
-// result, x and v_y for their sums and again for v_x, at 5.3 to 6.2 TB/s (1080p x 64 bfloat16, silu: statistics 46 us,
-// result 85, sums 96, v_x 140). With draws the vector units are (225 x 400 x 128 x 6 float16: 58, 69 and 78 us).
+// result, x and v_y for their sums and again for v_x, at 5.3 to 6.2 TB/s (1080p x 64 bfloat16, silu: statistics 48 us,
+// result 87, sums 94, v_x 140). Draws hold back the result and the sums (225 x 400 x 128 x 6 float16: 56 us, 4.9 TB/s, and
+// 66, 4.2; v_x stays at the memory's rate, 76, 5.5 TB/s). A mask in front of short passes with draws does too: its bytes come
+// before the loads that they decide on (128 x 2048 x 65 float32, gelu: result 38, sums 42, v_x 43 us, 2.6 to 4.1 TB/s, at
+// 330 to 360 vector instructions a microsecond and SIMD of about 540 that other kernels here reach, with waves waiting 40 to
+// 48 % of their time; a training pass of the whole takes 139 us, 133 without the mask, 109 without draws).
 #pragma once
 #include "xsg_elements.h"
 #include "xsg_random.h"
@@ -57,7 +61,7 @@ template <bool EXACT> XSG_DEV float norm_sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
 // The normal distribution function and exp(-z^2 / 2). With t = 1 / (1 + 0.29 |z|), the tail is exp(-z^2 / 2) times a
-// polynomial in t of degree 8 (a least-squares fit of erfc(x) exp(x^2) / 2, weighted towards the least largest error: 2e-9
+// polynomial in t of degree 8 (a least-squares fit of erfc(x) exp(x^2) / 2, weighted towards the least largest error: 8e-9
 // of the function, 2e-7 with its roundings); relative to the tail itself it stays within 1e-6 down to z = -3, where
 // 1 + erf has lost that. Without branches, and both functions share the exponential.
 XSG_DEV float norm_phi(float z, float& e) {
@@ -208,7 +212,7 @@ template <int DT, int V> constexpr bool norm_may_stream() { return V * ElementSi
 // Pixels in flight in a thread, with the next as many on their way where vectors are of 16 bytes (a rig's blocks of 69 M
 // values with draws: 213 us the three passes, 226 without; wider ones run out of registers by it: 135 and 121 us)
 constexpr int norm_apply_unroll(int bytes) { return bytes > 16 ? 2 : 4; }
-constexpr int norm_grad_unroll(int) { return 2; }
+constexpr int kNormGradUnroll = 2;
 constexpr bool norm_ahead(int bytes) { return bytes <= 16; }
 // The forward in one launch, where a sample's groups fit workgroups; false where they do not.
 bool norm_small(const xsg_norm_desc* d, const NormArgs& a, void* y, float* stats, hipStream_t s);
